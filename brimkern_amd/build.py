@@ -1,9 +1,10 @@
 """Build recipe for the native parts of brimkern_amd (no cmake / node-gyp needed).
 
 1. ``csrc/kernels/brik_kernels.hip`` -> ``_build/brik_gfx950.hsaco``  (hipcc --genco, gfx950 only), then
-   ``check_lds_reads.py`` on its disassembly (the GEMM's inline-asm LDS reads)
+   ``check_lds_reads.py`` on its disassembly (the GEMM's inline-asm LDS reads); beside it
+   ``csrc/kernels/brik_attn_kernels.hip`` -> ``_build/brik_attn_gfx950.hsaco`` (the attention side)
 2. ``csrc/brik_scratch.hip`` -> ``_build/brik_scratch.o`` (hipcc -c: the no-allocation scratch array)
-3. ``csrc/brik_runtime.cpp`` + ``csrc/brik_embed.S`` (embeds the code object) + that object ->
+3. ``csrc/brik_runtime.cpp`` + ``csrc/brik_embed.S`` (embeds the code objects) + that object ->
    ``libbrik.so`` (the C ABI declared in ``include/brik.h``)
 4. ``csrc/brik_napi.cc`` -> ``js/brik.node`` (Node N-API addon over libbrik.so, rpath $ORIGIN/..)
 5. ``tests/native/host_sanitize.cpp`` + the runtime sources, host code built with AddressSanitizer and
@@ -14,6 +15,7 @@ Run ``python -m brimkern_amd.build`` or call :func:`build`.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -26,6 +28,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 NODE_INC = "/usr/include/node"
 
 HSACO = os.path.join(BUILD, "brik_gfx950.hsaco")
+ATTN_HSACO = os.path.join(BUILD, "brik_attn_gfx950.hsaco")
 SCRATCH_OBJ = os.path.join(BUILD, "brik_scratch.o")
 LIB = os.path.join(PKG, "libbrik.so")
 ADDON = os.path.join(PKG, "js", "brik.node")
@@ -51,14 +54,21 @@ def _run(cmd, verbose):
     subprocess.check_call(cmd)
 
 
-def build_hsaco(verbose=False):
+def _genco(src, out, extra, verbose):
     os.makedirs(BUILD, exist_ok=True)
-    src = os.path.join(CSRC, "kernels", "brik_kernels.hip")
-    tmp = HSACO + ".tmp"
-    _run([os.path.join(ROCM, "bin", "hipcc"), "--genco", "--no-gpu-bundle-output", *HIP_DEVICE_FLAGS,
-          "-Xoffload-linker", f"--section-start=.text={TEXT_ADDR:#x}", "-o", tmp, src], verbose)
-    os.replace(tmp, HSACO)
-    return HSACO
+    tmp = out + ".tmp"
+    _run([os.path.join(ROCM, "bin", "hipcc"), "--genco", "--no-gpu-bundle-output", *HIP_DEVICE_FLAGS, *extra, "-o", tmp,
+          os.path.join(CSRC, "kernels", src)], verbose)
+    os.replace(tmp, out)
+    return out
+
+
+def build_hsaco(verbose=False):
+    return _genco("brik_kernels.hip", HSACO, ["-Xoffload-linker", f"--section-start=.text={TEXT_ADDR:#x}"], verbose)
+
+
+def build_attn_hsaco(verbose=False):
+    return _genco("brik_attn_kernels.hip", ATTN_HSACO, [], verbose)
 
 
 def build_scratch(verbose=False):
@@ -76,7 +86,7 @@ def build_lib(verbose=False):
     tmp = LIB + ".tmp"
     _run(["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", "-Wextra",
           "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROCM, "include"),
-          f'-DBRIK_HSACO_PATH="{HSACO}"',
+          f'-DBRIK_HSACO_PATH="{HSACO}"', f'-DBRIK_ATTN_HSACO_PATH="{ATTN_HSACO}"',
           os.path.join(CSRC, "brik_runtime.cpp"), os.path.join(CSRC, "brik_embed.S"), SCRATCH_OBJ,
           "-L", os.path.join(ROCM, "lib"), "-lamdhip64", f"-Wl,-rpath,{os.path.join(ROCM, 'lib')}",
           "-Wl,--no-undefined", "-o", tmp], verbose)
@@ -106,7 +116,7 @@ def build_host_sanitize(verbose=False):
         _run(["g++", "-O1", "-g", "-std=c++17", "-Wall", "-Wextra", "-fno-omit-frame-pointer",
               "-fsanitize=address,undefined", "-fno-sanitize-recover=undefined", "-static-libasan",
               "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROCM, "include"), "-I", os.path.join(ROOT, "include"),
-              f'-DBRIK_HSACO_PATH="{HSACO}"', SANITIZE_SRC,
+              f'-DBRIK_HSACO_PATH="{HSACO}"', f'-DBRIK_ATTN_HSACO_PATH="{ATTN_HSACO}"', SANITIZE_SRC,
               os.path.join(CSRC, "brik_runtime.cpp"), os.path.join(CSRC, "brik_embed.S"), SCRATCH_OBJ,
               "-L", os.path.join(ROCM, "lib"), "-lamdhip64", f"-Wl,-rpath,{os.path.join(ROCM, 'lib')}",
               "-o", tmp], verbose)
@@ -130,9 +140,10 @@ def check_hsaco(verbose=False):
 
 
 def build(verbose=False):
-    build_hsaco(verbose)
+    with concurrent.futures.ThreadPoolExecutor(3) as pool:        # three compilers side by side
+        for job in [pool.submit(f, verbose) for f in (build_hsaco, build_attn_hsaco, build_scratch)]:
+            job.result()
     check_hsaco(verbose)
-    build_scratch(verbose)
     build_lib(verbose)
     build_addon(verbose)
     build_host_sanitize(verbose)

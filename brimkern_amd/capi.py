@@ -78,6 +78,10 @@ SIGNATURES = {
     "brik_lm_head_topk_q4": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _I, ctypes.c_float, ctypes.c_float, _I, _P, _P]),
     "brik_lm_head_topk_q3": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _P, _I, ctypes.c_float, ctypes.c_float, _I, _P,
                                   _P]),
+    "brik_qk_norm_rope": (_I, [_P, _P, _P]),
+    "brik_kv_write": (_I, [_P, _P, _P, _P]),
+    "brik_kv_read": (_I, [_P, _P, _P, _P, _P]),
+    "brik_attention": (_I, [_P, _P, _P, _P]),
 }
 BRIK_TOPK_MAX = 64
 BRIK_NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -99,6 +103,38 @@ class GemvJobEx(ctypes.Structure):
 
 
 BRIK_JOB_GAIN_ONE_PLUS, BRIK_JOB_ACT_GELU = 1, 2
+
+
+_I32, _I64, _F32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+
+
+class KvCache(ctypes.Structure):
+    """``brik_kv_cache`` of include/brik.h."""
+    _fields_ = [("fmt", _I32), ("heads", _I32), ("head_dim", _I32), ("page", _I32), ("pages", _I32), ("reserved", _I32),
+                ("k", _P), ("v", _P), ("k_scales", _P), ("v_scales", _P), ("k_mins", _P), ("v_mins", _P)]
+
+
+class KvBatch(ctypes.Structure):
+    """``brik_kv_batch`` of include/brik.h."""
+    _fields_ = [("seqs", _I32), ("rows", _I32), ("row_off", _P), ("kv_len", _P), ("table", _P), ("table_cols", _I32),
+                ("max_len", _I32), ("max_rows", _I32), ("prefix_len", _I32), ("prefix_table", _P)]
+
+
+class QkvRows(ctypes.Structure):
+    """``brik_qkv_rows`` of include/brik.h."""
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_out", _P), ("k_out", _P), ("q_stride", _I64), ("k_stride", _I64),
+                ("v_stride", _I64), ("q_out_stride", _I64), ("k_out_stride", _I64), ("q_norm", _P), ("k_norm", _P),
+                ("inv_freq", _P), ("positions", _P), ("heads", _I32), ("kv_heads", _I32), ("head_dim", _I32),
+                ("rot_dim", _I32), ("flags", _I32), ("eps", _F32)]
+
+
+class AttnArgs(ctypes.Structure):
+    """``brik_attn_args`` of include/brik.h."""
+    _fields_ = [("q", _P), ("out", _P), ("q_stride", _I64), ("out_stride", _I64), ("heads", _I32), ("window", _I32),
+                ("scale", _F32), ("softcap", _F32)]
+
+
+BRIK_QKV_GAIN_ONE_PLUS, BRIK_QKV_INTERLEAVED = 1, 2
 
 
 class BrikError(RuntimeError):
@@ -354,6 +390,53 @@ class Context:
         tail = (K, vocab, _addr(recent), n_recent, penalty, softcap, k, _addr(ids), _addr(vals))
         fn = getattr(self.lib, f"brik_lm_head_topk_{fmt}")
         self._check(fn(self.handle, _addr(x), *[_addr(p) for p in planes], *tail))
+
+    # ---- the attention side of a decoder layer -------------------------------------------------
+    # The structures below are made once and used in every step: they hold addresses, not contents.
+    @staticmethod
+    def kv_cache(fmt: str, heads, head_dim, page, pages, k, v) -> KvCache:
+        """A paged cache over the planes of ``k`` and ``v``: q8 (codes, sc), q4 (nib, sc, mn)."""
+        k, v = [_addr(p) for p in k], [_addr(p) for p in v]
+        mins = (k[2], v[2]) if fmt == "q4" else (None, None)
+        return KvCache(FMT_CODES[fmt], heads, head_dim, page, pages, 0, k[0], v[0], k[1], v[1], *mins)
+
+    @staticmethod
+    def kv_batch(seqs, rows, kv_len=None, table=None, table_cols=0, max_len=0, row_off=None, max_rows=0, prefix_len=0,
+                 prefix_table=None) -> KvBatch:
+        """The sequences of a step: device arrays ``kv_len`` [seqs], ``table`` [seqs, table_cols] and, unless every sequence
+        has rows / seqs rows, ``row_off`` [seqs + 1]; ``prefix_table`` for a shared prefix of ``prefix_len`` tokens."""
+        return KvBatch(seqs, rows, _addr(row_off), _addr(kv_len), _addr(table), table_cols, max_len, max_rows, prefix_len,
+                       _addr(prefix_table))
+
+    @staticmethod
+    def qkv_rows(head_dim, heads=0, kv_heads=0, q=None, k=None, v=None, q_out=None, k_out=None, q_norm=None, k_norm=None,
+                 eps=1e-6, inv_freq=None, rot_dim=0, positions=None, one_plus=False, interleaved=False, q_stride=0, k_stride=0,
+                 v_stride=0, q_out_stride=0, k_out_stride=0) -> QkvRows:
+        """The q / k / v rows of a step and what is done to them (``brik_qkv_rows``)."""
+        flags = (BRIK_QKV_GAIN_ONE_PLUS if one_plus else 0) | (BRIK_QKV_INTERLEAVED if interleaved else 0)
+        return QkvRows(_addr(q), _addr(k), _addr(v), _addr(q_out), _addr(k_out), q_stride, k_stride, v_stride, q_out_stride,
+                       k_out_stride, _addr(q_norm), _addr(k_norm), _addr(inv_freq), _addr(positions), heads, kv_heads,
+                       head_dim, rot_dim, flags, eps)
+
+    @staticmethod
+    def attn_args(q, out, heads, scale, window=0, softcap=0.0, q_stride=0, out_stride=0) -> AttnArgs:
+        return AttnArgs(_addr(q), _addr(out), q_stride, out_stride, heads, window, scale, softcap)
+
+    def qk_norm_rope(self, batch: KvBatch, rows: QkvRows):
+        """Head norms and rotation of q and k (brik_qk_norm_rope)."""
+        self._check(self.lib.brik_qk_norm_rope(self.handle, ctypes.addressof(batch), ctypes.addressof(rows)))
+
+    def kv_write(self, cache: KvCache, batch: KvBatch, rows: QkvRows):
+        """k and v quantized into the cache, q and k normed and rotated on the way (brik_kv_write)."""
+        self._check(self.lib.brik_kv_write(self.handle, ctypes.addressof(cache), ctypes.addressof(batch), ctypes.addressof(rows)))
+
+    def kv_read(self, cache: KvCache, batch: KvBatch, k, v):
+        """The batch's tokens read back as f32 rows (brik_kv_read)."""
+        self._check(self.lib.brik_kv_read(self.handle, ctypes.addressof(cache), ctypes.addressof(batch), _addr(k), _addr(v)))
+
+    def attention(self, cache: KvCache, batch: KvBatch, args: AttnArgs):
+        """Attention of the batch's rows over the cache (brik_attention)."""
+        self._check(self.lib.brik_attention(self.handle, ctypes.addressof(cache), ctypes.addressof(batch), ctypes.addressof(args)))
 
     def dequant_q8(self, codes, sc, out, n):
         self._check(self.lib.brik_dequant_q8_f32(self.handle, _addr(codes), _addr(sc), _addr(out), n))

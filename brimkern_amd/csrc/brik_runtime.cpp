@@ -5,6 +5,8 @@
 // with hipModuleLaunchKernel on the context's own stream. Host API surface: device selection,
 // hipMalloc/hipFree, hipMemcpy(Async), module load + launch, events for timing.
 #include "../../include/brik.h"
+#include "attn_check.h"
+#include "kernels/attn_abi.h"
 #include "kernels/stage_abi.h"
 
 #include <hip/hip_runtime_api.h>
@@ -20,6 +22,7 @@
 
 extern "C" const unsigned char brik_hsaco_begin[];
 extern "C" const unsigned char brik_hsaco_end[];
+extern "C" const unsigned char brik_attn_hsaco_begin[];
 // brik_scratch.hip: device address of the fixed scratch array on the current device (a hipError_t)
 extern "C" int brik_scratch_resolve(int device, void** out, size_t* bytes);
 
@@ -50,6 +53,9 @@ const char* const kKernelNames[K_COUNT] = {
     "brik_gemv_stage_q8", "brik_gemv_stage_q4", "brik_gemv_stage_q3", "brik_gemv_stage1_q4", "brik_gemv_stage1_q3",
     "brik_splitk_reduce", "brik_frag_rows_f16",
 };
+
+// Kernels of the attention side's code object. Teams of 8, 16, 32, 64 lanes: brik_rows_<rope, q8, q4>_<lanes>.
+enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_PLAIN = A_READ + 2, A_COUNT = A_PLAIN + 2 };
 
 // GEMV variants {team, r, u, d}, in the order of BRIK_GEMV_FMT in gemv.hip: TEAM lanes per row team,
 // R rows per team, U groups per pipeline step, pipeline depth D; kernels brik_gemv_<fmt>_t<T>_r<R>_u<U>_d<D>
@@ -224,6 +230,8 @@ struct brik_graph {
 struct brik_ctx {
     int device = -1;
     hipModule_t module = nullptr;
+    hipModule_t attn_module = nullptr;
+    hipFunction_t attn_fn[A_COUNT] = {};
     hipFunction_t fn[K_COUNT] = {};
     hipFunction_t gemv[3][kNumGemvVariants] = {};
     hipFunction_t gemvg[3][kNumGemvVariants] = {};
@@ -1425,6 +1433,15 @@ int brik_create(int device, brik_ctx** out)
         snprintf(name, sizeof name, "brik_gemm_f16_%dx1%s", g.bm, g.nw == 8 ? "w8" : "");
         if (hipModuleGetFunction(&c->gemm_f16[t], c->module, name) != hipSuccess) return bail(BRIK_EMODULE);
     }
+    if (hipModuleLoadData(&c->attn_module, brik_attn_hsaco_begin) != hipSuccess) return bail(BRIK_EMODULE);
+    for (int k = 0; k < A_COUNT; ++k) {
+        char name[64];
+        const char* const rows[3] = {"rope", "q8", "q4"};
+        if (k < A_READ) snprintf(name, sizeof name, "brik_rows_%s_%d", rows[k / 4], 8 << k % 4);
+        else if (k < A_PLAIN) snprintf(name, sizeof name, "brik_kv_read_%s", kFmtNames[k - A_READ]);
+        else snprintf(name, sizeof name, "brik_attn_plain_%s", kFmtNames[k - A_PLAIN]);
+        if (hipModuleGetFunction(&c->attn_fn[k], c->attn_module, name) != hipSuccess) return bail(BRIK_EMODULE);
+    }
     // the fixed scratch of brik_matmul_t_q4_noalloc, with this device current (once per device)
     c->scratch_err = brik_scratch_resolve(device, &c->scratch, &c->scratch_bytes);
     constexpr int kSkl[3] = {2, 4, 8};
@@ -1473,6 +1490,7 @@ void brik_destroy(brik_ctx* c)
     if (c->kws) (void)hipFree(c->kws);
     if (c->qws) (void)hipFree(c->qws);
     if (c->module) (void)hipModuleUnload(c->module);
+    if (c->attn_module) (void)hipModuleUnload(c->attn_module);
     delete c;
 }
 
@@ -2436,6 +2454,95 @@ void brik_graph_destroy(brik_ctx* c, brik_graph* g)
     if (g->exec) (void)hipGraphExecDestroy(g->exec);
     if (g->graph) (void)hipGraphDestroy(g->graph);
     delete g;
+}
+
+static int refuse(brik_ctx* c, int code, const brik_check::Why& w) { return fail(c, code, "%s", w.text); }
+
+// Blocks per row: one row's heads in one block where the rows alone fill the device several times over, else a
+// block per 256 / lanes heads (a single row: 0.9 us less than in one block).
+static unsigned row_blocks(int rows, int units, int per_block)
+{
+    const int most = (units + per_block - 1) / per_block, want = (int)((4 * kCUs + rows - 1) / rows);
+    return (unsigned)std::min(most, std::max(1, want));
+}
+
+static int qkv_rows(brik_ctx* c, const char* who, const brik_kv_cache* cache, const brik_kv_batch* batch,
+                    const brik_qkv_rows* rows)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    if (!rows) return fail(c, BRIK_EINVAL, "%s: rows is null", who);
+    int rc = BRIK_OK;
+    const bool write = cache != nullptr;
+    brik_rows_launch a{};
+    a.r = *rows;
+    if (batch) rc = brik_check::batch(w, who, batch, write, a.r.inv_freq && !a.r.positions);
+    else rc = brik_check::no(w, BRIK_EINVAL, "%s: batch is null", who);
+    if (rc == BRIK_OK) rc = brik_check::rows(w, who, cache, batch, a.r, write);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (batch->rows == 0) return BRIK_OK;
+    a.s = brik_check::step(*batch, cache);
+    if (cache) a.c = *cache;
+    a.nq = a.r.q ? a.r.heads : 0;
+    a.nk = a.r.k ? a.r.kv_heads : 0;
+    a.nv = write ? a.r.kv_heads : 0;
+    const int units = a.nq + a.nk + a.nv;
+    if (units == 0) return BRIK_OK;
+    int team = 0;
+    while ((8 << team) * 4 < a.r.head_dim) ++team;
+    const int fmt = !cache ? 0 : cache->fmt == BRIK_FMT_Q8 ? 1 : 2;
+    void* args[] = {&a};
+    return launch_fn(c, c->attn_fn[A_ROWS + 4 * fmt + team], (unsigned)batch->rows, row_blocks(batch->rows, units, 32 >> team), 256, 0, args);
+}
+
+int brik_qk_norm_rope(brik_ctx* c, const brik_kv_batch* batch, const brik_qkv_rows* rows)
+{
+    return qkv_rows(c, "qk_norm_rope", nullptr, batch, rows);
+}
+
+int brik_kv_write(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* batch, const brik_qkv_rows* rows)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    const int rc = brik_check::cache(w, "kv_write", cache);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    return qkv_rows(c, "kv_write", cache, batch, rows);
+}
+
+int brik_kv_read(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* batch, float* k, float* v)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    int rc = brik_check::cache(w, "kv_read", cache);
+    if (rc == BRIK_OK) rc = brik_check::batch(w, "kv_read", batch, true, true);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(c, BRIK_EALIGN, "kv_read: k and v must be 16-byte aligned");
+    if (batch->rows == 0 || (!k && !v)) return BRIK_OK;
+    brik_read_launch a{brik_check::step(*batch, cache), *cache, k, v};
+    const int quads = ((k ? 1 : 0) + (v ? 1 : 0)) * cache->heads * cache->head_dim / 4;
+    void* args[] = {&a};
+    return launch_fn(c, c->attn_fn[A_READ + (cache->fmt == BRIK_FMT_Q4)], (unsigned)batch->rows, row_blocks(batch->rows, quads, 256),
+                     256, 0, args);
+}
+
+int brik_attention(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* batch, const brik_attn_args* args)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    int rc = brik_check::cache(w, "attention", cache);
+    if (rc == BRIK_OK) rc = brik_check::batch(w, "attention", batch, true, true);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (!args) return fail(c, BRIK_EINVAL, "attention: args is null");
+    brik_attn_launch a{};
+    a.a = *args;
+    rc = brik_check::attn(w, "attention", cache, batch, a.a);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (batch->rows == 0) return BRIK_OK;
+    a.s = brik_check::step(*batch, cache);
+    a.c = *cache;
+    void* kargs[] = {&a};
+    return launch_fn(c, c->attn_fn[A_PLAIN + (cache->fmt == BRIK_FMT_Q4)], (unsigned)batch->rows, (unsigned)(a.a.heads + 3) / 4, 256, 0,
+                     kargs);
 }
 
 int brik_timer_begin(brik_ctx* c)

@@ -345,6 +345,103 @@ int brik_matmul_t_f16w(brik_ctx *ctx, const float *x, const uint16_t *w, float *
  * shader (shaders.ts:932-943) decodes those two as infinity / NaN; every other input agrees. */
 int brik_f16_to_f32(brik_ctx *ctx, const uint16_t *src, float *out, size_t n_elems);
 
+/* ---- the attention side of a decoder layer ------------------------------------------------------
+ * What a decoder layer runs between its q / k / v projections and wo (recordLayerKV, src/lib/webgpu/kernels.ts:1690-1744;
+ * quantize_kv src/lib/webgpu/shaders.ts:1673, attention_q8kv :1711, attention_decode_q8kv :1856, rope :1361): head
+ * norms and rotation, the keys and values quantized into a paged cache, attention that reads the cache as it is.
+ *
+ * The cache: two .brik tensors (keys, values) of [pages, heads, page, head_dim] values in the planes of fmt, in 32-value
+ * groups along head_dim: q8 codes, scales; q4 nibbles, scales, mins. brik_dequant_* and brik_quantize_* read and write
+ * whole caches as any other tensor. head_dim: a multiple of 32, 32 to 256 (brik_attention: 64, 96, 128, 192 or 256).
+ * page (tokens per page): a power of two, 16 to 65536. Code planes 16-byte, scales and mins 16-byte aligned. */
+typedef struct brik_kv_cache {
+    int32_t fmt;             /* BRIK_FMT_Q8 or BRIK_FMT_Q4 */
+    int32_t heads;           /* key / value heads */
+    int32_t head_dim;
+    int32_t page;
+    int32_t pages;
+    int32_t reserved;        /* 0 */
+    void *k, *v;             /* code planes */
+    uint16_t *k_scales, *v_scales;
+    uint16_t *k_mins, *v_mins;   /* q4; NULL for q8 */
+} brik_kv_cache;
+
+/* The sequences of one step. Rows are tokens: `rows` of them, those of sequence b being [row_off[b], row_off[b + 1])
+ * (row_off NULL: rows / seqs each). They are the last tokens of their sequence: the i-th of n rows has position
+ * kv_len[b] - n + i, kv_len[b] counting the prefix and this step's rows. Token p of sequence b lies in slot
+ * (p - prefix_len) % page of page table[b, (p - prefix_len) / page], or, for p < prefix_len, in slot p % page of page
+ * prefix_table[p / page]: a prefix that all sequences share, in the cache once.
+ * row_off, kv_len, table, prefix_table: DEVICE arrays, read when the call runs (a recorded call reads what they hold
+ * at the replay). max_len and max_rows bound kv_len and the rows of a sequence and size the launch. Tokens at or past
+ * max_len, tokens past the table and tokens on a page outside [0, pages) do not exist: they are not written, read as
+ * zeros and not attended to. A row past row_off[seqs] is left as it is; row_off must not decrease. */
+typedef struct brik_kv_batch {
+    int32_t seqs, rows;
+    const int32_t *row_off;      /* [seqs + 1], or NULL */
+    const int32_t *kv_len;       /* [seqs] */
+    const int32_t *table;        /* [seqs, table_cols] */
+    int32_t table_cols;
+    int32_t max_len;
+    int32_t max_rows;            /* 0: rows */
+    int32_t prefix_len;          /* 0: no prefix */
+    const int32_t *prefix_table; /* [ceil(prefix_len / page)] */
+} brik_kv_batch;
+
+/* The q / k / v rows of a step: f32, [rows, heads, head_dim], a row every *_stride values (0: packed; strides are
+ * multiples of 4). Every head of q and k is, in this order,
+ *   normed:  y = x / sqrt(sum(x^2) / head_dim + eps) * g, g = q_norm or k_norm [head_dim] (BRIK_QKV_GAIN_ONE_PLUS: 1 + g);
+ *            skipped where the weight is NULL
+ *   rotated: pairs (a, b) of the first rot_dim values become (a cos t - b sin t, b cos t + a sin t), pair i by
+ *            t = p * inv_freq[i] with p the row's position (positions[row] if given); the pairs are (i, i + rot_dim / 2)
+ *            or, with BRIK_QKV_INTERLEAVED, (2i, 2i + 1); skipped where inv_freq is NULL
+ * with angles (|t| < 2^31), sums and products in 64 bits and one rounding to f32 at the end: a quantized key does not
+ * depend on whether it was rotated in the same call. rot_dim: a multiple of 8, at most head_dim.
+ * q_out may be q, k_out may be k (with the same stride); other overlaps are not allowed. All 16-byte aligned. */
+#define BRIK_QKV_GAIN_ONE_PLUS 1
+#define BRIK_QKV_INTERLEAVED 2
+typedef struct brik_qkv_rows {
+    const float *q, *k, *v;          /* NULL: none of these */
+    float *q_out, *k_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    const float *q_norm, *k_norm;
+    const float *inv_freq;           /* [rot_dim / 2] */
+    const int32_t *positions;        /* DEVICE [rows], or NULL */
+    int32_t heads, kv_heads, head_dim, rot_dim;
+    int32_t flags;
+    float eps;
+} brik_qkv_rows;
+
+/* q_out and k_out from q and k (v is not looked at). The batch gives rows and the positions. */
+int brik_qk_norm_rope(brik_ctx *ctx, const brik_kv_batch *batch, const brik_qkv_rows *rows);
+
+/* k (normed and rotated as asked for) and v quantized into their tokens' slots, in the planes' exact .brik encoding
+ * (the bytes of brik_quantize_* on the same f32 values); q, if given, is normed and rotated into q_out in the same
+ * launch, and k_out, if given, receives the f32 keys. Tokens of the prefix are not written (write a prefix as a sequence
+ * of its own). Two rows on one slot (sequences that share a page) leave one of them, or a mixture, there. */
+int brik_kv_write(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batch *batch, const brik_qkv_rows *rows);
+
+/* The batch's tokens (prefix tokens included) read back: k and v f32 [rows, heads, head_dim] packed, 16-byte aligned;
+ * either may be NULL. To read whole sequences make all their tokens rows. */
+int brik_kv_read(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batch *batch, float *k, float *v);
+
+/* out[row, h] = sum over the tokens j that the row sees of softmax_j(x_j) v_j, with x_j = scale * (q[row, h] . k_j),
+ * softcap > 0: x_j = softcap * tanh(x_j / softcap). Query head h reads key / value head h / (heads / kv heads). A row at
+ * position p sees the tokens j <= p, with window > 0 only those j > p - window; a row that sees none gives zeros, a
+ * row of NaN gives NaN, and what lies in tokens that a row does not see (infinities, NaN) does not reach it. A shared
+ * prefix is read once for all sequences. q and out: f32 [rows, heads, head_dim], a row every *_stride values (0: packed);
+ * out must not overlap q. f32-accurate: every product takes the codes exactly and the other operand as two halves.
+ * Workspace: partial results of split key ranges, grown on demand. */
+typedef struct brik_attn_args {
+    const float *q;
+    float *out;
+    int64_t q_stride, out_stride;
+    int32_t heads;
+    int32_t window;              /* 0: all tokens */
+    float scale;
+    float softcap;               /* 0: none */
+} brik_attn_args;
+int brik_attention(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batch *batch, const brik_attn_args *args);
+
 /* ---- timing and tuning -------------------------------------------------------------------
  * The reference has no kernel timing (it times whole tokens with performance.now(),
  * src/app/page.tsx:1313-1376). brik_timer_begin/end record HIP events on the context stream
