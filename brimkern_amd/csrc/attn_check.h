@@ -53,6 +53,7 @@ inline int batch(Why& w, const char* who, const brik_kv_batch* b, bool tokens, b
     if (!b) return no(w, BRIK_EINVAL, "%s: batch is null", who);
     if (b->seqs < 0 || b->rows < 0 || b->table_cols < 0 || b->max_len < 0 || b->max_rows < 0 || b->prefix_len < 0)
         return no(w, BRIK_EINVAL, "%s: negative size in the batch", who);
+    if (b->rows > (1 << 24) - 1) return no(w, BRIK_EINVAL, "%s: %d rows exceed 2^24 - 1 in one call", who, b->rows);
     if (b->rows == 0 || (!tokens && !lens)) return BRIK_OK;
     if (b->seqs == 0) return no(w, BRIK_EINVAL, "%s: %d rows of no sequences", who, b->rows);
     if (!b->row_off && b->rows % b->seqs)
@@ -138,6 +139,8 @@ inline int attn(Why& w, const char* who, const brik_kv_cache* c, const brik_kv_b
     BRIK_CHECK(stride(w, who, "q", a.q_stride, width));
     BRIK_CHECK(stride(w, who, "out", a.out_stride, width));
     if (b->rows == 0) return BRIK_OK;
+    if ((long long)b->rows * a.heads >= (1ll << 27))
+        return no(w, BRIK_EINVAL, "%s: %d rows of %d heads exceed 2^27 in one call", who, b->rows, a.heads);
     if (!a.q || !a.out) return no(w, BRIK_EINVAL, "%s: q or out is null", who);
     if (off(a.q, 16) || off(a.out, 16)) return no(w, BRIK_EALIGN, "%s: q and out must be 16-byte aligned", who);
     if (overlap(a.q, a.q_stride, width, a.out, a.out_stride, width, b->rows)) return no(w, BRIK_EINVAL, "%s: out overlaps q", who);

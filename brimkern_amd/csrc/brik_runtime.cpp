@@ -55,7 +55,9 @@ const char* const kKernelNames[K_COUNT] = {
 };
 
 // Kernels of the attention side's code object. Teams of 8, 16, 32, 64 lanes: brik_rows_<rope, q8, q4>_<lanes>.
-enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_PLAIN = A_READ + 2, A_COUNT = A_PLAIN + 2 };
+// Attention of up to 16 rows a tile: brik_attn_few_<fmt>_<head_dim>.
+enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_JOIN = A_FEW + 10, A_COUNT };
+constexpr int kAttnDims[5] = {64, 96, 128, 192, 256};
 
 // GEMV variants {team, r, u, d}, in the order of BRIK_GEMV_FMT in gemv.hip: TEAM lanes per row team,
 // R rows per team, U groups per pipeline step, pipeline depth D; kernels brik_gemv_<fmt>_t<T>_r<R>_u<U>_d<D>
@@ -267,6 +269,8 @@ struct brik_ctx {
     size_t cws_bytes = 0;
     void* pws = nullptr;   // split-K partial tiles [slice][row][column] f32 (grow-only)
     size_t pws_bytes = 0;
+    void* aws = nullptr;   // attention: partial results of split keys (grow-only)
+    size_t aws_bytes = 0;
     void* qws = nullptr;   // few-row GEMM: partial tiles (fixed size, so graphs may hold its address)
     void* fws = nullptr;   // fragment GEMM: x panels and the f16 weight panels of one column slab (grow-only)
     size_t fws_bytes = 0;
@@ -1438,8 +1442,9 @@ int brik_create(int device, brik_ctx** out)
         char name[64];
         const char* const rows[3] = {"rope", "q8", "q4"};
         if (k < A_READ) snprintf(name, sizeof name, "brik_rows_%s_%d", rows[k / 4], 8 << k % 4);
-        else if (k < A_PLAIN) snprintf(name, sizeof name, "brik_kv_read_%s", kFmtNames[k - A_READ]);
-        else snprintf(name, sizeof name, "brik_attn_plain_%s", kFmtNames[k - A_PLAIN]);
+        else if (k < A_FEW) snprintf(name, sizeof name, "brik_kv_read_%s", kFmtNames[k - A_READ]);
+        else if (k < A_JOIN) snprintf(name, sizeof name, "brik_attn_few_%s_%d", kFmtNames[(k - A_FEW) / 5], kAttnDims[(k - A_FEW) % 5]);
+        else snprintf(name, sizeof name, "brik_attn_join");
         if (hipModuleGetFunction(&c->attn_fn[k], c->attn_module, name) != hipSuccess) return bail(BRIK_EMODULE);
     }
     // the fixed scratch of brik_matmul_t_q4_noalloc, with this device current (once per device)
@@ -1489,6 +1494,7 @@ void brik_destroy(brik_ctx* c)
     if (c->fws) (void)hipFree(c->fws);
     if (c->kws) (void)hipFree(c->kws);
     if (c->qws) (void)hipFree(c->qws);
+    if (c->aws) (void)hipFree(c->aws);
     if (c->module) (void)hipModuleUnload(c->module);
     if (c->attn_module) (void)hipModuleUnload(c->attn_module);
     delete c;
@@ -2525,6 +2531,52 @@ int brik_kv_read(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* b
                      256, 0, args);
 }
 
+// Splits of a section's keys (at most `keys` of them): enough blocks to fill the device, each with at least four blocks
+// of 32 keys, one per wave.
+static int attn_splits(long blocks, long keys)
+{
+    const long most = std::max(1l, (keys + 127) / 128), want = (2 * kCUs + blocks - 1) / std::max(1l, blocks);
+    return (int)std::min({most, std::max(1l, want), 64l});
+}
+
+static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
+{
+    constexpr int BM = 16;
+    const long KV = a.c.heads, G = a.a.heads / KV, rows = a.s.rows;
+    const long own_keys = std::min<long>((long)a.s.max_len - a.s.prefix_len, (long)a.s.table_cols << a.s.shift);
+    const long prefix_keys = std::min(a.s.prefix_len, a.s.max_len);
+    // row tiles of the sequences: the same number for each where that is not many more than there can be
+    const long most = max_rows ? std::min<long>(max_rows, rows) : rows;
+    const long per_seq = a.s.row_off ? (most * G + BM - 1) / BM : (a.s.per_seq * G + BM - 1) / BM;
+    const long bound = (rows * G + BM - 1) / BM + a.s.seqs;
+    long tiles = per_seq * a.s.seqs;
+    a.tiles_per_seq = (int)per_seq;
+    if (a.s.row_off && tiles > 2 * bound) {
+        a.tiles_per_seq = 0;
+        tiles = bound;
+    }
+    a.own_splits = attn_splits(KV * tiles, own_keys);
+    if (prefix_keys > 0) {
+        a.prefix_tiles = (int)((rows * G + BM - 1) / BM);
+        a.prefix_splits = attn_splits(KV * a.prefix_tiles, prefix_keys);
+    }
+    const int slots = a.prefix_splits + a.own_splits;
+    if (slots > 1) {
+        const size_t vectors = (size_t)slots * rows * a.a.heads, d = (size_t)a.c.head_dim;
+        HIP_TRY_RC(ensure_buf(c, c->aws, c->aws_bytes, 4 * vectors * (d + 2)));
+        a.part = static_cast<float*>(c->aws);
+        a.ml = a.part + vectors * d;
+    }
+    const long blocks = KV * (tiles * a.own_splits + (long)a.prefix_tiles * a.prefix_splits);
+    if (blocks >= (1l << 24)) return fail(c, BRIK_EINVAL, "attention: %ld blocks in one call", blocks);
+    int dim = 0;
+    while (kAttnDims[dim] != a.c.head_dim) ++dim;
+    void* args[] = {&a};
+    HIP_TRY_RC(launch_fn(c, c->attn_fn[A_FEW + 5 * (a.c.fmt == BRIK_FMT_Q4) + dim], (unsigned)blocks, 1, 256, 0, args));
+    if (slots > 1) return launch_fn(c, c->attn_fn[A_JOIN], (unsigned)rows, (unsigned)a.a.heads, 256, 0, args);
+    return BRIK_OK;
+}
+
 int brik_attention(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* batch, const brik_attn_args* args)
 {
     if (!c) return BRIK_EINVAL;
@@ -2540,9 +2592,7 @@ int brik_attention(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch*
     if (batch->rows == 0) return BRIK_OK;
     a.s = brik_check::step(*batch, cache);
     a.c = *cache;
-    void* kargs[] = {&a};
-    return launch_fn(c, c->attn_fn[A_PLAIN + (cache->fmt == BRIK_FMT_Q4)], (unsigned)batch->rows, (unsigned)(a.a.heads + 3) / 4, 256, 0,
-                     kargs);
+    return attention(c, a, batch->max_rows);
 }
 
 int brik_timer_begin(brik_ctx* c)

@@ -88,4 +88,8 @@ typedef struct brik_attn_launch {
     brik_kv_cache c;
     float *part;           // partial outputs [slot][row][head][head_dim]
     float *ml;             // their reference exponents and sums [slot][row][head][2]
+    // The grid: row tiles of the prefix's keys (rows of all sequences) and of the sequences' own keys, each tile's keys
+    // split over so many blocks; slots: prefix_splits, then own_splits. tiles_per_seq: the tile's sequence by division (0:
+    // by a search over the sequences' rows).
+    int32_t prefix_tiles, prefix_splits, own_splits, tiles_per_seq;
 } brik_attn_launch;

@@ -1,0 +1,260 @@
+// What the attention kernels share: the rows of a tile, which keys they see, the split of the keys, half pairs.
+#pragma once
+#include "attn_abi.h"
+#include "common.h"
+
+namespace {
+
+constexpr float ATTN_LOG2E = 1.44269504088896340736f;
+constexpr float ATTN_NONE = -1e30f;      // reference exponent of a row that has seen no key
+
+// v of the lower and of the upper lane of this lane's pair (l, l ^ 32; quarter_pair: l, l ^ 16): both lanes get the same two
+// values. (The elements are copied out first: a bit cast of a vector's element reads element 0.)
+__device__ __forceinline__ void half_pair(float v, float& a, float& b)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    a = __builtin_bit_cast(float, lo);
+    b = __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ void quarter_pair(float v, float& a, float& b)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    a = __builtin_bit_cast(float, lo);
+    b = __builtin_bit_cast(float, hi);
+}
+// Maximum / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float quarters_max(float v)
+{
+    float a, b;
+    quarter_pair(v, a, b);
+    half_pair(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float quarters_sum(float v)
+{
+    float a, b;
+    quarter_pair(v, a, b);
+    half_pair(a + b, a, b);
+    return a + b;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Min / max over the 64 lanes (uniform result).
+__device__ __forceinline__ int wave_min(int v)
+{
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v = min(v, __shfl_xor(v, m));
+    return uniform(v);
+}
+__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+
+// The sequence of row t: how many of row_off[1..seqs] are at most t. One load round trip per 64 sequences.
+__device__ __forceinline__ int seq_of_row(const brik_step& s, int t)
+{
+    if (!s.row_off) return t / s.per_seq;
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int base = 0; base < s.seqs; base += 64) {
+        const int i = base + lane;
+        const int32_t end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
+        count += __popcll(__ballot(end <= t));
+    }
+    return count;
+}
+
+// The same for a row per lane, whose rows are t0 + (0 .. count - 1) over the wave: every candidate row is compared with 64 ends
+// at a time, so no lane follows a chain of dependent loads.
+__device__ __forceinline__ int seq_of_lane(const brik_step& s, int t, int t0, int count)
+{
+    if (!s.row_off) return t / s.per_seq;
+    const int lane = threadIdx.x & 63;
+    int mine = 0;
+    for (int base = 0; base < s.seqs; base += 64) {
+        const int i = base + lane;
+        const int32_t end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
+        for (int k = 0; k < count; ++k) {
+            const int c = __popcll(__ballot(end <= t0 + k));
+            if (t == t0 + k) mine += c;
+        }
+    }
+    return mine;
+}
+
+// The position of row t of sequence b.
+__device__ __forceinline__ int32_t row_position(const brik_step& s, int b, int t)
+{
+    const int32_t end = s.row_off ? s.row_off[b + 1] : (b + 1) * s.per_seq;
+    return s.kv_len[b] - end + t;
+}
+
+// Tile `tile` of the sequences' row tiles (BM rows of rows * G each), in order: its sequence and its place in it.
+// b == seqs: there is no such tile.
+__device__ __forceinline__ void find_tile(const brik_step& s, int tile, int G, int BM, int& b, int& j)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < s.seqs; base += 64) {
+        const int i = base + lane;
+        int32_t first, n = 0;
+        if (i < s.seqs) brik_rows_of(s, i, first, n);
+        const int tiles = (int)(((long long)n * G + BM - 1) / BM);
+        int sum = tiles;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int o = __shfl_up(sum, m);
+            if (lane >= m) sum += o;
+        }
+        const uint64_t past = __ballot(before + sum > tile);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            b = uniform(base + l);
+            j = uniform(tile - before - (__shfl(sum, l) - __shfl(tiles, l)));
+            return;
+        }
+        before += __shfl(sum, 63);
+    }
+    b = s.seqs;
+    j = 0;
+}
+
+// One block's work: which rows, which keys.
+struct Work {
+    int head;                  // key / value head
+    int slot;                  // of the partial results
+    bool prefix;               // keys of the prefix, rows of all sequences
+    int b;                     // sequence (own keys)
+    int first, count;          // its rows
+    int r0;                    // first of the tile's rows, counted over count * G
+    int split, splits;
+};
+
+// The grid: heads fastest, then the splits, then the row tiles; the prefix's blocks before the own keys'.
+template <int BM>
+__device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
+{
+    const int KV = a.c.heads, G = a.a.heads / KV;
+    int id = blockIdx.x;
+    w.head = id % KV;
+    id /= KV;
+    const int pre = a.prefix_tiles * a.prefix_splits;
+    w.prefix = id < pre;
+    if (w.prefix) {
+        w.splits = a.prefix_splits;
+        w.split = id % w.splits;
+        w.slot = w.split;
+        w.b = 0;
+        w.first = 0;
+        w.count = a.s.rows;
+        w.r0 = id / w.splits * BM;
+        return true;
+    }
+    id -= pre;
+    w.splits = a.own_splits;
+    w.split = id % w.splits;
+    w.slot = a.prefix_splits + w.split;
+    int tile = id / w.splits, j;
+    if (a.tiles_per_seq) {
+        w.b = tile / a.tiles_per_seq;
+        j = tile - w.b * a.tiles_per_seq;
+    } else {
+        find_tile(a.s, tile, G, BM, w.b, j);
+        if (w.b >= a.s.seqs) return false;
+    }
+    brik_rows_of(a.s, w.b, w.first, w.count);
+    // the last tiles see the most keys: they come first
+    const int tiles = (int)(((long long)w.count * G + BM - 1) / BM);
+    if (j >= tiles) return false;
+    w.r0 = (tiles - 1 - j) * BM;
+    return true;
+}
+
+// A row of a tile (this lane's): its token and head, and the keys it sees, [lo, hi) in the section's own numbering
+// (prefix tokens, or own tokens behind the prefix). A row past the tile's end sees everything and is not stored.
+struct Row {
+    int t, h;
+    bool real;
+    int lo, hi;
+};
+
+template <int BM>
+__device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w, int m)
+{
+    const int G = a.a.heads / a.c.heads;
+    Row r;
+    const int i = w.r0 + m, rel = i / G;
+    r.real = rel < w.count;
+    r.t = w.first + rel;
+    r.h = w.head * G + i - rel * G;
+    r.lo = 0;
+    r.hi = 0x7fffffff;
+    int b = w.b;
+    if (w.prefix) {
+        const int t0 = uniform(w.r0 / G), last = min((w.r0 + BM - 1) / G, a.s.rows - 1);
+        b = seq_of_lane(a.s, r.t, t0, uniform(last) - t0 + 1);
+        r.real = r.real && b < a.s.seqs;
+    }
+    if (!r.real) return r;
+    const int32_t pos = row_position(a.s, b, r.t), first = w.prefix ? 0 : a.s.prefix_len;
+    const int32_t end = w.prefix ? min(a.s.prefix_len, a.s.max_len)
+                                 : (int32_t)min((long long)a.s.max_len - first, (long long)a.s.table_cols << a.s.shift);
+    r.hi = max(0, min(pos + 1 - first, end));
+    r.lo = a.a.window ? max(0, pos - a.a.window + 1 - first) : 0;
+    return r;
+}
+
+// The tile's key blocks [t0, t1) of 32 keys that this split works on: the blocks that any row sees, divided over the
+// splits in pieces of at least `least`.
+__device__ __forceinline__ void find_keys(const Work& w, const Row& r, int least, int& t0, int& t1)
+{
+    const int lo = wave_min(r.real ? r.lo : 0x7fffffff), hi = wave_max(r.real ? r.hi : 0);
+    t0 = t1 = 0;
+    if (lo >= hi) return;
+    const int first = lo >> 5, n = ((hi + 31) >> 5) - first;
+    const int each = max(least, (n + w.splits - 1) / w.splits);
+    t0 = first + min(n, w.split * each);
+    t1 = first + min(n, (w.split + 1) * each);
+}
+
+// The pages of keys 32 t .. 32 t + 31: of the first and of the last 16 (the same page unless a page holds 16 tokens), -1
+// where they do not exist, and the slot of the first key.
+struct KeyPages {
+    int32_t p[2];
+};
+__device__ __forceinline__ KeyPages key_pages(const brik_attn_launch& a, const Work& w, int t)
+{
+    KeyPages k;
+    const int32_t* const tab = w.prefix ? a.s.prefix_table : a.s.table + (size_t)w.b * a.s.table_cols;
+    const int cols = w.prefix ? (a.s.prefix_len + (1 << a.s.shift) - 1) >> a.s.shift : a.s.table_cols;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = (32 * t + 16 * i) >> a.s.shift;
+        const int32_t id = c < cols ? tab[c] : -1;
+        k.p[i] = (uint32_t)id < (uint32_t)a.s.pages ? id : -1;
+    }
+    return k;
+}
+
+__device__ __forceinline__ half2_t halves(float a, float b)
+{
+    half2_t h;
+    h.x = (_Float16)a;
+    h.y = (_Float16)b;
+    return h;
+}
+
+// tanh in f32: the exponential, and near 0, where that cancels, the odd series (next term below 2^-28 of the value).
+__device__ __forceinline__ float attn_tanh(float u)
+{
+    const float z = u * u;
+    const float s = u * fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    const float e = __builtin_amdgcn_exp2f(u * (2.f * ATTN_LOG2E));
+    const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+    return fabsf(u) < 0.25f ? s : t;
+}
+
+}  // namespace

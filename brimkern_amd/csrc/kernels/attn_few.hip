@@ -1,0 +1,473 @@
+// Attention of up to 16 rows (query heads of a key / value head, times rows) over the quantized cache: decoding.
+//
+//   x_j = sum over groups g of s_jg (q . c_j)_g (+ m_jg sum(q)_g),   o = sum_j p_j v_j / sum_j p_j
+//
+// Four waves of a block take every fourth block of 32 keys; each is a pass over the keys of its own, with a running
+// reference exponent M and sum, and they are joined at the end. The products run on the matrix cores in a form that
+// keeps f32 accuracy: codes are small integers, exact in f16, and the other operand is split into two halves
+// (22 bits). A group is 32 values, so one 16x16x32 product is one group of 16 keys and 16 rows:
+//   scores: S^T = K Q^T, a product per group, its f32 result times the key's scale of the group (and, q4, the min times
+//           the group's sum of q). A lane then holds 8 keys of one row: softmax needs no LDS.
+//   output: O^T = V^T P'^T with P'_jg = p_j s_jg per group, split into halves in the registers where p lies. The order of
+//           the keys within the product follows from that; V's transposed operand is read in it (ds_read_b64_tr_b8).
+//   q4:     s n + m is taken as s (n - 8) + (m + 8 s), the second sum on the vector units.
+// p s may be far from 1 (scales of any size), and a half holds 2^-24 to 65504. So M bounds x_j + e_j, e_j the exponent of the
+// key's largest value scale, within 2^8; p is 2^7 times exp2(x - M) and P' stays below 2^15.
+//
+// Keys and values go through the wave's own LDS: whole 16-byte chunks of rows are loaded a block ahead into registers, and
+// written rotated by row so that reading a column of chunks meets every bank once.
+#include "attn_common.h"
+
+namespace {
+
+template <int FMT, int D>
+struct FewTile {
+    static constexpr int NG = D / 32;
+    static constexpr int CH = (FMT == FMT_Q8 ? D : D / 2) / 16;          // 16-byte chunks of a row
+    static constexpr int NI = (CH + 1) / 2;                              // loads of 64 chunks for 32 rows
+    static constexpr int P2 = CH % 16 == 0 ? 4 : CH % 8 == 0 ? 3 : CH % 4 == 0 ? 2 : CH % 2 == 0 ? 1 : 0;
+    static constexpr int SD = 16 * NG;                                   // dwords of the 32 keys' scales
+    static constexpr int SI = (SD + 63) / 64;
+    static constexpr int HP = FMT == FMT_Q4 ? 2 : 1;                     // planes of halves: scales, mins
+    static constexpr int K = 0, V = 512 * CH, KS = 2 * V, VS = KS + 4 * SD, E = VS + 4 * SD;
+    static constexpr int KM = E + 128, VM = KM + (HP - 1) * 8 * SD, STAGE = VM + (HP - 1) * 8 * SD;     // mins: f32
+    static constexpr int OS = D + 4;                                     // floats of a row of the joined output
+    static constexpr int JOIN = 16 * OS * 4;
+    static constexpr int BYTES = STAGE > JOIN ? STAGE : JOIN;
+    // how far the chunks of a row are rotated: rows whose chunks would share banks differ
+    static __device__ __forceinline__ int rot(int row) { return (row >> (4 - P2)) & ((1 << P2) - 1); }
+};
+
+// A block of 32 keys in registers.
+template <int FMT, int D>
+struct FewLoad {
+    using T = FewTile<FMT, D>;
+    u32x4_t k[T::NI], v[T::NI];
+    uint32_t ks[T::HP * T::SI], vs[T::HP * T::SI];
+};
+
+template <int FMT, int D>
+__device__ __forceinline__ void few_load(FewLoad<FMT, D>& f, const brik_attn_launch& a, const Work& w, int t, const KeyPages& kp)
+{
+    using T = FewTile<FMT, D>;
+    const int lane = threadIdx.x & 63, slot = (32 * t) & ((1 << a.s.shift) - 1);
+    // vectors of the first key and of the 17th (on page 0 where there is none: read and not used)
+    const size_t v0 = (((size_t)max(kp.p[0], 0) * a.c.heads + w.head) << a.s.shift) + slot;
+    const size_t v1 = a.s.shift > 4 ? v0 + 16 : ((size_t)max(kp.p[1], 0) * a.c.heads + w.head) << 4;
+#pragma unroll
+    for (int i = 0; i < T::NI; ++i) {
+        const int c = 64 * i + lane, row = c / T::CH;
+        if (T::CH % 2 && c >= 32 * T::CH) break;
+        int chunk = c - row * T::CH - T::rot(row);
+        chunk = chunk < 0 ? chunk + T::CH : chunk;
+        const size_t at = ((row < 16 ? v0 : v1) + (row & 15)) * (size_t)(16 * T::CH) + 16 * chunk;
+        f.k[i] = *(const u32x4_t*)((const uint8_t*)a.c.k + at);
+        f.v[i] = *(const u32x4_t*)((const uint8_t*)a.c.v + at);
+    }
+#pragma unroll
+    for (int i = 0; i < T::SI; ++i) {
+        const int d = 64 * i + lane;
+        if (d < T::SD) {
+            const bool first = d < T::SD / 2;
+            const size_t at = (first ? v0 : v1) * T::NG / 2 + (first ? d : d - T::SD / 2);          // dwords: two halves each
+            f.ks[i] = ((const uint32_t*)a.c.k_scales)[at];
+            f.vs[i] = ((const uint32_t*)a.c.v_scales)[at];
+            if constexpr (FMT == FMT_Q4) {
+                f.ks[T::SI + i] = ((const uint32_t*)a.c.k_mins)[at];
+                f.vs[T::SI + i] = ((const uint32_t*)a.c.v_mins)[at];
+            }
+        }
+    }
+}
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x2_t centred_mins(uint32_t s, uint32_t m)
+{
+    f32x2_t r;
+    r.x = fmaf(8.f, f16_bits_to_f32(s & 0xffffu), f16_bits_to_f32(m & 0xffffu));
+    r.y = fmaf(8.f, f16_bits_to_f32(s >> 16), f16_bits_to_f32(m >> 16));
+    return r;
+}
+
+template <int FMT, int D>
+__device__ __forceinline__ void few_spread(const FewLoad<FMT, D>& f, unsigned char* lds)
+{
+    using T = FewTile<FMT, D>;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < T::NI; ++i) {
+        if (T::CH % 2 && 64 * i + lane >= 32 * T::CH) break;
+        *(u32x4_t*)(lds + T::K + 1024 * i + 16 * lane) = f.k[i];
+        *(u32x4_t*)(lds + T::V + 1024 * i + 16 * lane) = f.v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < T::SI; ++i) {
+        const int d = 64 * i + lane;
+        if (d < T::SD) {
+            *(uint32_t*)(lds + T::KS + 4 * d) = f.ks[i];
+            *(uint32_t*)(lds + T::VS + 4 * d) = f.vs[i];
+            if constexpr (FMT == FMT_Q4) {
+                // a value is s n + m = s (n - 8) + (m + 8 s)
+                *(f32x2_t*)(lds + T::KM + 8 * d) = centred_mins(f.ks[i], f.ks[T::SI + i]);
+                *(f32x2_t*)(lds + T::VM + 8 * d) = centred_mins(f.vs[i], f.vs[T::SI + i]);
+            }
+        }
+    }
+}
+
+// Orders a wave's LDS writes before its own later reads of what other lanes wrote (a wave's LDS operations complete in issue
+// order, so this only binds the compiler).
+__device__ __forceinline__ void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
+
+// Eight int8 codes as f16, the bytes of each word in the order 0, 2, 1, 3: 1024 + (c + 128) has the code's bits in its low
+// byte, and the subtraction is exact.
+__device__ __forceinline__ half8_t halves_q8(uint32_t w0, uint32_t w1)
+{
+    const half2_t off = {(_Float16)-1152.f, (_Float16)-1152.f};
+    half8_t r;
+    w0 ^= 0x80808080u;
+    w1 ^= 0x80808080u;
+    const uint32_t u[4] = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04020400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030401u),
+                           __builtin_amdgcn_perm(0x64646464u, w1, 0x04020400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030401u)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2_t h = __builtin_bit_cast(half2_t, u[i]) + off;
+        r[2 * i] = h.x;
+        r[2 * i + 1] = h.y;
+    }
+    return r;
+}
+
+// Codes in the low nibbles of each 16 bits as f16 less 8. The products of values have to be of both signs: the matrix
+// cores' sums cut the bits that do not fit, and over sums of nearly equal terms that shows (7e-5 with codes from 0).
+__device__ __forceinline__ half8_t centred_q4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    const half2_t off = {(_Float16)-1032.f, (_Float16)-1032.f};
+    const uint32_t u[4] = {a, b, c, d};
+    half8_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2_t h = __builtin_bit_cast(half2_t, (u[i] & 0x000f000fu) | 0x64006400u) + off;
+        r[2 * i] = h.x;
+        r[2 * i + 1] = h.y;
+    }
+    return r;
+}
+
+// Half k of the halves that a lane read of 4 keys (NG each, in order).
+template <int N>
+__device__ __forceinline__ float half_of(const u32x2_t (&v)[N], int k)
+{
+    const uint32_t w = (k & 2) ? v[k >> 2].y : v[k >> 2].x;
+    return f16_bits_to_f32((k & 1) ? w >> 16 : w & 0xffffu);
+}
+
+template <int FMT, int D>
+__device__ __forceinline__ void few_body(const brik_attn_launch& a)
+{
+    using T = FewTile<FMT, D>;
+    constexpr int NG = T::NG;
+    constexpr bool Q4 = FMT == FMT_Q4;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * T::BYTES];
+    __shared__ float joinm[4][16], joinl[4][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+    unsigned char* const lds = smem + wave * T::BYTES;
+
+    Work w;
+    if (!find_work<16>(a, w)) return;
+    const Row row = find_row<16>(a, w, m);
+    int t0, t1;
+    find_keys(w, row, 4, t0, t1);
+
+    // first block's loads, then q while they are on the way
+    FewLoad<FMT, D> next;
+    KeyPages kp = {{-1, -1}}, kn = {{-1, -1}};
+    int t = uniform(t0 + wave);
+    if (t < t1) {
+        kp = key_pages(a, w, t);
+        few_load(next, a, w, t, kp);
+        if (t + 4 < t1) kn = key_pages(a, w, t + 4);
+    }
+
+    // q: this lane's values of its row, eight of each group, times a power of two that puts the row's largest below 2^15
+    half8_t qh[NG], ql[NG];
+    float qsum[NG], top = 0.f;
+    {
+        f32x4_t v[NG][2];
+        const float* const src = a.a.q + (row.real ? row.t * a.a.q_stride + (size_t)row.h * D : 0) + 8 * q;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[g][i] = row.real ? *(const f32x4_t*)(src + 32 * g + 4 * i) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[g][i][e]));
+            }
+        top = quarters_max(top);
+        const int up = top > 0.f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float x[8], sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_ldexpf(v[g][i >> 2][i & 3], up);
+                sum += x[i];
+            }
+            // the order of the codes' conversion: words of four codes as 0, 2, 1, 3 (q8), eight nibbles as 0, 4, 1, 5, ... (q4)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int s = Q4 ? (i >> 1) + 4 * (i & 1) : (i & 4) + ((i & 1) << 1) + ((i >> 1) & 1);
+                qh[g][i] = (_Float16)x[s];
+                ql[g][i] = (_Float16)(x[s] - (float)qh[g][i]);
+            }
+            qsum[g] = Q4 ? quarters_sum(sum) : 0.f;
+        }
+        top = __builtin_amdgcn_ldexpf(a.a.scale, -up);
+    }
+    const bool cap = a.a.softcap > 0.f;
+    const float xs = cap ? top / a.a.softcap : top * ATTN_LOG2E, ys = a.a.softcap * ATTN_LOG2E;
+
+    // no mask inside [all_lo, all_hi)
+    const int all_lo = wave_max(row.real ? row.lo : 0), all_hi = wave_min(row.hi);
+
+    f32x4_t o[2 * NG];
+    float om[NG], M = ATTN_NONE, l = 0.f;
+#pragma unroll
+    for (int n = 0; n < 2 * NG; ++n) o[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) om[g] = 0.f;
+
+    // row of V that this lane's address names in a transposed read: keys 4 q .. 4 q + 3 of both 16-key halves
+    const int vrow = ((lane & 15) >> 3) * 16 + 4 * q + (((lane & 15) >> 1) & 3);
+
+    for (; t < t1; t += 4) {
+        wave_lds_fence();
+        few_spread(next, lds);
+        const bool have[2] = {kp.p[0] >= 0, kp.p[1] >= 0};
+        if (t + 4 < t1) {
+            kp = kn;
+            few_load(next, a, w, t + 4, kp);
+            if (t + 8 < t1) kn = key_pages(a, w, t + 8);
+        }
+        wave_lds_fence();
+        // e_j of the 32 keys
+        {
+            const uint16_t* const s = (const uint16_t*)(lds + T::VS) + (lane & 31) * NG;
+            uint32_t top16 = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) top16 = max(top16, (uint32_t)s[g] & 0x7fffu);
+            *(float*)(lds + T::E + 4 * (lane & 31)) = (float)((int)(top16 >> 10) - 14);
+        }
+        // scores: y[4 i + r] of key 16 i + 4 q + r
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u32x2_t s[NG];
+            f32x4_t mn[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                s[g] = *(const u32x2_t*)(lds + T::KS + (16 * i + 4 * q) * 2 * NG + 8 * g);
+                if constexpr (Q4) mn[g] = *(const f32x4_t*)(lds + T::KM + (16 * i + 4 * q) * 4 * NG + 16 * g);
+            }
+            const int krow = 16 * i + m;
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                half8_t k;
+                if constexpr (Q4) {
+                    int chunk = g + T::rot(krow);
+                    chunk = chunk >= T::CH ? chunk - T::CH : chunk;
+                    const uint32_t c = *(const uint32_t*)(lds + T::K + krow * 16 * T::CH + 16 * chunk + 4 * q);
+                    k = centred_q4(c, c >> 4, c >> 8, c >> 12);
+                } else {
+                    int chunk = 2 * g + (q >> 1) + T::rot(krow);
+                    chunk = chunk >= T::CH ? chunk - T::CH : chunk;
+                    const u32x2_t c = *(const u32x2_t*)(lds + T::K + krow * 16 * T::CH + 16 * chunk + 8 * (q & 1));
+                    k = halves_q8(c.x, c.y);
+                }
+                floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[g], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[g], acc, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = fmaf(half_of(s, r * NG + g), acc[r], x[r]);
+                    if constexpr (Q4) x[r] = fmaf(mn[(r * NG + g) >> 2][(r * NG + g) & 3], qsum[g], x[r]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[4 * i + r] = x[r] * xs;
+        }
+        if (cap) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = ys * attn_tanh(y[i]);
+        }
+        const bool whole = 32 * t >= all_lo && 32 * t + 32 <= all_hi && have[0] && have[1];
+        uint32_t seen = 0xffu;
+        if (!whole) {
+            seen = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = 32 * t + 16 * (i >> 2) + 4 * q + (i & 3);
+                const bool in = key >= row.lo && key < row.hi && have[i >> 2];
+                seen |= (uint32_t)in << i;
+                y[i] = in ? y[i] : -__builtin_inff();
+            }
+        }
+        wave_lds_fence();
+        const f32x4_t e0 = *(const f32x4_t*)(lds + T::E + 16 * q), e1 = *(const f32x4_t*)(lds + T::E + 64 + 16 * q);
+        float tm = ATTN_NONE;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, fmaxf(y[i] + e0[i], y[4 + i] + e1[i]));
+        if (__any(tm > M + 8.f)) {
+            const float Mn = fmaxf(M, quarters_max(tm)), f = __builtin_amdgcn_exp2f(M - Mn);
+            M = Mn;
+            l *= f;
+#pragma unroll
+            for (int n = 0; n < 2 * NG; ++n) o[n] *= f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) om[g] *= f;
+        }
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(y[i] - (M - 7.f));
+            l += p[i];
+        }
+        u32x2_t s0[NG], s1[NG];
+        f32x4_t m0[NG], m1[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            s0[g] = *(const u32x2_t*)(lds + T::VS + 4 * q * 2 * NG + 8 * g);
+            s1[g] = *(const u32x2_t*)(lds + T::VS + (16 + 4 * q) * 2 * NG + 8 * g);
+            if constexpr (Q4) {
+                m0[g] = *(const f32x4_t*)(lds + T::VM + 4 * q * 4 * NG + 16 * g);
+                m1[g] = *(const f32x4_t*)(lds + T::VM + (16 + 4 * q) * 4 * NG + 16 * g);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            half8_t ph, pl;
+            float ps[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ps[i] = p[i] * (i < 4 ? half_of(s0, i * NG + g) : half_of(s1, (i - 4) * NG + g));
+                float pm = p[i];
+                if (!whole) {                            // 0 times an infinity or a NaN of a token that is not seen
+                    const bool in = (seen >> i) & 1;
+                    ps[i] = in ? ps[i] : 0.f;
+                    if constexpr (Q4) pm *= in ? (i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3]) : 0.f;
+                } else {
+                    if constexpr (Q4) pm *= i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3];
+                }
+                if constexpr (Q4) om[g] += pm;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                // the order of V's conversion: keys 0, 2, 1, 3 of each half
+                const float u = ps[(i & 4) + ((i & 2) >> 1)], v = ps[(i & 4) + ((i & 2) >> 1) + 2];
+                const half2_t h = halves(u, v), e = halves(u - (float)h.x, v - (float)h.y);
+                ph[i] = h.x;
+                ph[i + 1] = h.y;
+                pl[i] = e.x;
+                pl[i + 1] = e.y;
+            }
+            if constexpr (Q4) {
+                int chunk = g + T::rot(vrow);
+                chunk = chunk >= T::CH ? chunk - T::CH : chunk;
+                const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(lds + T::V + vrow * 16 * T::CH + 16 * chunk + 8 * (lane & 1)));
+                const uint32_t c0 = (uint32_t)c.x, c1 = (uint32_t)c.y;
+                const half8_t lo = centred_q4(c0, c0 >> 8, c1, c1 >> 8), hi = centred_q4(c0 >> 4, c0 >> 12, c1 >> 4, c1 >> 12);
+                o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ph, o[2 * g], 0, 0, 0);
+                o[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ph, o[2 * g + 1], 0, 0, 0);
+                o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pl, o[2 * g], 0, 0, 0);
+                o[2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pl, o[2 * g + 1], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    int chunk = 2 * g + j + T::rot(vrow);
+                    chunk = chunk >= T::CH ? chunk - T::CH : chunk;
+                    const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(lds + T::V + vrow * 16 * T::CH + 16 * chunk + 8 * (lane & 1)));
+                    const half8_t v = halves_q8((uint32_t)c.x, (uint32_t)c.y);
+                    o[2 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[2 * g + j], 0, 0, 0);
+                    o[2 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[2 * g + j], 0, 0, 0);
+                }
+            }
+        }
+    }
+
+    // the four waves' results joined in LDS
+    l = quarters_sum(l);
+    if (q == 0) {
+        joinm[wave][m] = M;
+        joinl[wave][m] = l;
+    }
+    __syncthreads();
+    float Mb = fmaxf(fmaxf(joinm[0][m], joinm[1][m]), fmaxf(joinm[2][m], joinm[3][m]));
+    const float f = __builtin_amdgcn_exp2f(M - Mb);
+    float* const mine = (float*)lds + m * T::OS;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        if constexpr (Q4) {
+            const float add = quarters_sum(om[g]);
+            // tile 2 g + j, row 4 q + r holds value 32 g + 2 (4 q + r) + j
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f32x4_t v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (o[2 * g + (i & 1)][2 * h + (i >> 1)] + add) * f;
+                *(f32x4_t*)(mine + 32 * g + 8 * q + 4 * h) = v;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) *(f32x4_t*)(mine + 32 * g + 16 * j + 4 * q) = o[2 * g + j] * f;
+        }
+    }
+    __syncthreads();
+    const int G = a.a.heads / a.c.heads, slots = a.prefix_splits + a.own_splits;
+    const size_t all = (size_t)a.s.rows * a.a.heads;
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
+        const int rel = (w.r0 + r) / G;
+        if (rel >= w.count) continue;
+        if (w.prefix && a.s.row_off && w.first + rel >= a.s.row_off[a.s.seqs]) continue;
+        const int tok = w.first + rel, h = w.head * G + w.r0 + r - rel * G;
+        float Mr = joinm[0][r], L = 0.f;
+#pragma unroll
+        for (int k = 1; k < 4; ++k) Mr = fmaxf(Mr, joinm[k][r]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) L += joinl[k][r] * __builtin_amdgcn_exp2f(joinm[k][r] - Mr);
+        f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v += *(const f32x4_t*)((const float*)(smem + k * T::BYTES) + r * T::OS + d);
+        if (slots == 1) {
+            *(f32x4_t*)(a.a.out + tok * a.a.out_stride + (size_t)h * D + d) = L == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : v / L;
+        } else {
+            const size_t at = w.slot * all + (size_t)tok * a.a.heads + h;
+            if (L != 0.f) *(f32x4_t*)(a.part + at * D + d) = v;
+            if (d == 0) {
+                a.ml[2 * at] = Mr;
+                a.ml[2 * at + 1] = L;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+#define BRIK_ATTN_FEW(D)                                                                                                             \
+    extern "C" __global__ __launch_bounds__(256) void brik_attn_few_q8_##D(brik_attn_launch a) { few_body<FMT_Q8, D>(a); }             \
+    extern "C" __global__ __launch_bounds__(256) void brik_attn_few_q4_##D(brik_attn_launch a) { few_body<FMT_Q4, D>(a); }
+BRIK_ATTN_FEW(64)
+BRIK_ATTN_FEW(96)
+BRIK_ATTN_FEW(128)
+BRIK_ATTN_FEW(192)
+BRIK_ATTN_FEW(256)

@@ -10,31 +10,10 @@
 // quantization group is 8 neighbouring lanes; sums over a head and the scales of a group are cross-lane reductions, and
 // no value passes through LDS. A block works on one row: its cosines and sines are computed once in LDS and serve
 // all its heads.
-#include "attn_abi.h"
+#include "attn_common.h"
 #include "encode.h"
 
 namespace {
-
-// The sequence of row t: how many of row_off[1..seqs] are at most t. One load round trip per 64 sequences.
-__device__ __forceinline__ int seq_of_row(const brik_step& s, int t)
-{
-    if (!s.row_off) return t / s.per_seq;
-    const int lane = threadIdx.x & 63;
-    int count = 0;
-    for (int base = 0; base < s.seqs; base += 64) {
-        const int i = base + lane;
-        const int32_t end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
-        count += __popcll(__ballot(end <= t));
-    }
-    return count;
-}
-
-// The position of row t of sequence b.
-__device__ __forceinline__ int32_t row_position(const brik_step& s, int b, int t)
-{
-    const int32_t end = s.row_off ? s.row_off[b + 1] : (b + 1) * s.per_seq;
-    return s.kv_len[b] - end + t;
-}
 
 // cos and sin of an angle in radians, |a| < 2^31: a - n pi/2 by two fused multiply-adds with pi/2 in two parts (n has
 // up to 31 bits, so the first difference is exact to 2^-53 and the second part's error is below 2^-75), then the
