@@ -5,6 +5,8 @@
 
 namespace {
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
 constexpr float ATTN_LOG2E = 1.44269504088896340736f;
 constexpr float ATTN_NONE = -1e30f;      // reference exponent of a row that has seen no key
 
@@ -239,12 +241,21 @@ __device__ __forceinline__ KeyPages key_pages(const brik_attn_launch& a, const W
     return k;
 }
 
+// Both values as halves, to nearest (one instruction).
 __device__ __forceinline__ half2_t halves(float a, float b)
 {
-    half2_t h;
-    h.x = (_Float16)a;
-    h.y = (_Float16)b;
-    return h;
+    const f32x2_t v = {a, b};
+    return __builtin_convertvector(v, half2_t);
+}
+
+// v less half I of h, exact (one mixed-precision instruction; the compiler would convert and subtract).
+template <int I>
+__device__ __forceinline__ float residual(half2_t h, float v)
+{
+    float r;
+    if constexpr (I == 0) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(v));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(v));
+    return r;
 }
 
 // tanh in f32: the exponential, and near 0, where that cancels, the odd series (next term below 2^-28 of the value).

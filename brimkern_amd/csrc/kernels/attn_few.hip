@@ -18,6 +18,8 @@
 // written rotated by row so that reading a column of chunks meets every bank once.
 #include "attn_common.h"
 
+#include <type_traits>
+
 namespace {
 
 template <int FMT, int D>
@@ -46,41 +48,56 @@ struct FewLoad {
     uint32_t ks[T::HP * T::SI], vs[T::HP * T::SI];
 };
 
-template <int FMT, int D>
-__device__ __forceinline__ void few_load(FewLoad<FMT, D>& f, const brik_attn_launch& a, const Work& w, int t, const KeyPages& kp)
+// Loads the 32 vectors from `v0` on, those of row r moved by `moved(r)` vectors: uniform base addresses and lane offsets that
+// do not change from block to block.
+template <int FMT, int D, class F>
+__device__ __forceinline__ void few_fetch(FewLoad<FMT, D>& f, const brik_attn_launch& a, size_t v0, F moved)
 {
     using T = FewTile<FMT, D>;
-    const int lane = threadIdx.x & 63, slot = (32 * t) & ((1 << a.s.shift) - 1);
-    // vectors of the first key and of the 17th (on page 0 where there is none: read and not used)
-    const size_t v0 = (((size_t)max(kp.p[0], 0) * a.c.heads + w.head) << a.s.shift) + slot;
-    const size_t v1 = a.s.shift > 4 ? v0 + 16 : ((size_t)max(kp.p[1], 0) * a.c.heads + w.head) << 4;
+    const int lane = threadIdx.x & 63;
+    const uint8_t* const kb = (const uint8_t*)a.c.k + v0 * (16 * T::CH);
+    const uint8_t* const vb = (const uint8_t*)a.c.v + v0 * (16 * T::CH);
 #pragma unroll
     for (int i = 0; i < T::NI; ++i) {
         const int c = 64 * i + lane, row = c / T::CH;
         if (T::CH % 2 && c >= 32 * T::CH) break;
         int chunk = c - row * T::CH - T::rot(row);
         chunk = chunk < 0 ? chunk + T::CH : chunk;
-        const size_t at = ((row < 16 ? v0 : v1) + (row & 15)) * (size_t)(16 * T::CH) + 16 * chunk;
-        f.k[i] = *(const u32x4_t*)((const uint8_t*)a.c.k + at);
-        f.v[i] = *(const u32x4_t*)((const uint8_t*)a.c.v + at);
+        const uint32_t off = 16u * (uint32_t)(row * T::CH + chunk);
+        const size_t far = moved(row) * (16 * T::CH);
+        f.k[i] = *(const u32x4_t*)(kb + far + off);
+        f.v[i] = *(const u32x4_t*)(vb + far + off);
     }
+    const size_t h0 = v0 * (2 * T::NG);                  // bytes
 #pragma unroll
     for (int i = 0; i < T::SI; ++i) {
         const int d = 64 * i + lane;
         if (d < T::SD) {
-            const bool first = d < T::SD / 2;
-            const size_t at = (first ? v0 : v1) * T::NG / 2 + (first ? d : d - T::SD / 2);          // dwords: two halves each
-            f.ks[i] = ((const uint32_t*)a.c.k_scales)[at];
-            f.vs[i] = ((const uint32_t*)a.c.v_scales)[at];
+            const uint32_t off = 4u * (uint32_t)d;
+            const size_t far = moved(d < T::SD / 2 ? 0 : 16) * (2 * T::NG);
+            f.ks[i] = *(const uint32_t*)((const uint8_t*)a.c.k_scales + h0 + far + off);
+            f.vs[i] = *(const uint32_t*)((const uint8_t*)a.c.v_scales + h0 + far + off);
             if constexpr (FMT == FMT_Q4) {
-                f.ks[T::SI + i] = ((const uint32_t*)a.c.k_mins)[at];
-                f.vs[T::SI + i] = ((const uint32_t*)a.c.v_mins)[at];
+                f.ks[T::SI + i] = *(const uint32_t*)((const uint8_t*)a.c.k_mins + h0 + far + off);
+                f.vs[T::SI + i] = *(const uint32_t*)((const uint8_t*)a.c.v_mins + h0 + far + off);
             }
         }
     }
 }
 
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
+template <int FMT, int D>
+__device__ __forceinline__ void few_load(FewLoad<FMT, D>& f, const brik_attn_launch& a, const Work& w, int t, const KeyPages& kp)
+{
+    const int slot = (32 * t) & ((1 << a.s.shift) - 1);
+    // vectors of the first key and of the 17th (on page 0 where there is none: read and not used)
+    const size_t v0 = (((size_t)max(kp.p[0], 0) * a.c.heads + w.head) << a.s.shift) + slot;
+    if (a.s.shift > 4) {
+        few_fetch<FMT, D>(f, a, v0, [](int) { return (size_t)0; });
+    } else {
+        const size_t v1 = ((size_t)max(kp.p[1], 0) * a.c.heads + w.head) << 4, jump = v1 - (v0 + 16);
+        few_fetch<FMT, D>(f, a, v0, [=](int row) { return row < 16 ? (size_t)0 : jump; });
+    }
+}
 
 __device__ __forceinline__ f32x2_t centred_mins(uint32_t s, uint32_t m)
 {
@@ -249,16 +266,8 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
     // row of V that this lane's address names in a transposed read: keys 4 q .. 4 q + 3 of both 16-key halves
     const int vrow = ((lane & 15) >> 3) * 16 + 4 * q + (((lane & 15) >> 1) & 3);
 
-    for (; t < t1; t += 4) {
-        wave_lds_fence();
-        few_spread(next, lds);
-        const bool have[2] = {kp.p[0] >= 0, kp.p[1] >= 0};
-        if (t + 4 < t1) {
-            kp = kn;
-            few_load(next, a, w, t + 4, kp);
-            if (t + 8 < t1) kn = key_pages(a, w, t + 8);
-        }
-        wave_lds_fence();
+    // One block of keys, in LDS. masked: some of its keys are not seen by some row.
+    auto block = [&](auto masked, int t, const bool (&have)[2]) {
         // e_j of the 32 keys
         {
             const uint16_t* const s = (const uint16_t*)(lds + T::VS) + (lane & 31) * NG;
@@ -310,10 +319,8 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = ys * attn_tanh(y[i]);
         }
-        const bool whole = 32 * t >= all_lo && 32 * t + 32 <= all_hi && have[0] && have[1];
-        uint32_t seen = 0xffu;
-        if (!whole) {
-            seen = 0;
+        uint32_t seen = 0;
+        if constexpr (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = 32 * t + 16 * (i >> 2) + 4 * q + (i & 3);
@@ -355,31 +362,27 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            half8_t ph, pl;
+            u32x4_t phw, plw;
             float ps[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                ps[i] = p[i] * (i < 4 ? half_of(s0, i * NG + g) : half_of(s1, (i - 4) * NG + g));
-                float pm = p[i];
-                if (!whole) {                            // 0 times an infinity or a NaN of a token that is not seen
-                    const bool in = (seen >> i) & 1;
-                    ps[i] = in ? ps[i] : 0.f;
-                    if constexpr (Q4) pm *= in ? (i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3]) : 0.f;
-                } else {
-                    if constexpr (Q4) pm *= i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3];
+                ps[i] = fmaf(i < 4 ? half_of(s0, i * NG + g) : half_of(s1, (i - 4) * NG + g), p[i], 0.f);
+                // 0 times an infinity or a NaN of a token that is not seen
+                if constexpr (masked) ps[i] = (seen >> i) & 1 ? ps[i] : 0.f;
+                if constexpr (Q4) {
+                    const float mn = i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3];
+                    om[g] = fmaf(p[i], !masked || ((seen >> i) & 1) ? mn : 0.f, om[g]);
                 }
-                if constexpr (Q4) om[g] += pm;
             }
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 // the order of V's conversion: keys 0, 2, 1, 3 of each half
                 const float u = ps[(i & 4) + ((i & 2) >> 1)], v = ps[(i & 4) + ((i & 2) >> 1) + 2];
-                const half2_t h = halves(u, v), e = halves(u - (float)h.x, v - (float)h.y);
-                ph[i] = h.x;
-                ph[i + 1] = h.y;
-                pl[i] = e.x;
-                pl[i + 1] = e.y;
+                const half2_t h = halves(u, v);
+                phw[i / 2] = __builtin_bit_cast(uint32_t, h);
+                plw[i / 2] = __builtin_bit_cast(uint32_t, halves(residual<0>(h, u), residual<1>(h, v)));
             }
+            const half8_t ph = __builtin_bit_cast(half8_t, phw), pl = __builtin_bit_cast(half8_t, plw);
             if constexpr (Q4) {
                 int chunk = g + T::rot(vrow);
                 chunk = chunk >= T::CH ? chunk - T::CH : chunk;
@@ -402,6 +405,20 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
                 }
             }
         }
+    };
+
+    for (; t < t1; t += 4) {
+        const bool have[2] = {kp.p[0] >= 0, kp.p[1] >= 0};
+        wave_lds_fence();
+        few_spread(next, lds);
+        if (t + 4 < t1) {
+            kp = kn;
+            few_load(next, a, w, t + 4, kp);
+            if (t + 8 < t1) kn = key_pages(a, w, t + 8);
+        }
+        wave_lds_fence();
+        if (32 * t >= all_lo && 32 * t + 32 <= all_hi && have[0] && have[1]) block(std::false_type{}, t, have);
+        else block(std::true_type{}, t, have);
     }
 
     // the four waves' results joined in LDS
@@ -464,8 +481,8 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 }  // namespace
 
 #define BRIK_ATTN_FEW(D)                                                                                                             \
-    extern "C" __global__ __launch_bounds__(256) void brik_attn_few_q8_##D(brik_attn_launch a) { few_body<FMT_Q8, D>(a); }             \
-    extern "C" __global__ __launch_bounds__(256) void brik_attn_few_q4_##D(brik_attn_launch a) { few_body<FMT_Q4, D>(a); }
+    extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void brik_attn_few_q8_##D(brik_attn_launch a) { few_body<FMT_Q8, D>(a); }             \
+    extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void brik_attn_few_q4_##D(brik_attn_launch a) { few_body<FMT_Q4, D>(a); }
 BRIK_ATTN_FEW(64)
 BRIK_ATTN_FEW(96)
 BRIK_ATTN_FEW(128)
