@@ -55,8 +55,8 @@ const char* const kKernelNames[K_COUNT] = {
 };
 
 // Kernels of the attention side's code object. Teams of 8, 16, 32, 64 lanes: brik_rows_<rope, q8, q4>_<lanes>.
-// Attention of up to 16 rows a tile: brik_attn_few_<fmt>_<head_dim>.
-enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_JOIN = A_FEW + 10, A_COUNT };
+// Attention by tiles of 16 rows, brik_attn_few_<fmt>_<head_dim>, and of 128, brik_attn_tile_<fmt>_<head_dim>.
+enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE = A_FEW + 10, A_JOIN = A_TILE + 10, A_COUNT };
 constexpr int kAttnDims[5] = {64, 96, 128, 192, 256};
 
 // GEMV variants {team, r, u, d}, in the order of BRIK_GEMV_FMT in gemv.hip: TEAM lanes per row team,
@@ -1443,7 +1443,8 @@ int brik_create(int device, brik_ctx** out)
         const char* const rows[3] = {"rope", "q8", "q4"};
         if (k < A_READ) snprintf(name, sizeof name, "brik_rows_%s_%d", rows[k / 4], 8 << k % 4);
         else if (k < A_FEW) snprintf(name, sizeof name, "brik_kv_read_%s", kFmtNames[k - A_READ]);
-        else if (k < A_JOIN) snprintf(name, sizeof name, "brik_attn_few_%s_%d", kFmtNames[(k - A_FEW) / 5], kAttnDims[(k - A_FEW) % 5]);
+        else if (k < A_JOIN) snprintf(name, sizeof name, "brik_attn_%s_%s_%d", k < A_TILE ? "few" : "tile",
+                                    kFmtNames[(k - A_FEW) % 10 / 5], kAttnDims[(k - A_FEW) % 5]);
         else snprintf(name, sizeof name, "brik_attn_join");
         if (hipModuleGetFunction(&c->attn_fn[k], c->attn_module, name) != hipSuccess) return bail(BRIK_EMODULE);
     }
@@ -2541,14 +2542,17 @@ static int attn_splits(long blocks, long keys)
 
 static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
 {
-    constexpr int BM = 16;
     const long KV = a.c.heads, G = a.a.heads / KV, rows = a.s.rows;
     const long own_keys = std::min<long>((long)a.s.max_len - a.s.prefix_len, (long)a.s.table_cols << a.s.shift);
     const long prefix_keys = std::min(a.s.prefix_len, a.s.max_len);
+    const long most = a.s.row_off ? std::min<long>(max_rows ? max_rows : rows, rows) : a.s.per_seq;    // rows of a sequence
+    int dim = 0;
+    while (kAttnDims[dim] != a.c.head_dim) ++dim;
+    const int which = 5 * (a.c.fmt == BRIK_FMT_Q4) + dim;
+    // Rows of one tile of the 16-row kernel: that one, else the 128-row kernel, each section by itself.
+    const int own_bm = most * G <= 16 ? 16 : 128, prefix_bm = rows * G <= 16 ? 16 : 128;
     // row tiles of the sequences: the same number for each where that is not many more than there can be
-    const long most = max_rows ? std::min<long>(max_rows, rows) : rows;
-    const long per_seq = a.s.row_off ? (most * G + BM - 1) / BM : (a.s.per_seq * G + BM - 1) / BM;
-    const long bound = (rows * G + BM - 1) / BM + a.s.seqs;
+    const long per_seq = (most * G + own_bm - 1) / own_bm, bound = (rows * G + own_bm - 1) / own_bm + a.s.seqs;
     long tiles = per_seq * a.s.seqs;
     a.tiles_per_seq = (int)per_seq;
     if (a.s.row_off && tiles > 2 * bound) {
@@ -2557,7 +2561,7 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     }
     a.own_splits = attn_splits(KV * tiles, own_keys);
     if (prefix_keys > 0) {
-        a.prefix_tiles = (int)((rows * G + BM - 1) / BM);
+        a.prefix_tiles = (int)((rows * G + prefix_bm - 1) / prefix_bm);
         a.prefix_splits = attn_splits(KV * a.prefix_tiles, prefix_keys);
     }
     const int slots = a.prefix_splits + a.own_splits;
@@ -2567,12 +2571,18 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         a.part = static_cast<float*>(c->aws);
         a.ml = a.part + vectors * d;
     }
-    const long blocks = KV * (tiles * a.own_splits + (long)a.prefix_tiles * a.prefix_splits);
-    if (blocks >= (1l << 24)) return fail(c, BRIK_EINVAL, "attention: %ld blocks in one call", blocks);
-    int dim = 0;
-    while (kAttnDims[dim] != a.c.head_dim) ++dim;
+    const long own_blocks = KV * tiles * a.own_splits, prefix_blocks = KV * a.prefix_tiles * a.prefix_splits;
+    if (own_blocks + prefix_blocks >= (1l << 24)) return fail(c, BRIK_EINVAL, "attention: %ld blocks in one call", own_blocks + prefix_blocks);
+    auto kernel = [&](int bm) { return c->attn_fn[(bm == 16 ? A_FEW : A_TILE) + which]; };
     void* args[] = {&a};
-    HIP_TRY_RC(launch_fn(c, c->attn_fn[A_FEW + 5 * (a.c.fmt == BRIK_FMT_Q4) + dim], (unsigned)blocks, 1, 256, 0, args));
+    if (prefix_blocks && prefix_bm != own_bm) {
+        // two launches: the kernels see the blocks from `first_block` on
+        HIP_TRY_RC(launch_fn(c, kernel(prefix_bm), (unsigned)prefix_blocks, 1, 256, 0, args));
+        a.first_block = (int)prefix_blocks;
+        HIP_TRY_RC(launch_fn(c, kernel(own_bm), (unsigned)own_blocks, 1, 256, 0, args));
+    } else {
+        HIP_TRY_RC(launch_fn(c, kernel(own_bm), (unsigned)(own_blocks + prefix_blocks), 1, 256, 0, args));
+    }
     if (slots > 1) return launch_fn(c, c->attn_fn[A_JOIN], (unsigned)rows, (unsigned)a.a.heads, 256, 0, args);
     return BRIK_OK;
 }

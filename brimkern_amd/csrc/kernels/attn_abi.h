@@ -92,4 +92,5 @@ typedef struct brik_attn_launch {
     // split over so many blocks; slots: prefix_splits, then own_splits. tiles_per_seq: the tile's sequence by division (0:
     // by a search over the sequences' rows).
     int32_t prefix_tiles, prefix_splits, own_splits, tiles_per_seq;
+    int32_t first_block;   // number of the launch's first block
 } brik_attn_launch;

@@ -44,14 +44,31 @@ __device__ __forceinline__ float quarters_sum(float v)
     return a + b;
 }
 
+// Maximum over the 32 lanes of a half wave.
+__device__ __forceinline__ float half_max(float v)
+{
+    v = BRIK_DPP_MAX(v, DPP_QUAD_1032);
+    v = BRIK_DPP_MAX(v, DPP_QUAD_2301);
+    v = BRIK_DPP_MAX(v, DPP_ROW_ROR4);
+    v = BRIK_DPP_MAX(v, DPP_ROW_ROR8);
+    float a, b;
+    quarter_pair(v, a, b);
+    return fmaxf(a, b);
+}
+
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Min / max over the 64 lanes (uniform result).
 __device__ __forceinline__ int wave_min(int v)
 {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = min(v, __shfl_xor(v, m));
-    return uniform(v);
+    v = min(v, __builtin_amdgcn_mov_dpp(v, DPP_QUAD_1032, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_mov_dpp(v, DPP_QUAD_2301, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_mov_dpp(v, DPP_ROW_ROR4, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_mov_dpp(v, DPP_ROW_ROR8, 0xF, 0xF, false));
+    const auto q = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = min((int)q[0], (int)q[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    return uniform(min((int)h[0], (int)h[1]));
 }
 __device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
 
@@ -140,7 +157,7 @@ template <int BM>
 __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
 {
     const int KV = a.c.heads, G = a.a.heads / KV;
-    int id = blockIdx.x;
+    int id = a.first_block + blockIdx.x;
     w.head = id % KV;
     id /= KV;
     const int pre = a.prefix_tiles * a.prefix_splits;
@@ -183,12 +200,13 @@ struct Row {
     int lo, hi;
 };
 
-template <int BM>
-__device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w, int m)
+// Row m of the ROWS rows from r0 on, counted over count * G.
+template <int ROWS>
+__device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w, int r0, int m)
 {
     const int G = a.a.heads / a.c.heads;
     Row r;
-    const int i = w.r0 + m, rel = i / G;
+    const int i = r0 + m, rel = i / G;
     r.real = rel < w.count;
     r.t = w.first + rel;
     r.h = w.head * G + i - rel * G;
@@ -196,24 +214,23 @@ __device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w
     r.hi = 0x7fffffff;
     int b = w.b;
     if (w.prefix) {
-        const int t0 = uniform(w.r0 / G), last = min((w.r0 + BM - 1) / G, a.s.rows - 1);
+        const int t0 = uniform(r0 / G), last = min((r0 + ROWS - 1) / G, a.s.rows - 1);
         b = seq_of_lane(a.s, r.t, t0, uniform(last) - t0 + 1);
         r.real = r.real && b < a.s.seqs;
     }
     if (!r.real) return r;
     const int32_t pos = row_position(a.s, b, r.t), first = w.prefix ? 0 : a.s.prefix_len;
     const int32_t end = w.prefix ? min(a.s.prefix_len, a.s.max_len)
-                                 : (int32_t)min((long long)a.s.max_len - first, (long long)a.s.table_cols << a.s.shift);
+                                 : (int32_t)min((long long)a.s.max_len - first, min((long long)a.s.table_cols << a.s.shift, 0x7fffffc0ll));
     r.hi = max(0, min(pos + 1 - first, end));
     r.lo = a.a.window ? max(0, pos - a.a.window + 1 - first) : 0;
     return r;
 }
 
-// The tile's key blocks [t0, t1) of 32 keys that this split works on: the blocks that any row sees, divided over the
-// splits in pieces of at least `least`.
-__device__ __forceinline__ void find_keys(const Work& w, const Row& r, int least, int& t0, int& t1)
+// The key blocks [t0, t1) of 32 keys that this split works on: those of the keys [lo, hi) that any row sees, divided over
+// the splits in pieces of at least `least`.
+__device__ __forceinline__ void find_keys(const Work& w, int lo, int hi, int least, int& t0, int& t1)
 {
-    const int lo = wave_min(r.real ? r.lo : 0x7fffffff), hi = wave_max(r.real ? r.hi : 0);
     t0 = t1 = 0;
     if (lo >= hi) return;
     const int first = lo >> 5, n = ((hi + 31) >> 5) - first;
@@ -239,6 +256,41 @@ __device__ __forceinline__ KeyPages key_pages(const brik_attn_launch& a, const W
         k.p[i] = (uint32_t)id < (uint32_t)a.s.pages ? id : -1;
     }
     return k;
+}
+
+// Eight int8 codes as f16, the bytes of each word in the order 0, 2, 1, 3: 1024 + (c + 128) has the code's bits in its low
+// byte, and the subtraction is exact.
+__device__ __forceinline__ half8_t halves_q8(uint32_t w0, uint32_t w1)
+{
+    const half2_t off = {(_Float16)-1152.f, (_Float16)-1152.f};
+    half8_t r;
+    w0 ^= 0x80808080u;
+    w1 ^= 0x80808080u;
+    const uint32_t u[4] = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04020400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030401u),
+                           __builtin_amdgcn_perm(0x64646464u, w1, 0x04020400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030401u)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2_t h = __builtin_bit_cast(half2_t, u[i]) + off;
+        r[2 * i] = h.x;
+        r[2 * i + 1] = h.y;
+    }
+    return r;
+}
+
+// Codes in the low nibbles of each 16 bits as f16 less 8. The products of values have to be of both signs: the matrix
+// cores' sums cut the bits that do not fit, and over sums of nearly equal terms that shows (7e-5 with codes from 0).
+__device__ __forceinline__ half8_t centred_q4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    const half2_t off = {(_Float16)-1032.f, (_Float16)-1032.f};
+    const uint32_t u[4] = {a, b, c, d};
+    half8_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const half2_t h = __builtin_bit_cast(half2_t, (u[i] & 0x000f000fu) | 0x64006400u) + off;
+        r[2 * i] = h.x;
+        r[2 * i + 1] = h.y;
+    }
+    return r;
 }
 
 // Both values as halves, to nearest (one instruction).

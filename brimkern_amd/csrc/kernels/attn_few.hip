@@ -145,41 +145,6 @@ __device__ __forceinline__ void wave_lds_fence()
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
 
-// Eight int8 codes as f16, the bytes of each word in the order 0, 2, 1, 3: 1024 + (c + 128) has the code's bits in its low
-// byte, and the subtraction is exact.
-__device__ __forceinline__ half8_t halves_q8(uint32_t w0, uint32_t w1)
-{
-    const half2_t off = {(_Float16)-1152.f, (_Float16)-1152.f};
-    half8_t r;
-    w0 ^= 0x80808080u;
-    w1 ^= 0x80808080u;
-    const uint32_t u[4] = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04020400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030401u),
-                           __builtin_amdgcn_perm(0x64646464u, w1, 0x04020400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030401u)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const half2_t h = __builtin_bit_cast(half2_t, u[i]) + off;
-        r[2 * i] = h.x;
-        r[2 * i + 1] = h.y;
-    }
-    return r;
-}
-
-// Codes in the low nibbles of each 16 bits as f16 less 8. The products of values have to be of both signs: the matrix
-// cores' sums cut the bits that do not fit, and over sums of nearly equal terms that shows (7e-5 with codes from 0).
-__device__ __forceinline__ half8_t centred_q4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
-{
-    const half2_t off = {(_Float16)-1032.f, (_Float16)-1032.f};
-    const uint32_t u[4] = {a, b, c, d};
-    half8_t r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const half2_t h = __builtin_bit_cast(half2_t, (u[i] & 0x000f000fu) | 0x64006400u) + off;
-        r[2 * i] = h.x;
-        r[2 * i + 1] = h.y;
-    }
-    return r;
-}
-
 // Half k of the halves that a lane read of 4 keys (NG each, in order).
 template <int N>
 __device__ __forceinline__ float half_of(const u32x2_t (&v)[N], int k)
@@ -201,9 +166,9 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 
     Work w;
     if (!find_work<16>(a, w)) return;
-    const Row row = find_row<16>(a, w, m);
+    const Row row = find_row<16>(a, w, w.r0, m);
     int t0, t1;
-    find_keys(w, row, 4, t0, t1);
+    find_keys(w, wave_min(row.real ? row.lo : 0x7fffffff), wave_max(row.real ? row.hi : 0), 4, t0, t1);
 
     // first block's loads, then q while they are on the way
     FewLoad<FMT, D> next;
