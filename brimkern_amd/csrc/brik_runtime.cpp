@@ -55,8 +55,9 @@ const char* const kKernelNames[K_COUNT] = {
 };
 
 // Kernels of the attention side's code object. Teams of 8, 16, 32, 64 lanes: brik_rows_<rope, q8, q4>_<lanes>.
-// Attention by tiles of 16 rows, brik_attn_few_<fmt>_<head_dim>, and of 128, brik_attn_tile_<fmt>_<head_dim>.
-enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE = A_FEW + 10, A_JOIN = A_TILE + 10, A_COUNT };
+// Attention by tiles of 16 rows, brik_attn_few_<fmt>_<head_dim>, and of 128 and 256, brik_attn_tile<waves>_<fmt>_<head_dim>
+// (256: up to head_dim 128).
+enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE4 = A_FEW + 10, A_TILE8 = A_TILE4 + 10, A_JOIN = A_TILE8 + 10, A_COUNT };
 constexpr int kAttnDims[5] = {64, 96, 128, 192, 256};
 
 // GEMV variants {team, r, u, d}, in the order of BRIK_GEMV_FMT in gemv.hip: TEAM lanes per row team,
@@ -1443,9 +1444,10 @@ int brik_create(int device, brik_ctx** out)
         const char* const rows[3] = {"rope", "q8", "q4"};
         if (k < A_READ) snprintf(name, sizeof name, "brik_rows_%s_%d", rows[k / 4], 8 << k % 4);
         else if (k < A_FEW) snprintf(name, sizeof name, "brik_kv_read_%s", kFmtNames[k - A_READ]);
-        else if (k < A_JOIN) snprintf(name, sizeof name, "brik_attn_%s_%s_%d", k < A_TILE ? "few" : "tile",
+        else if (k < A_JOIN) snprintf(name, sizeof name, "brik_attn_%s_%s_%d", k < A_TILE4 ? "few" : k < A_TILE8 ? "tile4" : "tile8",
                                     kFmtNames[(k - A_FEW) % 10 / 5], kAttnDims[(k - A_FEW) % 5]);
         else snprintf(name, sizeof name, "brik_attn_join");
+        if (k >= A_TILE8 && k < A_JOIN && kAttnDims[(k - A_FEW) % 5] > 128) continue;
         if (hipModuleGetFunction(&c->attn_fn[k], c->attn_module, name) != hipSuccess) return bail(BRIK_EMODULE);
     }
     // the fixed scratch of brik_matmul_t_q4_noalloc, with this device current (once per device)
@@ -2549,8 +2551,9 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     int dim = 0;
     while (kAttnDims[dim] != a.c.head_dim) ++dim;
     const int which = 5 * (a.c.fmt == BRIK_FMT_Q4) + dim;
-    // Rows of one tile of the 16-row kernel: that one, else the 128-row kernel, each section by itself.
-    const int own_bm = most * G <= 16 ? 16 : 128, prefix_bm = rows * G <= 16 ? 16 : 128;
+    // Rows of one tile of the 16-row kernel: that one, else 128 or 256 rows a tile, each section by itself.
+    auto tile_rows = [&](long n) { return n <= 16 ? 16 : n <= 128 || a.c.head_dim > 128 ? 128 : 256; };
+    const int own_bm = tile_rows(most * G), prefix_bm = tile_rows(rows * G);
     // row tiles of the sequences: the same number for each where that is not many more than there can be
     const long per_seq = (most * G + own_bm - 1) / own_bm, bound = (rows * G + own_bm - 1) / own_bm + a.s.seqs;
     long tiles = per_seq * a.s.seqs;
@@ -2573,15 +2576,19 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     }
     const long own_blocks = KV * tiles * a.own_splits, prefix_blocks = KV * a.prefix_tiles * a.prefix_splits;
     if (own_blocks + prefix_blocks >= (1l << 24)) return fail(c, BRIK_EINVAL, "attention: %ld blocks in one call", own_blocks + prefix_blocks);
-    auto kernel = [&](int bm) { return c->attn_fn[(bm == 16 ? A_FEW : A_TILE) + which]; };
+    auto run = [&](int bm, long blocks) {
+        const int k = bm == 16 ? A_FEW : bm == 128 ? A_TILE4 : A_TILE8;
+        void* args[] = {&a};
+        return launch_fn(c, c->attn_fn[k + which], (unsigned)blocks, 1, bm == 256 ? 512 : 256, 0, args);
+    };
     void* args[] = {&a};
     if (prefix_blocks && prefix_bm != own_bm) {
         // two launches: the kernels see the blocks from `first_block` on
-        HIP_TRY_RC(launch_fn(c, kernel(prefix_bm), (unsigned)prefix_blocks, 1, 256, 0, args));
+        HIP_TRY_RC(run(prefix_bm, prefix_blocks));
         a.first_block = (int)prefix_blocks;
-        HIP_TRY_RC(launch_fn(c, kernel(own_bm), (unsigned)own_blocks, 1, 256, 0, args));
+        HIP_TRY_RC(run(own_bm, own_blocks));
     } else {
-        HIP_TRY_RC(launch_fn(c, kernel(own_bm), (unsigned)(own_blocks + prefix_blocks), 1, 256, 0, args));
+        HIP_TRY_RC(run(own_bm, own_blocks + prefix_blocks));
     }
     if (slots > 1) return launch_fn(c, c->attn_fn[A_JOIN], (unsigned)rows, (unsigned)a.a.heads, 256, 0, args);
     return BRIK_OK;

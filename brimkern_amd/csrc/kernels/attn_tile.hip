@@ -1,6 +1,6 @@
 // Attention of many rows over the quantized cache: prefill, and the rows of all sequences over a shared prefix.
 //
-// 128 rows a block, 32 a wave (a row: a query head of the key / value head, of a token); 32 keys a step, in LDS for all
+// 128 or 256 rows a block, 32 a wave (a row: a query head of the key / value head, of a token); 32 keys a step, in LDS for all
 // four waves, two buffers. As in attn_few.hip the products keep f32 accuracy on the f16 matrix cores, here with
 // 32x32x16 products and the conversion done once per block:
 //   scores: S^T = K Q^T; codes exact in f16 (q4: less 8), q as two halves; per group one f32 result, times the key's scale.
@@ -18,9 +18,8 @@
 
 namespace {
 
-constexpr int TILE_ROWS = 128;
-
-template <int FMT, int D>
+// NW: waves of a block, 32 rows each.
+template <int FMT, int D, int NW>
 struct TileCfg {
     static constexpr bool Q4 = FMT == FMT_Q4;
     static constexpr int NG = D / 32, U = D / 8;                       // groups, 8-value chunks of a row
@@ -31,18 +30,24 @@ struct TileCfg {
     static constexpr int KB = 32 * 16 + 16, RB = 2 * D + (2 * D % 128 ? 0 : 64);
     static constexpr int KC = 0, VH = U * KB, VL = VH + 32 * RB, KS = VL + 32 * RB, G = KS + 64 * NG, BAD = G + 128, KM = BAD + 128;
     static constexpr int BUF = KM + 1024 * MM;
-    static constexpr int ITEMS = NG;                                   // chunks a thread brings in (keys, then values)
-    static constexpr int VITEMS = (NG + 1) / 2, V0 = NG / 2;           // those that may be values: from item V0 on
-    static constexpr int SW = (NG + 1) / 2;                            // dwords of a key's scales (NG odd: padded)
-    static __device__ __forceinline__ bool value(int i) { return NG % 2 == 0 ? i >= V0 : (int)threadIdx.x + 256 * i >= 4 * D; }
+    // chunks that a thread brings in: 4 D of keys, then 4 D of values, NT at a time (kinds the same for a wave)
+    static constexpr int NT = 64 * NW, ITEMS = (8 * D + NT - 1) / NT;
+    static constexpr int V0 = 4 * D / NT, VITEMS = ITEMS - V0;         // from item V0 on they may be values
+    static constexpr bool EVEN = 4 * D % NT == 0;
+    static __device__ __forceinline__ bool value(int i) { return EVEN ? i >= V0 : (int)threadIdx.x + NT * i >= 4 * D; }
+    static __device__ __forceinline__ bool live(int i) { return (i + 1) * NT <= 8 * D || (int)threadIdx.x + NT * i < 8 * D; }
+    // A key's chunks lie in 8, 16 or 32 consecutive lanes: a thread loads its own group's scale and the key's maximum is a
+    // cross-lane one. Otherwise every thread loads all scales of its key.
+    static constexpr bool ROWS = U == 8 || U == 16 || U == 32;
+    static constexpr int SW = (NG + 1) / 2, VS = ROWS ? 1 : SW;        // dwords of a key's scales (NG odd: padded)
 };
 
 // A block of 32 keys on its way: raw codes and scales in registers.
-template <int FMT, int D>
+template <int FMT, int D, int NW>
 struct TileLoad {
-    using T = TileCfg<FMT, D>;
+    using T = TileCfg<FMT, D, NW>;
     uint32_t code[T::ITEMS][FMT == FMT_Q8 ? 2 : 1];
-    uint32_t vs[T::VITEMS][T::SW], vm[T::VITEMS][FMT == FMT_Q4 ? T::SW : 1];   // of the items that are values
+    uint32_t vs[T::VITEMS][T::VS], vm[T::VITEMS][FMT == FMT_Q4 ? T::VS : 1];   // of the items that are values
     uint32_t ks[T::SW], km[FMT == FMT_Q4 ? T::SW : 1];                           // threads 0..31: of key threadIdx.x
 };
 
@@ -66,10 +71,10 @@ __device__ __forceinline__ uint32_t half_bits(const uint32_t (&v)[N], int g)
     return g & 1 ? v[g >> 1] >> 16 : v[g >> 1] & 0xffffu;
 }
 
-template <int FMT, int D>
-__device__ __forceinline__ void tile_load(TileLoad<FMT, D>& f, const brik_attn_launch& a, const Work& w, int t, const KeyPages& kp)
+template <int FMT, int D, int NW>
+__device__ __forceinline__ void tile_load(TileLoad<FMT, D, NW>& f, const brik_attn_launch& a, const Work& w, int t, const KeyPages& kp)
 {
-    using T = TileCfg<FMT, D>;
+    using T = TileCfg<FMT, D, NW>;
     constexpr int RC = FMT == FMT_Q8 ? D : D / 2;                      // bytes of a row of codes
     const int tid = threadIdx.x, slot = (32 * t) & ((1 << a.s.shift) - 1);
     const size_t v0 = (((size_t)max(kp.p[0], 0) * a.c.heads + w.head) << a.s.shift) + slot;
@@ -79,8 +84,9 @@ __device__ __forceinline__ void tile_load(TileLoad<FMT, D>& f, const brik_attn_l
     const uint8_t* const vb = (const uint8_t*)a.c.v + v0 * RC;
 #pragma unroll
     for (int i = 0; i < T::ITEMS; ++i) {
-        const int it = tid + 256 * i;
-        const bool value = T::value(i);                                // the same for a wave
+        if (!T::live(i)) break;
+        const int it = tid + T::NT * i;
+        const bool value = T::value(i);
         const int j = value ? it - 4 * D : it, key = j / T::U, u = j - key * T::U;
         const size_t far = key < 16 ? 0 : jump;
         const uint8_t* const p = (value ? vb : kb) + far * RC + (uint32_t)(key * RC + u * (RC / T::U));
@@ -92,8 +98,15 @@ __device__ __forceinline__ void tile_load(TileLoad<FMT, D>& f, const brik_attn_l
             f.code[i][0] = *(const uint32_t*)p;
         }
         if (value) {
-            load_halves<T::NG>(f.vs[i < T::V0 ? 0 : i - T::V0], a.c.v_scales + (v0 + far + key) * T::NG);
-            if constexpr (FMT == FMT_Q4) load_halves<T::NG>(f.vm[i < T::V0 ? 0 : i - T::V0], a.c.v_mins + (v0 + far + key) * T::NG);
+            const int n = i < T::V0 ? 0 : i - T::V0;
+            const size_t at = (v0 + far + key) * T::NG;
+            if constexpr (T::ROWS) {
+                f.vs[n][0] = a.c.v_scales[at + (u >> 2)];
+                if constexpr (FMT == FMT_Q4) f.vm[n][0] = a.c.v_mins[at + (u >> 2)];
+            } else {
+                load_halves<T::NG>(f.vs[n], a.c.v_scales + at);
+                if constexpr (FMT == FMT_Q4) load_halves<T::NG>(f.vm[n], a.c.v_mins + at);
+            }
         }
     }
     if (tid < 32) {
@@ -103,14 +116,34 @@ __device__ __forceinline__ void tile_load(TileLoad<FMT, D>& f, const brik_attn_l
     }
 }
 
-template <int FMT, int D>
-__device__ __forceinline__ void tile_spread(const TileLoad<FMT, D>& f, unsigned char* buf)
+// Maximum / union over the groups of a key whose U chunks lie in U consecutive lanes, four chunks a group.
+template <int U, class F>
+__device__ __forceinline__ uint32_t key_fold(uint32_t v, F f)
 {
-    using T = TileCfg<FMT, D>;
+    if constexpr (U == 8) return f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, DPP_ROW_HALF_MIRROR, 0xF, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, DPP_ROW_ROR4, 0xF, 0xF, false));
+    v = f(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, DPP_ROW_ROR8, 0xF, 0xF, false));
+    if constexpr (U == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        const uint32_t a = r[0], b = r[1];
+        v = f(a, b);
+    }
+    return v;
+}
+template <int U>
+__device__ __forceinline__ uint32_t key_max(uint32_t v) { return key_fold<U>(v, [](uint32_t a, uint32_t b) { return max(a, b); }); }
+template <int U>
+__device__ __forceinline__ uint32_t key_or(uint32_t v) { return key_fold<U>(v, [](uint32_t a, uint32_t b) { return a | b; }); }
+
+template <int FMT, int D, int NW>
+__device__ __forceinline__ void tile_spread(const TileLoad<FMT, D, NW>& f, unsigned char* buf)
+{
+    using T = TileCfg<FMT, D, NW>;
     const int tid = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < T::ITEMS; ++i) {
-        const int it = tid + 256 * i;
+        if (!T::live(i)) break;
+        const int it = tid + T::NT * i;
         const bool value = T::value(i);
         const int j = value ? it - 4 * D : it, key = j / T::U, u = j - key * T::U;
         if (!value) {
@@ -123,27 +156,35 @@ __device__ __forceinline__ void tile_spread(const TileLoad<FMT, D>& f, unsigned 
         const auto& vs = f.vs[i < T::V0 ? 0 : i - T::V0];
         const auto& vm = f.vm[i < T::V0 ? 0 : i - T::V0];
         // the key's exponent, and which of its groups are not finite
-        uint32_t top = 0, bad = 0;
-#pragma unroll
-        for (int g = 0; g < T::NG; ++g) {
-            uint32_t s = half_bits(vs, g) & 0x7fffu, m = 0;
-            if constexpr (T::Q4) m = half_bits(vm, g) & 0x7fffu;
+        const int g = u >> 2;
+        uint32_t top = 0, bad = 0, sb = 0, mb = 0;
+        auto take = [&](uint32_t sbits, uint32_t mbits, int group) {
+            const uint32_t s = sbits & 0x7fffu, m = mbits & 0x7fffu;
             const bool odd = s >= 0x7c00u || m >= 0x7c00u;
-            bad |= (uint32_t)odd << g;
-            m = m < (4u << 10) ? 0u : m - (4u << 10);                  // |s n + m| < 2^8 both ways
-            top = max(top, odd ? 0u : max(s, m));
-        }
-        const int e = (int)(top >> 10) - 14, g = u >> 2;
-        uint32_t sb = half_bits(vs, 0);
+            bad |= (uint32_t)odd << group;
+            const uint32_t n = T::Q4 ? max(s, m < (4u << 10) ? 0u : m - (4u << 10)) : s;          // |s n + m| < 2^8 both ways
+            top = max(top, odd ? 0u : n);
+        };
+        if constexpr (T::ROWS) {
+            sb = vs[0];
+            mb = T::Q4 ? vm[0] : 0;
+            take(sb, mb, g);
+            top = key_max<T::U>(top);
+            bad = key_or<T::U>(bad);
+        } else {
 #pragma unroll
-        for (int k = 1; k < T::NG; ++k) sb = g == k ? half_bits(vs, k) : sb;
+            for (int k = 0; k < T::NG; ++k) {
+                const uint32_t s = half_bits(vs, k), m = T::Q4 ? half_bits(vm, k) : 0;
+                take(s, m, k);
+                sb = g == k ? s : sb;
+                mb = g == k ? m : mb;
+            }
+        }
+        const int e = (int)(top >> 10) - 14;
         const bool ok = !((bad >> g) & 1);
         const float s = ok ? __builtin_amdgcn_ldexpf(f16_bits_to_f32(sb), -e) : 0.f;
         float v[8];
         if constexpr (T::Q4) {
-            uint32_t mb = half_bits(vm, 0);
-#pragma unroll
-            for (int k = 1; k < T::NG; ++k) mb = g == k ? half_bits(vm, k) : mb;
             const float m = ok ? __builtin_amdgcn_ldexpf(f16_bits_to_f32(mb), -e) : 0.f;
             const uint32_t lo = f.code[i][0] & 0x0f0f0f0fu, hi = (f.code[i][0] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
@@ -208,31 +249,37 @@ __device__ __forceinline__ half8_t v_frag(const unsigned char* p)
     return __builtin_bit_cast(half8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-template <int FMT, int D>
+template <int FMT, int D, int NW>
 __device__ __forceinline__ void tile_body(const brik_attn_launch& a)
 {
-    using T = TileCfg<FMT, D>;
+    using T = TileCfg<FMT, D, NW>;
     constexpr int NG = T::NG;
     constexpr bool Q4 = T::Q4;
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * T::BUF];
-    __shared__ int range[8];
+    __shared__ int range[2 * NW];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 31, h = lane >> 5;
 
     Work w;
-    if (!find_work<TILE_ROWS>(a, w)) return;
+    if (!find_work<32 * NW>(a, w)) return;
     const Row row = find_row<32>(a, w, w.r0 + 32 * wave, m);
     // keys that any row of the wave sees, [any_lo, any_hi), and that all see
     const int any_lo = wave_min(row.real ? row.lo : 0x7fffffff), any_hi = wave_max(row.real ? row.hi : 0);
     const int all_lo = wave_max(row.real ? row.lo : 0), all_hi = wave_min(row.hi);
     if (lane == 0) {
         range[wave] = any_lo;
-        range[4 + wave] = any_hi;
+        range[NW + wave] = any_hi;
     }
     __syncthreads();
     int t0, t1;
-    find_keys(w, min(min(range[0], range[1]), min(range[2], range[3])), max(max(range[4], range[5]), max(range[6], range[7])), 4, t0, t1);
+    int lo = range[0], hi = range[NW];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) {
+        lo = min(lo, range[i]);
+        hi = max(hi, range[NW + i]);
+    }
+    find_keys(w, uniform(lo), uniform(hi), 4, t0, t1);
 
-    TileLoad<FMT, D> next;
+    TileLoad<FMT, D, NW> next;
     KeyPages kp = {{-1, -1}}, kn = {{-1, -1}}, kf = {{-1, -1}};       // of this block of keys, the next and the one after
     if (t0 < t1) {
         kp = key_pages(a, w, t0);
@@ -463,11 +510,20 @@ __device__ __forceinline__ void tile_body(const brik_attn_launch& a)
 
 }  // namespace
 
-#define BRIK_ATTN_TILE(D)                                                                                                                      \
-    extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void brik_attn_tile_q8_##D(brik_attn_launch a) { tile_body<FMT_Q8, D>(a); }   \
-    extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void brik_attn_tile_q4_##D(brik_attn_launch a) { tile_body<FMT_Q4, D>(a); }
-BRIK_ATTN_TILE(64)
-BRIK_ATTN_TILE(96)
-BRIK_ATTN_TILE(128)
-BRIK_ATTN_TILE(192)
-BRIK_ATTN_TILE(256)
+#define BRIK_ATTN_TILE(D, NW)                                                                                            \
+    extern "C" __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void brik_attn_tile##NW##_q8_##D(brik_attn_launch a) \
+    {                                                                                                                     \
+        tile_body<FMT_Q8, D, NW>(a);                                                                                      \
+    }                                                                                                                     \
+    extern "C" __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void brik_attn_tile##NW##_q4_##D(brik_attn_launch a) \
+    {                                                                                                                     \
+        tile_body<FMT_Q4, D, NW>(a);                                                                                      \
+    }
+BRIK_ATTN_TILE(64, 4)
+BRIK_ATTN_TILE(96, 4)
+BRIK_ATTN_TILE(128, 4)
+BRIK_ATTN_TILE(192, 4)
+BRIK_ATTN_TILE(256, 4)
+BRIK_ATTN_TILE(64, 8)
+BRIK_ATTN_TILE(96, 8)
+BRIK_ATTN_TILE(128, 8)
