@@ -240,23 +240,45 @@ __device__ __forceinline__ void find_keys(const Work& w, int lo, int hi, int lea
 }
 
 // The pages of keys 32 t .. 32 t + 31: of the first and of the last 16 (the same page unless a page holds 16 tokens), -1
-// where they do not exist, and the slot of the first key.
+// where they do not exist.
 struct KeyPages {
     int32_t p[2];
 };
-__device__ __forceinline__ KeyPages key_pages(const brik_attn_launch& a, const Work& w, int t)
-{
-    KeyPages k;
-    const int32_t* const tab = w.prefix ? a.s.prefix_table : a.s.table + (size_t)w.b * a.s.table_cols;
-    const int cols = w.prefix ? (a.s.prefix_len + (1 << a.s.shift) - 1) >> a.s.shift : a.s.table_cols;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int c = (32 * t + 16 * i) >> a.s.shift;
-        const int32_t id = c < cols ? tab[c] : -1;
-        k.p[i] = (uint32_t)id < (uint32_t)a.s.pages ? id : -1;
+
+// A window of 64 columns of the section's table, one a lane: looking a page up reads a register. (Loaded one by one, every
+// look-up waited for all the loads before it, the keys of the next block among them.)
+struct PageWindow {
+    const int32_t* tab;
+    int cols, pages, shift, base;
+    int32_t id;                // of column base + lane
+
+    __device__ __forceinline__ PageWindow(const brik_attn_launch& a, const Work& w)
+    {
+        tab = w.prefix ? a.s.prefix_table : a.s.table + (size_t)w.b * a.s.table_cols;
+        cols = w.prefix ? (a.s.prefix_len + (1 << a.s.shift) - 1) >> a.s.shift : a.s.table_cols;
+        pages = a.s.pages;
+        shift = a.s.shift;
+        base = -64;
+        id = -1;
     }
-    return k;
-}
+    __device__ __forceinline__ int32_t page(int c)
+    {
+        if ((uint32_t)(c - base) >= 64u) {
+            base = c;
+            const int mine = c + (int)(threadIdx.x & 63);
+            const int32_t v = mine < cols ? tab[mine] : -1;
+            id = (uint32_t)v < (uint32_t)pages ? v : -1;
+        }
+        return __builtin_amdgcn_readlane(id, c - base);
+    }
+    __device__ __forceinline__ KeyPages of(int t)
+    {
+        KeyPages k;
+        k.p[0] = page((32 * t) >> shift);
+        k.p[1] = shift > 4 ? k.p[0] : page(2 * t + 1);
+        return k;
+    }
+};
 
 // Eight int8 codes as f16, the bytes of each word in the order 0, 2, 1, 3: 1024 + (c + 128) has the code's bits in its low
 // byte, and the subtraction is exact.

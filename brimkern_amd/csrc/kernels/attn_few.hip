@@ -172,12 +172,12 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 
     // first block's loads, then q while they are on the way
     FewLoad<FMT, D> next;
-    KeyPages kp = {{-1, -1}}, kn = {{-1, -1}};
+    PageWindow window(a, w);
+    KeyPages kp = {{-1, -1}};
     int t = uniform(t0 + wave);
     if (t < t1) {
-        kp = key_pages(a, w, t);
+        kp = window.of(t);
         few_load(next, a, w, t, kp);
-        if (t + 4 < t1) kn = key_pages(a, w, t + 4);
     }
 
     // q: this lane's values of its row, eight of each group, times a power of two that puts the row's largest below 2^15
@@ -377,9 +377,8 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
         wave_lds_fence();
         few_spread(next, lds);
         if (t + 4 < t1) {
-            kp = kn;
+            kp = window.of(t + 4);
             few_load(next, a, w, t + 4, kp);
-            if (t + 8 < t1) kn = key_pages(a, w, t + 8);
         }
         wave_lds_fence();
         if (32 * t >= all_lo && 32 * t + 32 <= all_hi && have[0] && have[1]) block(std::false_type{}, t, have);

@@ -280,11 +280,11 @@ __device__ __forceinline__ void tile_body(const brik_attn_launch& a)
     find_keys(w, uniform(lo), uniform(hi), 4, t0, t1);
 
     TileLoad<FMT, D, NW> next;
-    KeyPages kp = {{-1, -1}}, kn = {{-1, -1}}, kf = {{-1, -1}};       // of this block of keys, the next and the one after
+    PageWindow window(a, w);
+    KeyPages kp = {{-1, -1}}, kn = {{-1, -1}};       // of this block of keys and the next
     if (t0 < t1) {
-        kp = key_pages(a, w, t0);
+        kp = window.of(t0);
         tile_load(next, a, w, t0, kp);
-        if (t0 + 1 < t1) kn = key_pages(a, w, t0 + 1);
     }
 
     // q: eight values of each half group, times a power of two that puts the row's largest below 2^6; a negative scale
@@ -459,8 +459,8 @@ __device__ __forceinline__ void tile_body(const brik_attn_launch& a)
     if (t0 < t1) {
         tile_spread(next, smem);
         if (t0 + 1 < t1) {
+            kn = window.of(t0 + 1);
             tile_load(next, a, w, t0 + 1, kn);
-            if (t0 + 2 < t1) kf = key_pages(a, w, t0 + 2);
         }
     }
     for (int t = t0; t < t1; ++t) {
@@ -470,10 +470,9 @@ __device__ __forceinline__ void tile_body(const brik_attn_launch& a)
         kp = kn;
         if (t + 1 < t1) {
             tile_spread(next, smem + ((t + 1 - t0) & 1) * T::BUF);
-            kn = kf;
             if (t + 2 < t1) {
+                kn = window.of(t + 2);
                 tile_load(next, a, w, t + 2, kn);
-                if (t + 3 < t1) kf = key_pages(a, w, t + 3);
             }
         }
         if (32 * t >= any_hi || 32 * t + 32 <= any_lo) continue;
