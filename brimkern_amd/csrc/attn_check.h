@@ -130,7 +130,7 @@ inline bool attn_dim(int D) { return D == 64 || D == 96 || D == 128 || D == 192 
 inline int attn(Why& w, const char* who, const brik_kv_cache* c, const brik_kv_batch* b, brik_attn_args& a)
 {
     if (!attn_dim(c->head_dim)) return no(w, BRIK_EINVAL, "%s: head_dim %d (64, 96, 128, 192 or 256)", who, c->head_dim);
-    if (a.heads < 1 || a.heads > 65536 || a.heads % c->heads)
+    if (a.heads < 1 || a.heads > 65535 || a.heads % c->heads)
         return no(w, BRIK_EINVAL, "%s: %d query heads over %d key / value heads", who, a.heads, c->heads);
     if (a.window < 0) return no(w, BRIK_EINVAL, "%s: window %d", who, a.window);
     if (!std::isfinite(a.scale) || !(a.softcap >= 0) || !std::isfinite(a.softcap))

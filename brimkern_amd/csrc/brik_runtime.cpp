@@ -2551,9 +2551,14 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     int dim = 0;
     while (kAttnDims[dim] != a.c.head_dim) ++dim;
     const int which = 5 * (a.c.fmt == BRIK_FMT_Q4) + dim;
-    // Rows of one tile of the 16-row kernel: that one, else 128 or 256 rows a tile, each section by itself.
-    auto tile_rows = [&](long n) { return n <= 16 ? 16 : n <= 128 || a.c.head_dim > 128 ? 128 : 256; };
-    const int own_bm = tile_rows(most * G), prefix_bm = tile_rows(rows * G);
+    // Row tiles of 256 or 128 where they fill the device without splitting keys, else of 16 (a 32-key step of a tile takes 3 us
+    // however few blocks there are: 805 rows of 7 heads behind a window of 1024 keys 71 us by 256, 31 us by 16 rows).
+    auto tile_rows = [&](long most_rows, long all_rows) {
+        const long fill = KV * ((all_rows * G + 255) / 256);
+        if (most_rows * G <= 16 || fill < kCUs / 2) return 16;
+        return a.c.head_dim > 128 || most_rows * G <= 128 ? 128 : 256;
+    };
+    const int own_bm = tile_rows(most, rows), prefix_bm = tile_rows(rows, rows);
     // row tiles of the sequences: the same number for each where that is not many more than there can be
     const long per_seq = (most * G + own_bm - 1) / own_bm, bound = (rows * G + own_bm - 1) / own_bm + a.s.seqs;
     long tiles = per_seq * a.s.seqs;
@@ -2562,14 +2567,24 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         a.tiles_per_seq = 0;
         tiles = bound;
     }
-    a.own_splits = attn_splits(KV * tiles, own_keys);
+    // One tile a sequence, several sequences, and too few to fill the device evenly: blocks by the sequences' lengths, four per
+    // CU (a sequence's last one is part full). (Static splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for the longest.)
+    const long blocks32 = (std::max(0l, own_keys) + 31) / 32;
+    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && KV * a.s.seqs < 8 * kCUs && blocks32 > 4) {
+        a.own_blocks = (int)(std::min<long>((4 * kCUs + KV - 1) / KV, a.s.seqs * ((blocks32 + 3) / 4)) + a.s.seqs);
+        tiles = a.own_blocks;
+        a.own_splits = 1;
+    } else {
+        a.own_splits = attn_splits(KV * tiles, own_keys);
+    }
     if (prefix_keys > 0) {
         a.prefix_tiles = (int)((rows * G + prefix_bm - 1) / prefix_bm);
         a.prefix_splits = attn_splits(KV * a.prefix_tiles, prefix_keys);
     }
-    const int slots = a.prefix_splits + a.own_splits;
-    if (slots > 1) {
-        const size_t vectors = (size_t)slots * rows * a.a.heads, d = (size_t)a.c.head_dim;
+    a.whole = a.prefix_splits == 0 && a.own_splits == 1 && a.own_blocks == 0;
+    if (!a.whole) {
+        const size_t all = (size_t)rows * a.a.heads, d = (size_t)a.c.head_dim;
+        const size_t vectors = a.prefix_splits * all + (a.own_blocks ? (size_t)KV * a.own_blocks * 16 : a.own_splits * all);
         HIP_TRY_RC(ensure_buf(c, c->aws, c->aws_bytes, 4 * vectors * (d + 2)));
         a.part = static_cast<float*>(c->aws);
         a.ml = a.part + vectors * d;
@@ -2581,7 +2596,6 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         void* args[] = {&a};
         return launch_fn(c, c->attn_fn[k + which], (unsigned)blocks, 1, bm == 256 ? 512 : 256, 0, args);
     };
-    void* args[] = {&a};
     if (prefix_blocks && prefix_bm != own_bm) {
         // two launches: the kernels see the blocks from `first_block` on
         HIP_TRY_RC(run(prefix_bm, prefix_blocks));
@@ -2590,8 +2604,9 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     } else {
         HIP_TRY_RC(run(own_bm, own_blocks + prefix_blocks));
     }
-    if (slots > 1) return launch_fn(c, c->attn_fn[A_JOIN], (unsigned)rows, (unsigned)a.a.heads, 256, 0, args);
-    return BRIK_OK;
+    if (a.whole) return BRIK_OK;
+    void* args[] = {&a};
+    return launch_fn(c, c->attn_fn[A_JOIN], (unsigned)rows, (unsigned)a.a.heads, 256, 0, args);
 }
 
 int brik_attention(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* batch, const brik_attn_args* args)

@@ -72,6 +72,29 @@ __device__ __forceinline__ int wave_min(int v)
 }
 __device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
 
+// Sum of v over the lanes up to this one: within rows of 16 by shifts, then the sums of the rows before.
+__device__ __forceinline__ int wave_scan(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);       // row_shr 1, 2, 4, 8; zeros come in
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    const int row = (threadIdx.x & 63) >> 4;
+    const int a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31), c = __builtin_amdgcn_readlane(v, 47);
+    return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+__device__ __forceinline__ int wave_sum(int v)
+{
+    v += __builtin_amdgcn_mov_dpp(v, DPP_QUAD_1032, 0xF, 0xF, false);
+    v += __builtin_amdgcn_mov_dpp(v, DPP_QUAD_2301, 0xF, 0xF, false);
+    v += __builtin_amdgcn_mov_dpp(v, DPP_ROW_ROR4, 0xF, 0xF, false);
+    v += __builtin_amdgcn_mov_dpp(v, DPP_ROW_ROR8, 0xF, 0xF, false);
+    const auto q = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = (int)(q[0] + q[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    return uniform((int)(h[0] + h[1]));
+}
+
 // The sequence of row t: how many of row_off[1..seqs] are at most t. One load round trip per 64 sequences.
 __device__ __forceinline__ int seq_of_row(const brik_step& s, int t)
 {
@@ -122,12 +145,7 @@ __device__ __forceinline__ void find_tile(const brik_step& s, int tile, int G, i
         int32_t first, n = 0;
         if (i < s.seqs) brik_rows_of(s, i, first, n);
         const int tiles = (int)(((long long)n * G + BM - 1) / BM);
-        int sum = tiles;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int o = __shfl_up(sum, m);
-            if (lane >= m) sum += o;
-        }
+        const int sum = wave_scan(tiles);
         const uint64_t past = __ballot(before + sum > tile);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -144,12 +162,96 @@ __device__ __forceinline__ void find_tile(const brik_step& s, int tile, int G, i
 // One block's work: which rows, which keys.
 struct Work {
     int head;                  // key / value head
-    int slot;                  // of the partial results
+    int slot;                  // of the partial results, or block of the sequences' blocks
     bool prefix;               // keys of the prefix, rows of all sequences
     int b;                     // sequence (own keys)
     int first, count;          // its rows
     int r0;                    // first of the tile's rows, counted over count * G
     int split, splits;
+    int each;                  // blocks of 32 keys per split, or 0: to be divided evenly
+    int pos;                   // position of the first row (own keys)
+    bool whole;                // nothing to join: the block writes the output
+};
+
+// A sequence's rows, and the blocks of 32 of its own keys that they see (first, count).
+struct Seq {
+    int32_t row, rows, pos;      // first row, how many, the first row's position
+    int first, n;
+};
+__device__ __forceinline__ Seq find_seq(const brik_attn_launch& a, int b)
+{
+    Seq q;
+    brik_rows_of(a.s, b, q.row, q.rows);
+    const int32_t end_row = a.s.row_off ? a.s.row_off[b + 1] : (b + 1) * a.s.per_seq;
+    q.pos = a.s.kv_len[b] - end_row + q.row;
+    const int32_t before = a.s.prefix_len;
+    const int32_t end = (int32_t)min((long long)a.s.max_len - before, min((long long)a.s.table_cols << a.s.shift, 0x7fffffc0ll));
+    const int hi = min(q.pos + q.rows - before, end), lo = a.a.window ? max(0, q.pos - a.a.window + 1 - before) : 0;
+    q.first = lo >> 5;
+    q.n = q.rows > 0 && lo < hi ? ((hi + 31) >> 5) - q.first : 0;
+    return q;
+}
+
+// The blocks of the own keys go to the sequences by their lengths: `each` blocks of 32 keys a block, as few as the grid
+// allows and at least four, a sequence's blocks next to each other. Every wave reads all lengths, 64 at a time; up to 64
+// sequences stay in the lanes.
+struct Share {
+    int each;
+    Seq mine;                    // of sequence lane (of the last 64 read)
+    __device__ __forceinline__ explicit Share(const brik_attn_launch& a)
+    {
+        const int lane = threadIdx.x & 63;
+        int total = 0;
+        for (int base = 0; base < a.s.seqs; base += 64) {
+            mine.n = mine.rows = 0;
+            if (base + lane < a.s.seqs) mine = find_seq(a, base + lane);
+            total += wave_sum(mine.n);
+        }
+        const int spare = a.own_blocks - a.s.seqs;           // one of each sequence's blocks may be part full
+        each = max(4, (total + spare - 1) / spare);
+    }
+    __device__ __forceinline__ void read(const brik_attn_launch& a, int base)
+    {
+        if (a.s.seqs <= 64) return;
+        mine.n = mine.rows = 0;
+        if (base + (int)(threadIdx.x & 63) < a.s.seqs) mine = find_seq(a, base + (threadIdx.x & 63));
+    }
+    // A sequence with rows has at least one block (without keys its block writes the zeros).
+    __device__ __forceinline__ int count_of() const { return mine.rows > 0 ? max(1, (mine.n + each - 1) / each) : 0; }
+    // Whose is block i (b == seqs: nobody's), and which of its blocks; `mine` of lane b % 64 is then the sequence's.
+    __device__ __forceinline__ void owner(const brik_attn_launch& a, int i, int& b, int& k)
+    {
+        int before = 0;
+        for (int base = 0; base < a.s.seqs; base += 64) {
+            read(a, base);
+            const int blocks = count_of(), sum = wave_scan(blocks);
+            const uint64_t past = __ballot(before + sum > i);
+            if (past) {
+                const int l = __ffsll((unsigned long long)past) - 1;
+                b = base + l;
+                k = i - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(blocks, l));
+                return;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+        b = a.s.seqs;
+        k = 0;
+    }
+    // The blocks of sequence b: the first and how many.
+    __device__ __forceinline__ void blocks_of(const brik_attn_launch& a, int b, int& first, int& count)
+    {
+        first = count = 0;
+        for (int base = 0; base <= b; base += 64) {
+            read(a, base);
+            const int blocks = count_of(), sum = wave_scan(blocks);
+            if (b < base + 64) {
+                count = __builtin_amdgcn_readlane(blocks, b - base);
+                first += __builtin_amdgcn_readlane(sum, b - base) - count;
+            } else {
+                first += __builtin_amdgcn_readlane(sum, 63);
+            }
+        }
+    }
 };
 
 // The grid: heads fastest, then the splits, then the row tiles; the prefix's blocks before the own keys'.
@@ -161,6 +263,8 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
     w.head = id % KV;
     id /= KV;
     const int pre = a.prefix_tiles * a.prefix_splits;
+    w.each = 0;
+    w.whole = a.whole;
     w.prefix = id < pre;
     if (w.prefix) {
         w.splits = a.prefix_splits;
@@ -173,6 +277,21 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
         return true;
     }
     id -= pre;
+    if (a.own_blocks) {
+        Share share(a);
+        share.owner(a, id, w.b, w.split);
+        if (w.b >= a.s.seqs) return false;
+        w.each = share.each;
+        w.splits = max(1, (__builtin_amdgcn_readlane(share.mine.n, w.b & 63) + w.each - 1) / w.each);
+        w.whole = w.splits == 1 && a.prefix_splits == 0;
+        w.slot = id;
+        w.r0 = 0;
+        const int l = w.b & 63;
+        w.first = __builtin_amdgcn_readlane(share.mine.row, l);
+        w.count = __builtin_amdgcn_readlane(share.mine.rows, l);
+        w.pos = __builtin_amdgcn_readlane(share.mine.pos, l);
+        return true;
+    }
     w.splits = a.own_splits;
     w.split = id % w.splits;
     w.slot = a.prefix_splits + w.split;
@@ -185,6 +304,7 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
         if (w.b >= a.s.seqs) return false;
     }
     brik_rows_of(a.s, w.b, w.first, w.count);
+    w.pos = row_position(a.s, w.b, w.first);
     // the last tiles see the most keys: they come first
     const int tiles = (int)(((long long)w.count * G + BM - 1) / BM);
     if (j >= tiles) return false;
@@ -219,12 +339,20 @@ __device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w
         r.real = r.real && b < a.s.seqs;
     }
     if (!r.real) return r;
-    const int32_t pos = row_position(a.s, b, r.t), first = w.prefix ? 0 : a.s.prefix_len;
+    const int32_t pos = w.prefix ? row_position(a.s, b, r.t) : w.pos + rel, first = w.prefix ? 0 : a.s.prefix_len;
     const int32_t end = w.prefix ? min(a.s.prefix_len, a.s.max_len)
                                  : (int32_t)min((long long)a.s.max_len - first, min((long long)a.s.table_cols << a.s.shift, 0x7fffffc0ll));
     r.hi = max(0, min(pos + 1 - first, end));
     r.lo = a.a.window ? max(0, pos - a.a.window + 1 - first) : 0;
     return r;
+}
+
+// Where row m of the tile (token t, head h) keeps its partial result.
+__device__ __forceinline__ size_t part_at(const brik_attn_launch& a, const Work& w, int m, int t, int h)
+{
+    const size_t all = (size_t)a.s.rows * a.a.heads;
+    if (a.own_blocks && !w.prefix) return a.prefix_splits * all + ((size_t)w.head * a.own_blocks + w.slot) * 16 + m;
+    return w.slot * all + (size_t)t * a.a.heads + h;
 }
 
 // The key blocks [t0, t1) of 32 keys that this split works on: those of the keys [lo, hi) that any row sees, divided over
@@ -234,7 +362,7 @@ __device__ __forceinline__ void find_keys(const Work& w, int lo, int hi, int lea
     t0 = t1 = 0;
     if (lo >= hi) return;
     const int first = lo >> 5, n = ((hi + 31) >> 5) - first;
-    const int each = max(least, (n + w.splits - 1) / w.splits);
+    const int each = w.each ? w.each : max(least, (n + w.splits - 1) / w.splits);
     t0 = first + min(n, w.split * each);
     t1 = first + min(n, (w.split + 1) * each);
 }

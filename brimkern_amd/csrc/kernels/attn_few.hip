@@ -413,8 +413,7 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
         }
     }
     __syncthreads();
-    const int G = a.a.heads / a.c.heads, slots = a.prefix_splits + a.own_splits;
-    const size_t all = (size_t)a.s.rows * a.a.heads;
+    const int G = a.a.heads / a.c.heads;
     for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
         const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
         const int rel = (w.r0 + r) / G;
@@ -429,15 +428,12 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
         f32x4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < 4; ++k) v += *(const f32x4_t*)((const float*)(smem + k * T::BYTES) + r * T::OS + d);
-        if (slots == 1) {
+        if (w.whole) {
             *(f32x4_t*)(a.a.out + tok * a.a.out_stride + (size_t)h * D + d) = L == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : v / L;
         } else {
-            const size_t at = w.slot * all + (size_t)tok * a.a.heads + h;
+            const size_t at = part_at(a, w, r, tok, h);
             if (L != 0.f) *(f32x4_t*)(a.part + at * D + d) = v;
-            if (d == 0) {
-                a.ml[2 * at] = Mr;
-                a.ml[2 * at + 1] = L;
-            }
+            if (d == 0) *(f32x2_t*)(a.ml + 2 * at) = f32x2_t{Mr, L};
         }
     }
 }

@@ -4,29 +4,54 @@
 
 extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launch a)
 {
-    __shared__ float f[256];
     __shared__ f32x4_t sums[256];
-    const int D = a.c.head_dim, quads = D / 4, groups = 256 / quads, slots = a.prefix_splits + a.own_splits;
-    const int h = blockIdx.y, t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    if (a.s.row_off && t >= a.s.row_off[a.s.seqs]) return;          // behind the last sequence
+    const int D = a.c.head_dim, quads = D / 4, groups = 256 / quads;
+    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const size_t all = (size_t)a.s.rows * a.a.heads, row = (size_t)t * a.a.heads + h;
-    // every wave: the reference exponent, then the weights (slots <= 256)
-    float M = ATTN_NONE;
-    for (int s = lane; s < slots; s += 64) M = fmaxf(M, a.ml[2 * (s * all + row)]);
-    for (int m = 1; m < 64; m <<= 1) M = fmaxf(M, __shfl_xor(M, m));
-    float L = 0.f;
-    for (int s = lane; s < slots; s += 64) {
-        const float l = a.ml[2 * (s * all + row) + 1], w = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(a.ml[2 * (s * all + row)] - M);
-        f[s] = w;                                                    // every wave writes the same
-        L += l * w;
+    // vector of slot s: the prefix's and static ones are `all` apart, a sequence's blocks 16
+    int slots = a.prefix_splits + a.own_splits;
+    size_t own = 0;
+    if (a.own_blocks) {
+        Share share(a);                                              // first: its loads and the search's go together
+        const int b = seq_of_row(a.s, t);
+        if (b >= a.s.seqs) return;                                   // behind the last sequence
+        const int G = a.a.heads / a.c.heads, kvh = h / G;
+        int first, count;
+        share.blocks_of(a, b, first, count);
+        if (count == 1 && a.prefix_splits == 0) return;              // written by its block
+        slots = a.prefix_splits + count;
+        own = a.prefix_splits * all + ((size_t)kvh * a.own_blocks + first) * 16 + (t - __builtin_amdgcn_readlane(share.mine.row, b & 63)) * G + (h - kvh * G);
+    } else if (a.s.row_off && t >= a.s.row_off[a.s.seqs]) {
+        return;
     }
-    for (int m = 1; m < 64; m <<= 1) L += __shfl_xor(L, m);
-    __syncthreads();
+    auto vec = [&](int s) { return a.own_blocks && s >= a.prefix_splits ? own + (size_t)(s - a.prefix_splits) * 16 : s * all + row; };
+    // every wave: the reference exponent, then the weights (they stay in the cache: read twice rather than kept)
+    float M = ATTN_NONE;
+#pragma unroll 1
+    for (int s = lane; s < slots; s += 64) M = fmaxf(M, a.ml[2 * vec(s)]);
+    M = half_max(M);
+    float p, q;
+    half_pair(M, p, q);
+    M = fmaxf(p, q);
     const int g = tid / quads, d = 4 * (tid - g * quads);
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (g < groups)
-        for (int s = g; s < slots; s += groups)
-            if (f[s] != 0.f) v += *(const f32x4_t*)(a.part + (s * all + row) * D + d) * f[s];
+    float L = 0.f;
+#pragma unroll 1
+    for (int s0 = 0; s0 < slots; s0 += 64) {                         // 64 slots at a time, one a lane
+        float l = 0.f, f = 0.f;
+        if (s0 + lane < slots) {
+            const f32x2_t ml = *(const f32x2_t*)(a.ml + 2 * vec(s0 + lane));
+            l = ml.y;
+            f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+        }
+        L += quarters_sum(sum16(l * f));
+        const int n = min(64, slots - s0);
+        for (int s1 = 0; s1 < n; s1 += groups) {                     // as often in every lane: weights come from other lanes
+            const int s = s1 + g;
+            const float w = __shfl(f, min(s, 63));
+            if (g < groups && s < n && w != 0.f) v += *(const f32x4_t*)(a.part + vec(s0 + s) * D + d) * w;
+        }
+    }
     sums[tid] = v;
     __syncthreads();
     if (g != 0) return;

@@ -488,8 +488,8 @@ __device__ __forceinline__ void tile_body(const brik_attn_launch& a)
     float u, v;
     half_pair(l, u, v);
     const float L = u + v;
-    const bool whole = a.prefix_splits + a.own_splits == 1;
-    const size_t at = w.slot * ((size_t)a.s.rows * a.a.heads) + (size_t)row.t * a.a.heads + row.h;
+    const bool whole = w.whole;
+    const size_t at = part_at(a, w, 0, row.t, row.h);
     float* const dst = (whole ? a.a.out + row.t * a.a.out_stride + (size_t)row.h * D : a.part + at * D) + 4 * h;
     if (!whole && h == 0) {
         a.ml[2 * at] = M;
