@@ -2567,11 +2567,12 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         a.tiles_per_seq = 0;
         tiles = bound;
     }
-    // One tile a sequence, several sequences, and too few to fill the device evenly: blocks by the sequences' lengths, four per
-    // CU (a sequence's last one is part full). (Static splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for the longest.)
+    // One tile a sequence and several sequences: their keys in a row, shared out evenly over two blocks per CU, by the lengths
+    // that the call finds. (Splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for the longest. Up to
+    // 1024 keys a block per sequence is as fast, and one that begins a second sequence pays 4 us for it.)
     const long blocks32 = (std::max(0l, own_keys) + 31) / 32;
-    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && KV * a.s.seqs < 8 * kCUs && blocks32 > 4) {
-        a.own_blocks = (int)(std::min<long>((4 * kCUs + KV - 1) / KV, a.s.seqs * ((blocks32 + 3) / 4)) + a.s.seqs);
+    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32) {
+        a.own_blocks = (int)std::max(1l, std::min<long>((2 * kCUs + KV - 1) / KV, a.s.seqs * ((blocks32 + 3) / 4)));
         tiles = a.own_blocks;
         a.own_splits = 1;
     } else {
@@ -2584,7 +2585,7 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     a.whole = a.prefix_splits == 0 && a.own_splits == 1 && a.own_blocks == 0;
     if (!a.whole) {
         const size_t all = (size_t)rows * a.a.heads, d = (size_t)a.c.head_dim;
-        const size_t vectors = a.prefix_splits * all + (a.own_blocks ? (size_t)KV * a.own_blocks * 16 : a.own_splits * all);
+        const size_t vectors = a.prefix_splits * all + (a.own_blocks ? (size_t)KV * (a.own_blocks + a.s.seqs) * 16 : a.own_splits * all);
         HIP_TRY_RC(ensure_buf(c, c->aws, c->aws_bytes, 4 * vectors * (d + 2)));
         a.part = static_cast<float*>(c->aws);
         a.ml = a.part + vectors * d;

@@ -88,12 +88,12 @@ typedef struct brik_attn_launch {
     brik_kv_cache c;
     // Partial results, where keys are split: outputs [vector][head_dim], reference exponents and sums [vector][2]. Vectors:
     // [slot][row][head] with the slots of the prefix, then (own_blocks == 0) those of the own keys; own_blocks > 0: behind the
-    // prefix's, [key / value head][block][16 rows].
+    // prefix's, [key / value head][own_blocks + seqs parts][16 rows].
     float *part, *ml;
     // The grid: row tiles of the prefix's keys (rows of all sequences) and of the sequences' own keys, each tile's keys
     // split over so many blocks. tiles_per_seq: the tile's sequence by division (0: by a search over the sequences' rows).
     int32_t prefix_tiles, prefix_splits, own_splits, tiles_per_seq;
-    // One tile a sequence: own_blocks blocks per key / value head, given to the sequences by their lengths.
+    // One tile a sequence: own_blocks blocks per key / value head share the sequences' keys out by their lengths.
     int32_t own_blocks;
     int32_t first_block;   // number of the launch's first block
     int32_t whole;         // no splits, no prefix: the kernel writes the output

@@ -168,7 +168,7 @@ struct Work {
     int first, count;          // its rows
     int r0;                    // first of the tile's rows, counted over count * G
     int split, splits;
-    int each;                  // blocks of 32 keys per split, or 0: to be divided evenly
+    int t0, t1;                // blocks of 32 keys, where they are shared out (else t1 == 0: by split and splits)
     int pos;                   // position of the first row (own keys)
     bool whole;                // nothing to join: the block writes the output
 };
@@ -192,64 +192,50 @@ __device__ __forceinline__ Seq find_seq(const brik_attn_launch& a, int b)
     return q;
 }
 
-// The blocks of the own keys go to the sequences by their lengths: `each` blocks of 32 keys a block, as few as the grid
-// allows and at least four, a sequence's blocks next to each other. Every wave reads all lengths, 64 at a time; up to 64
-// sequences stay in the lanes.
+// The own keys of all sequences in a row, in blocks of 32, are shared out evenly: `each` blocks of keys for every block of the
+// grid (four at least, one per wave), which may end one sequence and begin the next. Its part of sequence b is number
+// block + b of the partial results: a sequence's parts follow each other, and no two parts share a number. Every wave reads
+// all lengths, 64 at a time, one a lane.
 struct Share {
-    int each;
-    Seq mine;                    // of sequence lane (of the last 64 read)
+    int each, total;
     __device__ __forceinline__ explicit Share(const brik_attn_launch& a)
     {
-        const int lane = threadIdx.x & 63;
-        int total = 0;
-        for (int base = 0; base < a.s.seqs; base += 64) {
-            mine.n = mine.rows = 0;
-            if (base + lane < a.s.seqs) mine = find_seq(a, base + lane);
-            total += wave_sum(mine.n);
-        }
-        const int spare = a.own_blocks - a.s.seqs;           // one of each sequence's blocks may be part full
-        each = max(4, (total + spare - 1) / spare);
+        total = 0;
+        for (int base = 0; base < a.s.seqs; base += 64) total += wave_sum(lane_seq(a, base).n);
+        each = max(4, (total + a.own_blocks - 1) / a.own_blocks);
     }
-    __device__ __forceinline__ void read(const brik_attn_launch& a, int base)
+    __device__ __forceinline__ static Seq lane_seq(const brik_attn_launch& a, int base)
     {
-        if (a.s.seqs <= 64) return;
-        mine.n = mine.rows = 0;
-        if (base + (int)(threadIdx.x & 63) < a.s.seqs) mine = find_seq(a, base + (threadIdx.x & 63));
+        Seq q;
+        q.n = q.rows = q.row = q.pos = q.first = 0;
+        const int b = base + (int)(threadIdx.x & 63);
+        if (b < a.s.seqs) q = find_seq(a, b);
+        return q;
     }
-    // A sequence with rows has at least one block (without keys its block writes the zeros).
-    __device__ __forceinline__ int count_of() const { return mine.rows > 0 ? max(1, (mine.n + each - 1) / each) : 0; }
-    // Whose is block i (b == seqs: nobody's), and which of its blocks; `mine` of lane b % 64 is then the sequence's.
-    __device__ __forceinline__ void owner(const brik_attn_launch& a, int i, int& b, int& k)
+    // Sequence b, all of it uniform, and the key blocks before it. b < 0: of the sequence that key block g < total belongs to.
+    __device__ __forceinline__ static Seq find(const brik_attn_launch& a, int& b, int g, int& start)
     {
         int before = 0;
-        for (int base = 0; base < a.s.seqs; base += 64) {
-            read(a, base);
-            const int blocks = count_of(), sum = wave_scan(blocks);
-            const uint64_t past = __ballot(before + sum > i);
-            if (past) {
-                const int l = __ffsll((unsigned long long)past) - 1;
+        for (int base = 0;; base += 64) {
+            const Seq q = lane_seq(a, base);
+            const int sum = wave_scan(q.n);
+            int l = b - base;
+            if (b < 0) {
+                const uint64_t past = __ballot(before + sum > g);
+                l = past ? __ffsll((unsigned long long)past) - 1 : 64;
+            }
+            if (l < 64) {
                 b = base + l;
-                k = i - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(blocks, l));
-                return;
+                Seq r;
+                r.row = __builtin_amdgcn_readlane(q.row, l);
+                r.rows = __builtin_amdgcn_readlane(q.rows, l);
+                r.pos = __builtin_amdgcn_readlane(q.pos, l);
+                r.first = __builtin_amdgcn_readlane(q.first, l);
+                r.n = __builtin_amdgcn_readlane(q.n, l);
+                start = before + __builtin_amdgcn_readlane(sum, l) - r.n;
+                return r;
             }
             before += __builtin_amdgcn_readlane(sum, 63);
-        }
-        b = a.s.seqs;
-        k = 0;
-    }
-    // The blocks of sequence b: the first and how many.
-    __device__ __forceinline__ void blocks_of(const brik_attn_launch& a, int b, int& first, int& count)
-    {
-        first = count = 0;
-        for (int base = 0; base <= b; base += 64) {
-            read(a, base);
-            const int blocks = count_of(), sum = wave_scan(blocks);
-            if (b < base + 64) {
-                count = __builtin_amdgcn_readlane(blocks, b - base);
-                first += __builtin_amdgcn_readlane(sum, b - base) - count;
-            } else {
-                first += __builtin_amdgcn_readlane(sum, 63);
-            }
         }
     }
 };
@@ -263,7 +249,7 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
     w.head = id % KV;
     id /= KV;
     const int pre = a.prefix_tiles * a.prefix_splits;
-    w.each = 0;
+    w.t0 = w.t1 = 0;
     w.whole = a.whole;
     w.prefix = id < pre;
     if (w.prefix) {
@@ -277,21 +263,6 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
         return true;
     }
     id -= pre;
-    if (a.own_blocks) {
-        Share share(a);
-        share.owner(a, id, w.b, w.split);
-        if (w.b >= a.s.seqs) return false;
-        w.each = share.each;
-        w.splits = max(1, (__builtin_amdgcn_readlane(share.mine.n, w.b & 63) + w.each - 1) / w.each);
-        w.whole = w.splits == 1 && a.prefix_splits == 0;
-        w.slot = id;
-        w.r0 = 0;
-        const int l = w.b & 63;
-        w.first = __builtin_amdgcn_readlane(share.mine.row, l);
-        w.count = __builtin_amdgcn_readlane(share.mine.rows, l);
-        w.pos = __builtin_amdgcn_readlane(share.mine.pos, l);
-        return true;
-    }
     w.splits = a.own_splits;
     w.split = id % w.splits;
     w.slot = a.prefix_splits + w.split;
@@ -310,6 +281,24 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
     if (j >= tiles) return false;
     w.r0 = (tiles - 1 - j) * BM;
     return true;
+}
+
+// The parts of a block of the shared-out keys: w is set to the part that begins at key block g (of all sequences' in a row), g
+// to the end of that part.
+__device__ __forceinline__ void next_part(const brik_attn_launch& a, int each, int block, int end, int& g, Work& w)
+{
+    int start;
+    w.b = -1;
+    const Seq q = Share::find(a, w.b, g, start);
+    w.first = q.row;
+    w.count = q.rows;
+    w.pos = q.pos;
+    w.r0 = 0;
+    w.slot = block + w.b;
+    w.t0 = q.first + (g - start);
+    g = min(end, start + q.n);
+    w.t1 = q.first + (g - start);
+    w.whole = a.prefix_splits == 0 && start / each == (start + q.n - 1) / each;
 }
 
 // A row of a tile (this lane's): its token and head, and the keys it sees, [lo, hi) in the section's own numbering
@@ -351,7 +340,7 @@ __device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w
 __device__ __forceinline__ size_t part_at(const brik_attn_launch& a, const Work& w, int m, int t, int h)
 {
     const size_t all = (size_t)a.s.rows * a.a.heads;
-    if (a.own_blocks && !w.prefix) return a.prefix_splits * all + ((size_t)w.head * a.own_blocks + w.slot) * 16 + m;
+    if (a.own_blocks && !w.prefix) return a.prefix_splits * all + ((size_t)w.head * (a.own_blocks + a.s.seqs) + w.slot) * 16 + m;
     return w.slot * all + (size_t)t * a.a.heads + h;
 }
 
@@ -359,10 +348,11 @@ __device__ __forceinline__ size_t part_at(const brik_attn_launch& a, const Work&
 // the splits in pieces of at least `least`.
 __device__ __forceinline__ void find_keys(const Work& w, int lo, int hi, int least, int& t0, int& t1)
 {
-    t0 = t1 = 0;
-    if (lo >= hi) return;
+    t0 = w.t0;
+    t1 = w.t1;
+    if (t1 || lo >= hi) return;
     const int first = lo >> 5, n = ((hi + 31) >> 5) - first;
-    const int each = w.each ? w.each : max(least, (n + w.splits - 1) / w.splits);
+    const int each = max(least, (n + w.splits - 1) / w.splits);
     t0 = first + min(n, w.split * each);
     t1 = first + min(n, (w.split + 1) * each);
 }
@@ -433,10 +423,13 @@ __device__ __forceinline__ half8_t centred_q4(uint32_t a, uint32_t b, uint32_t c
 {
     const half2_t off = {(_Float16)-1032.f, (_Float16)-1032.f};
     const uint32_t u[4] = {a, b, c, d};
+    // in a vector register, so that the mask and the bits of 1024 go into one instruction (two constants do not)
+    uint32_t thousand = 0x64006400u;
+    asm("" : "+v"(thousand));
     half8_t r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const half2_t h = __builtin_bit_cast(half2_t, (u[i] & 0x000f000fu) | 0x64006400u) + off;
+        const half2_t h = __builtin_bit_cast(half2_t, (u[i] & 0x000f000fu) | thousand) + off;
         r[2 * i] = h.x;
         r[2 * i + 1] = h.y;
     }

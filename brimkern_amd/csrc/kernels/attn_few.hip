@@ -18,8 +18,6 @@
 // written rotated by row so that reading a column of chunks meets every bank once.
 #include "attn_common.h"
 
-#include <type_traits>
-
 namespace {
 
 template <int FMT, int D>
@@ -31,13 +29,28 @@ struct FewTile {
     static constexpr int SD = 16 * NG;                                   // dwords of the 32 keys' scales
     static constexpr int SI = (SD + 63) / 64;
     static constexpr int HP = FMT == FMT_Q4 ? 2 : 1;                     // planes of halves: scales, mins
-    static constexpr int K = 0, V = 512 * CH, KS = 2 * V, VS = KS + 4 * SD, E = VS + 4 * SD;
-    static constexpr int KM = E + 128, VM = KM + (HP - 1) * 8 * SD, STAGE = VM + (HP - 1) * 8 * SD;     // mins: f32
+    static constexpr int K = 0, V = 512 * CH, KS = 2 * V, VS = KS + 4 * SD, E = VS + 4 * SD, BAD = E + 128;
+    static constexpr int KM = BAD + 128, VM = KM + (HP - 1) * 8 * SD, STAGE = VM + (HP - 1) * 8 * SD;     // mins: f32
     static constexpr int OS = D + 4;                                     // floats of a row of the joined output
     static constexpr int JOIN = 16 * OS * 4;
     static constexpr int BYTES = STAGE > JOIN ? STAGE : JOIN;
-    // how far the chunks of a row are rotated: rows whose chunks would share banks differ
+    // Where chunk c of a row lies: moved by a number of the row, so that rows whose chunks would share banks differ. By
+    // exclusive or where the count of chunks is a power of two (one address and an instruction per chunk), else rotated.
+    static constexpr bool XOR = CH == 1 << P2;
     static __device__ __forceinline__ int rot(int row) { return (row >> (4 - P2)) & ((1 << P2) - 1); }
+    static __device__ __forceinline__ int chunk_at(int place, int row)        // which chunk lies at `place`
+    {
+        const int c = place - rot(row);
+        return XOR ? place ^ rot(row) : c < 0 ? c + CH : c;
+    }
+    // byte of chunk `first + step` (step a compile-time number, its bits apart from first's) of the row; base: of (row, first)
+    static __device__ __forceinline__ int base(int row, int first) { return XOR ? 16 * (row * CH + (first ^ rot(row))) : 16 * row * CH; }
+    static __device__ __forceinline__ int at(int base, int row, int first, int step)
+    {
+        if constexpr (XOR) return base ^ (16 * step);
+        const int c = first + step + rot(row);
+        return base + 16 * (c >= CH ? c - CH : c);
+    }
 };
 
 // A block of 32 keys in registers.
@@ -61,8 +74,7 @@ __device__ __forceinline__ void few_fetch(FewLoad<FMT, D>& f, const brik_attn_la
     for (int i = 0; i < T::NI; ++i) {
         const int c = 64 * i + lane, row = c / T::CH;
         if (T::CH % 2 && c >= 32 * T::CH) break;
-        int chunk = c - row * T::CH - T::rot(row);
-        chunk = chunk < 0 ? chunk + T::CH : chunk;
+        const int chunk = T::chunk_at(c - row * T::CH, row);
         const uint32_t off = 16u * (uint32_t)(row * T::CH + chunk);
         const size_t far = moved(row) * (16 * T::CH);
         f.k[i] = *(const u32x4_t*)(kb + far + off);
@@ -99,6 +111,18 @@ __device__ __forceinline__ void few_load(FewLoad<FMT, D>& f, const brik_attn_lau
     }
 }
 
+// Orders a wave's LDS writes before its own later reads of what other lanes wrote (a wave's LDS operations complete in issue
+// order, so this only binds the compiler).
+__device__ __forceinline__ void wave_lds_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+// Bits 15 and 31: a half of w that is infinite or NaN.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+
 __device__ __forceinline__ f32x2_t centred_mins(uint32_t s, uint32_t m)
 {
     f32x2_t r;
@@ -107,8 +131,9 @@ __device__ __forceinline__ f32x2_t centred_mins(uint32_t s, uint32_t m)
     return r;
 }
 
+// Into LDS. Returns whether some value scale or min is not finite: those are put in as 0, with a bit per key and group.
 template <int FMT, int D>
-__device__ __forceinline__ void few_spread(const FewLoad<FMT, D>& f, unsigned char* lds)
+__device__ __forceinline__ bool few_spread(const FewLoad<FMT, D>& f, unsigned char* lds)
 {
     using T = FewTile<FMT, D>;
     const int lane = threadIdx.x & 63;
@@ -118,28 +143,38 @@ __device__ __forceinline__ void few_spread(const FewLoad<FMT, D>& f, unsigned ch
         *(u32x4_t*)(lds + T::K + 1024 * i + 16 * lane) = f.k[i];
         *(u32x4_t*)(lds + T::V + 1024 * i + 16 * lane) = f.v[i];
     }
+    uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < T::SI; ++i) {
         const int d = 64 * i + lane;
         if (d < T::SD) {
             *(uint32_t*)(lds + T::KS + 4 * d) = f.ks[i];
             *(uint32_t*)(lds + T::VS + 4 * d) = f.vs[i];
+            odd |= not_finite(f.vs[i]);
             if constexpr (FMT == FMT_Q4) {
                 // a value is s n + m = s (n - 8) + (m + 8 s)
                 *(f32x2_t*)(lds + T::KM + 8 * d) = centred_mins(f.ks[i], f.ks[T::SI + i]);
                 *(f32x2_t*)(lds + T::VM + 8 * d) = centred_mins(f.vs[i], f.vs[T::SI + i]);
+                odd |= not_finite(f.vs[T::SI + i]);
             }
         }
     }
-}
-
-// Orders a wave's LDS writes before its own later reads of what other lanes wrote (a wave's LDS operations complete in issue
-// order, so this only binds the compiler).
-__device__ __forceinline__ void wave_lds_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    if (!__any(odd != 0)) return false;
+    // rare: those groups become 0, noted by key
+    if (lane < 32) *(uint32_t*)(lds + T::BAD + 4 * lane) = 0;
+    wave_lds_fence();
+#pragma unroll 1
+    for (int e = lane; e < 2 * T::SD; e += 64) {
+        uint16_t* const s = (uint16_t*)(lds + T::VS) + e;
+        bool bad = (*s & 0x7c00u) == 0x7c00u;
+        if constexpr (FMT == FMT_Q4) bad = bad || !(fabsf(((const float*)(lds + T::VM))[e]) <= 3.4028235e38f);
+        if (bad) {
+            *s = 0;
+            if constexpr (FMT == FMT_Q4) ((float*)(lds + T::VM))[e] = 0.f;
+            atomicOr((uint32_t*)(lds + T::BAD) + e / T::NG, 1u << (e % T::NG));
+        }
+    }
+    return true;
 }
 
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
@@ -153,19 +188,16 @@ __device__ __forceinline__ float half_of(const u32x2_t (&v)[N], int k)
     return f16_bits_to_f32((k & 1) ? w >> 16 : w & 0xffffu);
 }
 
+// One tile of 16 rows over its part of the keys.
 template <int FMT, int D>
-__device__ __forceinline__ void few_body(const brik_attn_launch& a)
+__device__ __forceinline__ void few_part(const brik_attn_launch& a, const Work& w, unsigned char* smem, float (&joinm)[4][16], float (&joinl)[4][16])
 {
     using T = FewTile<FMT, D>;
     constexpr int NG = T::NG;
     constexpr bool Q4 = FMT == FMT_Q4;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * T::BYTES];
-    __shared__ float joinm[4][16], joinl[4][16];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
     unsigned char* const lds = smem + wave * T::BYTES;
 
-    Work w;
-    if (!find_work<16>(a, w)) return;
     const Row row = find_row<16>(a, w, w.r0, m);
     int t0, t1;
     find_keys(w, wave_min(row.real ? row.lo : 0x7fffffff), wave_max(row.real ? row.hi : 0), 4, t0, t1);
@@ -223,16 +255,18 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 
     f32x4_t o[2 * NG];
     float om[NG], M = ATTN_NONE, l = 0.f;
+    uint32_t bad = 0;                                    // groups of which this lane's row has seen a value that is not finite
 #pragma unroll
     for (int n = 0; n < 2 * NG; ++n) o[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) om[g] = 0.f;
 
     // row of V that this lane's address names in a transposed read: keys 4 q .. 4 q + 3 of both 16-key halves
-    const int vrow = ((lane & 15) >> 3) * 16 + 4 * q + (((lane & 15) >> 1) & 3);
+    const int vrow = ((lane & 15) >> 3) * 16 + 4 * q + (((lane & 15) >> 1) & 3), vbase = T::base(vrow, 0);
+    const int kfirst = Q4 ? 0 : q >> 1, kbase = T::base(m, kfirst);
 
-    // One block of keys, in LDS. masked: some of its keys are not seen by some row.
-    auto block = [&](auto masked, int t, const bool (&have)[2]) {
+    // One block of keys, in LDS. general: some of its keys are not seen by some row, or some values are not finite (odd).
+    auto block = [&](bool general, bool odd, int t, const bool (&have)[2]) {
         // e_j of the 32 keys
         {
             const uint16_t* const s = (const uint16_t*)(lds + T::VS) + (lane & 31) * NG;
@@ -252,20 +286,17 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
                 s[g] = *(const u32x2_t*)(lds + T::KS + (16 * i + 4 * q) * 2 * NG + 8 * g);
                 if constexpr (Q4) mn[g] = *(const f32x4_t*)(lds + T::KM + (16 * i + 4 * q) * 4 * NG + 16 * g);
             }
-            const int krow = 16 * i + m;
             float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 half8_t k;
+                // (rows 16 apart are moved alike)
+                const unsigned char* const src = lds + T::K + 256 * T::CH * i + T::at(kbase, m, kfirst, Q4 ? g : 2 * g);
                 if constexpr (Q4) {
-                    int chunk = g + T::rot(krow);
-                    chunk = chunk >= T::CH ? chunk - T::CH : chunk;
-                    const uint32_t c = *(const uint32_t*)(lds + T::K + krow * 16 * T::CH + 16 * chunk + 4 * q);
+                    const uint32_t c = *(const uint32_t*)(src + 4 * q);
                     k = centred_q4(c, c >> 4, c >> 8, c >> 12);
                 } else {
-                    int chunk = 2 * g + (q >> 1) + T::rot(krow);
-                    chunk = chunk >= T::CH ? chunk - T::CH : chunk;
-                    const u32x2_t c = *(const u32x2_t*)(lds + T::K + krow * 16 * T::CH + 16 * chunk + 8 * (q & 1));
+                    const u32x2_t c = *(const u32x2_t*)(src + 8 * (q & 1));
                     k = halves_q8(c.x, c.y);
                 }
                 floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -278,27 +309,29 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[4 * i + r] = x[r] * xs;
+            for (int r = 0; r < 4; ++r) y[4 * i + r] = x[r];
         }
+        float mul = xs;                                  // scores are y * mul
         if (cap) {
+            mul = 1.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = ys * attn_tanh(y[i]);
+            for (int i = 0; i < 8; ++i) y[i] = ys * attn_tanh(y[i] * xs);
         }
-        uint32_t seen = 0;
-        if constexpr (masked) {
+        if (general) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int key = 32 * t + 16 * (i >> 2) + 4 * q + (i & 3);
-                const bool in = key >= row.lo && key < row.hi && have[i >> 2];
-                seen |= (uint32_t)in << i;
-                y[i] = in ? y[i] : -__builtin_inff();
+                const int k = 16 * (i >> 2) + 4 * q + (i & 3);
+                const bool in = 32 * t + k >= row.lo && 32 * t + k < row.hi && have[i >> 2];
+                y[i] = in ? y[i] * mul : -__builtin_inff();
+                if (odd) bad |= in ? *(const uint32_t*)(lds + T::BAD + 4 * k) : 0u;
             }
+            mul = 1.f;
         }
         wave_lds_fence();
         const f32x4_t e0 = *(const f32x4_t*)(lds + T::E + 16 * q), e1 = *(const f32x4_t*)(lds + T::E + 64 + 16 * q);
         float tm = ATTN_NONE;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, fmaxf(y[i] + e0[i], y[4 + i] + e1[i]));
+        for (int i = 0; i < 4; ++i) tm = fmaxf(tm, fmaxf(fmaf(y[i], mul, e0[i]), fmaf(y[4 + i], mul, e1[i])));
         if (__any(tm > M + 8.f)) {
             const float Mn = fmaxf(M, quarters_max(tm)), f = __builtin_amdgcn_exp2f(M - Mn);
             M = Mn;
@@ -309,9 +342,10 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
             for (int g = 0; g < NG; ++g) om[g] *= f;
         }
         float p[8];
+        const float shift = 7.f - M;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(y[i] - (M - 7.f));
+            p[i] = __builtin_amdgcn_exp2f(fmaf(y[i], mul, shift));
             l += p[i];
         }
         u32x2_t s0[NG], s1[NG];
@@ -332,16 +366,13 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 ps[i] = fmaf(i < 4 ? half_of(s0, i * NG + g) : half_of(s1, (i - 4) * NG + g), p[i], 0.f);
-                // 0 times an infinity or a NaN of a token that is not seen
-                if constexpr (masked) ps[i] = (seen >> i) & 1 ? ps[i] : 0.f;
-                if constexpr (Q4) {
-                    const float mn = i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3];
-                    om[g] = fmaf(p[i], !masked || ((seen >> i) & 1) ? mn : 0.f, om[g]);
-                }
+                if constexpr (Q4)
+                    om[g] = fmaf(p[i], i < 4 ? m0[(i * NG + g) >> 2][(i * NG + g) & 3] : m1[((i - 4) * NG + g) >> 2][((i - 4) * NG + g) & 3], om[g]);
             }
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                // the order of V's conversion: keys 0, 2, 1, 3 of each half
+                // the order of V's conversion: keys 0, 2, 1, 3 of each half. (The product rounded to a half in one
+                // instruction, and again for the rest of it, takes twice the time of these four.)
                 const float u = ps[(i & 4) + ((i & 2) >> 1)], v = ps[(i & 4) + ((i & 2) >> 1) + 2];
                 const half2_t h = halves(u, v);
                 phw[i / 2] = __builtin_bit_cast(uint32_t, h);
@@ -349,9 +380,7 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
             }
             const half8_t ph = __builtin_bit_cast(half8_t, phw), pl = __builtin_bit_cast(half8_t, plw);
             if constexpr (Q4) {
-                int chunk = g + T::rot(vrow);
-                chunk = chunk >= T::CH ? chunk - T::CH : chunk;
-                const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(lds + T::V + vrow * 16 * T::CH + 16 * chunk + 8 * (lane & 1)));
+                const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(lds + T::V + T::at(vbase, vrow, 0, g) + 8 * (lane & 1)));
                 const uint32_t c0 = (uint32_t)c.x, c1 = (uint32_t)c.y;
                 const half8_t lo = centred_q4(c0, c0 >> 8, c1, c1 >> 8), hi = centred_q4(c0 >> 4, c0 >> 12, c1 >> 4, c1 >> 12);
                 o[2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ph, o[2 * g], 0, 0, 0);
@@ -361,9 +390,7 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
             } else {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    int chunk = 2 * g + j + T::rot(vrow);
-                    chunk = chunk >= T::CH ? chunk - T::CH : chunk;
-                    const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(lds + T::V + vrow * 16 * T::CH + 16 * chunk + 8 * (lane & 1)));
+                    const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)(lds + T::V + T::at(vbase, vrow, 0, 2 * g + j) + 8 * (lane & 1)));
                     const half8_t v = halves_q8((uint32_t)c.x, (uint32_t)c.y);
                     o[2 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[2 * g + j], 0, 0, 0);
                     o[2 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[2 * g + j], 0, 0, 0);
@@ -375,18 +402,20 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
     for (; t < t1; t += 4) {
         const bool have[2] = {kp.p[0] >= 0, kp.p[1] >= 0};
         wave_lds_fence();
-        few_spread(next, lds);
+        const bool odd = few_spread(next, lds);
         if (t + 4 < t1) {
             kp = window.of(t + 4);
             few_load(next, a, w, t + 4, kp);
         }
         wave_lds_fence();
-        if (32 * t >= all_lo && 32 * t + 32 <= all_hi && have[0] && have[1]) block(std::false_type{}, t, have);
-        else block(std::true_type{}, t, have);
+        const bool plain = 32 * t >= all_lo && 32 * t + 32 <= all_hi && have[0] && have[1] && !odd;
+        block(!plain, odd, t, have);
     }
 
     // the four waves' results joined in LDS
     l = quarters_sum(l);
+    bad |= (uint32_t)__shfl_xor((int)bad, 16);
+    bad |= (uint32_t)__shfl_xor((int)bad, 32);
     if (q == 0) {
         joinm[wave][m] = M;
         joinl[wave][m] = l;
@@ -397,6 +426,7 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
     float* const mine = (float*)lds + m * T::OS;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
+        if ((bad >> g) & 1) o[2 * g] = o[2 * g + 1] = f32x4_t{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
         if constexpr (Q4) {
             const float add = quarters_sum(om[g]);
             // tile 2 g + j, row 4 q + r holds value 32 g + 2 (4 q + r) + j
@@ -435,6 +465,35 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
             if (L != 0.f) *(f32x4_t*)(a.part + at * D + d) = v;
             if (d == 0) *(f32x2_t*)(a.ml + 2 * at) = f32x2_t{Mr, L};
         }
+    }
+}
+
+template <int FMT, int D>
+__device__ __forceinline__ void few_body(const brik_attn_launch& a)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char smem[4 * FewTile<FMT, D>::BYTES];
+    __shared__ float joinm[4][16], joinl[4][16];
+    // One tile's keys, or parts of one sequence after the other.
+    Work w;
+    w.head = (a.first_block + (int)blockIdx.x) % a.c.heads;
+    const int own = (a.first_block + (int)blockIdx.x) / a.c.heads - a.prefix_tiles * a.prefix_splits;
+    const bool parts = a.own_blocks && own >= 0;
+    int each = 0, g = 0, end = 0;
+    if (parts) {
+        const Share share(a);
+        each = uniform(share.each);
+        g = own * each;
+        end = min(g + each, uniform(share.total));
+        if (g >= end) return;
+        w.prefix = false;
+    } else if (!find_work<16>(a, w)) {
+        return;
+    }
+    for (;;) {
+        if (parts) next_part(a, each, own, end, g, w);
+        few_part<FMT, D>(a, w, smem, joinm, joinl);
+        if (!parts || g >= end) return;
+        __syncthreads();
     }
 }
 

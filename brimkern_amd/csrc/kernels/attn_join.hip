@@ -8,19 +8,19 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
     const int D = a.c.head_dim, quads = D / 4, groups = 256 / quads;
     const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const size_t all = (size_t)a.s.rows * a.a.heads, row = (size_t)t * a.a.heads + h;
-    // vector of slot s: the prefix's and static ones are `all` apart, a sequence's blocks 16
+    // vector of slot s: the prefix's and static ones are `all` apart, a sequence's parts 16
     int slots = a.prefix_splits + a.own_splits;
     size_t own = 0;
     if (a.own_blocks) {
-        Share share(a);                                              // first: its loads and the search's go together
-        const int b = seq_of_row(a.s, t);
+        const Share share(a);                                        // first: its loads and the search's go together
+        int b = uniform(seq_of_row(a.s, t)), start;
         if (b >= a.s.seqs) return;                                   // behind the last sequence
+        const Seq q = Share::find(a, b, 0, start);
         const int G = a.a.heads / a.c.heads, kvh = h / G;
-        int first, count;
-        share.blocks_of(a, b, first, count);
+        const int first = start / share.each, count = q.n ? (start + q.n - 1) / share.each - first + 1 : 0;
         if (count == 1 && a.prefix_splits == 0) return;              // written by its block
         slots = a.prefix_splits + count;
-        own = a.prefix_splits * all + ((size_t)kvh * a.own_blocks + first) * 16 + (t - __builtin_amdgcn_readlane(share.mine.row, b & 63)) * G + (h - kvh * G);
+        own = a.prefix_splits * all + ((size_t)kvh * (a.own_blocks + a.s.seqs) + first + b) * 16 + (t - q.row) * G + (h - kvh * G);
     } else if (a.s.row_off && t >= a.s.row_off[a.s.seqs]) {
         return;
     }
