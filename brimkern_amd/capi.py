@@ -20,6 +20,7 @@ BRIK_OPT_PATH, BRIK_OPT_GEMV_VARIANT = 1, 2
 BRIK_GEMV_VARIANTS = 11
 BRIK_OPT_GEMM_TILE, BRIK_GEMM_TILES = 3, 23
 BRIK_OPT_PLAN_STAGE, BRIK_OPT_PLAN_SETS, BRIK_OPT_SPLITK, BRIK_OPT_GEMV_BLOCKS = 4, 5, 6, 7
+BRIK_OPT_ATTN_ROWS, BRIK_OPT_ATTN_SPLITS = 8, 9
 PATH_AUTO, PATH_GEMV, PATH_GEMM = 0, 1, 2
 BRIK_PATH_GEMV, BRIK_PATH_GEMV_STAGED, BRIK_PATH_TILED, BRIK_PATH_SPLITK = 1, 2, 3, 4
 

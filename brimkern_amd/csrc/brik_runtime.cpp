@@ -260,6 +260,8 @@ struct brik_ctx {
     int opt_plan_sets = 0;   // plans: 0 auto, else row sets per block
     int opt_splitk = 0;      // GEMMs of few rows: 0 auto, 1 neither kernel for them, 2 split-K, 3 the few-row one
     int opt_gemv_blocks = 0; // single-matrix GEMV: 0 auto, else grid cap
+    int opt_attn_rows = 0;   // attention: 0 auto, else rows of a tile
+    int opt_attn_splits = 0; // attention: 0 auto, else splits of every tile's keys
     void* ws = nullptr;    // GEMM workspace: f16 activation rows, then per-row scales (grow-only)
     size_t ws_bytes = 0;
     void* tws = nullptr;   // top-k workspace: lane maxima, then LM-head logits (grow-only)
@@ -2536,8 +2538,9 @@ int brik_kv_read(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* b
 
 // Splits of a section's keys (at most `keys` of them): enough blocks to fill the device, each with at least four blocks
 // of 32 keys, one per wave.
-static int attn_splits(long blocks, long keys)
+static int attn_splits(const brik_ctx* c, long blocks, long keys)
 {
+    if (c->opt_attn_splits) return c->opt_attn_splits;
     const long most = std::max(1l, (keys + 127) / 128), want = (2 * kCUs + blocks - 1) / std::max(1l, blocks);
     return (int)std::min({most, std::max(1l, want), 64l});
 }
@@ -2554,6 +2557,7 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     // Row tiles of 256 or 128 where they fill the device without splitting keys, else of 16 (a 32-key step of a tile takes 3 us
     // however few blocks there are: 805 rows of 7 heads behind a window of 1024 keys 71 us by 256, 31 us by 16 rows).
     auto tile_rows = [&](long most_rows, long all_rows) {
+        if (c->opt_attn_rows) return a.c.head_dim > 128 ? std::min(c->opt_attn_rows, 128) : c->opt_attn_rows;
         const long fill = KV * ((all_rows * G + 255) / 256);
         if (most_rows * G <= 16 || fill < kCUs / 2) return 16;
         return a.c.head_dim > 128 || most_rows * G <= 128 ? 128 : 256;
@@ -2571,16 +2575,16 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     // that the call finds. (Splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for the longest. Up to
     // 1024 keys a block per sequence is as fast, and one that begins a second sequence pays 4 us for it.)
     const long blocks32 = (std::max(0l, own_keys) + 31) / 32;
-    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32) {
+    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32 && !c->opt_attn_splits) {
         a.own_blocks = (int)std::max(1l, std::min<long>((2 * kCUs + KV - 1) / KV, a.s.seqs * ((blocks32 + 3) / 4)));
         tiles = a.own_blocks;
         a.own_splits = 1;
     } else {
-        a.own_splits = attn_splits(KV * tiles, own_keys);
+        a.own_splits = attn_splits(c, KV * tiles, own_keys);
     }
     if (prefix_keys > 0) {
         a.prefix_tiles = (int)((rows * G + prefix_bm - 1) / prefix_bm);
-        a.prefix_splits = attn_splits(KV * a.prefix_tiles, prefix_keys);
+        a.prefix_splits = attn_splits(c, KV * a.prefix_tiles, prefix_keys);
     }
     a.whole = a.prefix_splits == 0 && a.own_splits == 1 && a.own_blocks == 0;
     if (!a.whole) {
@@ -2591,7 +2595,8 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         a.ml = a.part + vectors * d;
     }
     const long own_blocks = KV * tiles * a.own_splits, prefix_blocks = KV * a.prefix_tiles * a.prefix_splits;
-    if (own_blocks + prefix_blocks >= (1l << 24)) return fail(c, BRIK_EINVAL, "attention: %ld blocks in one call", own_blocks + prefix_blocks);
+    c->last_kernel = own_bm == 16 ? "attn_few" : own_bm == 128 ? "attn_tile4" : "attn_tile8";
+    if (own_blocks + prefix_blocks >= (1l << 23)) return fail(c, BRIK_EINVAL, "attention: %ld blocks in one call", own_blocks + prefix_blocks);
     auto run = [&](int bm, long blocks) {
         const int k = bm == 16 ? A_FEW : bm == 128 ? A_TILE4 : A_TILE8;
         void* args[] = {&a};
@@ -2766,6 +2771,15 @@ int brik_set_option(brik_ctx* c, int key, int value)
         if (value < 0 || value > (int)kGemvMaxBlocks)
             return fail(c, BRIK_EINVAL, "BRIK_OPT_GEMV_BLOCKS: %d not in 0..%u", value, kGemvMaxBlocks);
         c->opt_gemv_blocks = value;
+        return BRIK_OK;
+    case BRIK_OPT_ATTN_ROWS:
+        if (value != 0 && value != 16 && value != 128 && value != 256)
+            return fail(c, BRIK_EINVAL, "BRIK_OPT_ATTN_ROWS: %d is not 0, 16, 128 or 256", value);
+        c->opt_attn_rows = value;
+        return BRIK_OK;
+    case BRIK_OPT_ATTN_SPLITS:
+        if (value < 0 || value > 256) return fail(c, BRIK_EINVAL, "BRIK_OPT_ATTN_SPLITS: %d not in 0..256", value);
+        c->opt_attn_splits = value;
         return BRIK_OK;
     default:
         return fail(c, BRIK_EINVAL, "unknown option %d", key);

@@ -500,8 +500,8 @@ __device__ __forceinline__ void few_body(const brik_attn_launch& a)
 }  // namespace
 
 #define BRIK_ATTN_FEW(D)                                                                                                             \
-    extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void brik_attn_few_q8_##D(brik_attn_launch a) { few_body<FMT_Q8, D>(a); }             \
-    extern "C" __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void brik_attn_few_q4_##D(brik_attn_launch a) { few_body<FMT_Q4, D>(a); }
+    extern "C" __global__ __launch_bounds__(256, D <= 64 ? 3 : D <= 128 ? 2 : 1) void brik_attn_few_q8_##D(brik_attn_launch a) { few_body<FMT_Q8, D>(a); }             \
+    extern "C" __global__ __launch_bounds__(256, D <= 64 ? 3 : D <= 128 ? 2 : 1) void brik_attn_few_q4_##D(brik_attn_launch a) { few_body<FMT_Q4, D>(a); }
 BRIK_ATTN_FEW(64)
 BRIK_ATTN_FEW(96)
 BRIK_ATTN_FEW(128)

@@ -470,6 +470,9 @@ int brik_timer_end(brik_ctx *ctx, float *ms);
                                     3 the few-row kernel for the dense calls of at most 64 rows that it takes */
 #define BRIK_OPT_GEMV_BLOCKS 7   /* single-matrix GEMV launches: 0 auto, else at most this many blocks
                                     (each block then loops over several row sets) */
+#define BRIK_OPT_ATTN_ROWS 8       /* attention: 0 auto, else 16, 128 or 256 rows (row x query head of a key / value head) per
+                                    tile (256: as 128 where head_dim > 128) */
+#define BRIK_OPT_ATTN_SPLITS 9     /* attention: 0 auto, else every tile's keys split over so many blocks (up to 256) */
 int brik_set_option(brik_ctx *ctx, int key, int value);
 
 /* The path the last brik_matmul_t_* / brik_matmul_t_q4_noalloc / brik_moe_matmul_t_q4* call on this
@@ -485,7 +488,8 @@ int brik_last_path(const brik_ctx *ctx);
 /* The product kernel behind it, by the stem of its name without brik_ ("" before any call, or for K = 0):
  * gemv, gemm (tiled), gemmg (expert-grouped), gemm_sk (split-K), gemm_few (few rows), gemm_frag (fragments);
  * gemv_f16w, gemm_h, gemm_f16, gemm_f16w for f16 weights (and gemm_few); gemm_conv (tap by tap), gemm or
- * gemm_sk (im2col rows), conv2d_direct for convolutions. A diagnostic as brik_last_path. */
+ * gemm_sk (im2col rows), conv2d_direct for convolutions; attn_few (16 rows a tile), attn_tile4 (128), attn_tile8 (256) for the
+ * own keys of an attention. A diagnostic as brik_last_path. */
 const char *brik_last_kernel(const brik_ctx *ctx);
 
 #ifdef __cplusplus

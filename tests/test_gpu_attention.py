@@ -11,7 +11,7 @@ import pytest
 
 import kvref as R
 from brimkern_amd import synth
-from brimkern_amd.capi import BrikError, BRIK_EALIGN, BRIK_EINVAL, Context
+from brimkern_amd.capi import (BrikError, BRIK_EALIGN, BRIK_EINVAL, BRIK_OPT_ATTN_ROWS, BRIK_OPT_ATTN_SPLITS, Context)
 
 pytestmark = pytest.mark.gpu
 f32 = np.float32
@@ -256,6 +256,91 @@ def test_strides(dev, fmt):
     got = dev.down(ob, 6, 300)
     close(got[:, :256].reshape(6, 4, 64), a.want())
     assert np.isnan(got[:, 256:]).all()
+
+
+@pytest.fixture(params=[(16, 1), (16, 5), (128, 0), (128, 1), (128, 3), (256, 1), (256, 7)], ids=lambda p: f"rows{p[0]}-splits{p[1]}")
+def forced(request, ctx):
+    """The kernels by tile rows, their keys whole or split, whatever the sizes would choose."""
+    ctx.set_option(BRIK_OPT_ATTN_ROWS, request.param[0])
+    ctx.set_option(BRIK_OPT_ATTN_SPLITS, request.param[1])
+    yield request.param
+    ctx.set_option(BRIK_OPT_ATTN_ROWS, 0)
+    ctx.set_option(BRIK_OPT_ATTN_SPLITS, 0)
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+@pytest.mark.parametrize("H,KV,D,P,rows,lens,more", [
+    (8, 2, 128, 16, [70, 1, 0, 33], [70, 300, 5, 161], {}),
+    (14, 2, 64, 64, [40, 3], [333, 2], dict(window=50)),
+    (6, 3, 96, 32, [150, 20], [150, 90], dict(softcap=3.0, qscale=2.0)),
+    (4, 1, 192, 128, [65], [200], dict(behind=3)),
+    (10, 2, 256, 16, [30, 31], [97, 64], dict(window=17, softcap=20.0)),
+    (12, 3, 64, 16, [1, 2, 40], [203, 230, 240], dict(prefix=200)),
+    (8, 8, 128, 32, [20, 1], [90, 80], dict(prefix=77, window=60)),
+    (4, 2, 128, 16, [5, 50], [40, 300], dict(bad=[(0, 1, -1), (1, 3, 1 << 20)])),
+    (8, 2, 128, 32, [1, 60], [300, 100], dict(kscale=30.0, vscale=3e3, qscale=0.03, scale=0.1)),
+    (8, 2, 64, 32, [33], [100], dict(scale=-0.2)),
+])
+def test_every_kernel(dev, forced, fmt, H, KV, D, P, rows, lens, more):
+    c = Case(dev, fmt, H, KV, D, P, rows, lens, seed=D + H, **more)
+    c.check()
+    assert dev.ctx.last_kernel() == {16: "attn_few", 128: "attn_tile4", 256: "attn_tile4" if D > 128 else "attn_tile8"}[forced[0]]
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_every_kernel_on_hard_values(dev, forced, fmt, D):
+    """Values of very different size, rows of NaN, tokens with scales that are not finite: seen by later rows only."""
+    a = Case(dev, fmt, 4, 1, D, 16, [90, 3], [90, 64], seed=7)
+    rng = np.random.default_rng(5)
+    for ids, n in zip(a.tables, a.lens):
+        v = (rng.standard_normal((n, 1, D)) * 2.0 ** rng.integers(-9, 10, (n, 1, 1))).astype(f32)
+        a.c.put(ids, a.c.get("k", ids, n).astype(f32), v)
+    a.cache = dev.cache(a.c)
+    a.check()
+    a.q[40, 2] = np.nan
+    dev.ctx.h2d(a.args.q, a.q)
+    want = a.want(np.nan_to_num(a.q))
+    for n, p, t, g, bits in (("v", dev.pv, 60, 1, 0x7C00), ("v", dev.pv, 75, 0, 0xFE00)):
+        a.c.planes[n][1][a.tables[0][t // 16], 0, t % 16, g] = bits
+        dev.ctx.h2d(p[1], a.c.planes[n][1])
+    got = a.run()
+    assert np.isnan(got[40, 2]).all()
+    ok = np.ones(got.shape[:2], bool)
+    ok[40, 2] = False
+    ok[60:90] = False
+    close(got[ok], want[ok])
+    assert not np.isfinite(got[60:90, :, 32:64]).any() and not np.isfinite(got[75:90, :, :32]).any()
+    assert np.isfinite(got[60:75, :, :32]).all() and np.isfinite(got[60:90, :, 64:]).all()
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+@pytest.mark.parametrize("D,KV,H", [(64, 1, 4), (128, 2, 8), (96, 4, 4)])
+def test_shared_out_keys(dev, fmt, D, KV, H):
+    """Decoding of many sequences, one long: blocks end one sequence and begin the next, in the middle of 64 sequences and past
+    them; sequences without keys, without rows, with fewer keys than a block takes."""
+    rng = np.random.default_rng(D)
+    lens = [int(x) for x in rng.integers(0, 120, 90)]
+    lens[3], lens[50], lens[64], lens[66], lens[70], lens[89] = 1500, 0, 0, 700, 33, 0
+    rows = [1] * 90
+    rows[10] = rows[63] = rows[80] = 0
+    rows[20] = 3
+    lens[20] = 2
+    Case(dev, fmt, H, KV, D, 32, rows, lens, seed=2).check()
+    Case(dev, fmt, H, KV, D, 16, [1, 1, 1], [1100, 1, 2000], seed=3, window=700).check()
+
+
+@pytest.mark.parametrize("D,lens", [(64, [2500, 700, 2180, 31]), (192, [3100]), (96, [1290, 1025])])
+def test_joins_of_many_parts(dev, D, lens):
+    """Every number of parts: weights come from other lanes of the wave that joins them."""
+    a = Case(dev, "q8", 2, 1, D, 64, [1] * len(lens), lens, seed=4)
+    a.check()
+    for splits in (2, 3, 16, 17, 31, 33, 64, 65, 80):
+        dev.ctx.set_option(BRIK_OPT_ATTN_SPLITS, splits)
+        try:
+            a.check()
+        finally:
+            dev.ctx.set_option(BRIK_OPT_ATTN_SPLITS, 0)
 
 
 @pytest.mark.parametrize("fmt", ["q8", "q4"])
@@ -508,3 +593,11 @@ def test_refusals(dev):
     wrong = dev.batch([2], [9], [a.tables[0]])
     wrong.prefix_len = 3
     refused(BRIK_EINVAL, batch=wrong)
+
+
+def test_option_refusals(ctx):
+    for option, values in ((BRIK_OPT_ATTN_ROWS, (-1, 1, 32, 64, 512)), (BRIK_OPT_ATTN_SPLITS, (-1, 257))):
+        for value in values:
+            with pytest.raises(BrikError) as e:
+                ctx.set_option(option, value)
+            assert e.value.code == BRIK_EINVAL
