@@ -705,6 +705,181 @@ napi_value F16ToF32(napi_env env, napi_callback_info info)   // (ctx, src, out, 
     return undefined(env);
 }
 
+// ---- a cache of quantized keys and values, and attention over it ------------------------------
+
+// A named property of `o`; absent, undefined and null leave `*has` false.
+bool get_field(napi_env env, napi_value o, const char* name, napi_value* out, bool* has)
+{
+    napi_valuetype t;
+    NAPI_CALL_B(env, napi_typeof(env, o, &t));
+    if (t != napi_object) {
+        napi_throw_type_error(env, "BRIK_EINVAL", "expected an object");
+        return false;
+    }
+    NAPI_CALL_B(env, napi_get_named_property(env, o, name, out));
+    NAPI_CALL_B(env, napi_typeof(env, *out, &t));
+    *has = t != napi_undefined && t != napi_null;
+    return true;
+}
+
+// Optional fields: as they are where absent.
+bool opt_ptr(napi_env env, napi_value o, const char* name, void** out)
+{
+    napi_value f;
+    bool has;
+    return get_field(env, o, name, &f, &has) && (!has || get_ptr(env, f, out));
+}
+bool opt_f32(napi_env env, napi_value o, const char* name, float* out)
+{
+    napi_value f;
+    bool has;
+    return get_field(env, o, name, &f, &has) && (!has || get_f32(env, f, out));
+}
+// An integer of the range of its C type: anything else is refused, not cut off.
+bool opt_int(napi_env env, napi_value o, const char* name, double most, double* out)
+{
+    napi_value f;
+    bool has;
+    if (!get_field(env, o, name, &f, &has)) return false;
+    if (!has) return true;
+    if (napi_get_value_double(env, f, out) != napi_ok || !(*out >= -most && *out <= most) || *out != (double)(int64_t)*out) {
+        napi_throw_type_error(env, "BRIK_EINVAL", (std::string("expected an integer: ") + name).c_str());
+        return false;
+    }
+    return true;
+}
+bool opt_i32(napi_env env, napi_value o, const char* name, int32_t* out)
+{
+    double d = *out;
+    if (!opt_int(env, o, name, 2147483647.0, &d)) return false;
+    *out = (int32_t)d;
+    return true;
+}
+bool opt_i64(napi_env env, napi_value o, const char* name, int64_t* out)
+{
+    double d = (double)*out;
+    if (!opt_int(env, o, name, 9007199254740991.0, &d)) return false;
+    *out = (int64_t)d;
+    return true;
+}
+
+bool get_kv_cache(napi_env env, napi_value o, brik_kv_cache* c)
+{
+    void* p[6] = {};
+    static const char* const names[6] = {"k", "v", "kScales", "vScales", "kMins", "vMins"};
+    *c = brik_kv_cache{};
+    for (int i = 0; i < 6; ++i)
+        if (!opt_ptr(env, o, names[i], &p[i])) return false;
+    c->k = p[0];
+    c->v = p[1];
+    c->k_scales = (uint16_t*)p[2];
+    c->v_scales = (uint16_t*)p[3];
+    c->k_mins = (uint16_t*)p[4];
+    c->v_mins = (uint16_t*)p[5];
+    return opt_i32(env, o, "fmt", &c->fmt) && opt_i32(env, o, "heads", &c->heads) && opt_i32(env, o, "headDim", &c->head_dim) &&
+           opt_i32(env, o, "page", &c->page) && opt_i32(env, o, "pages", &c->pages);
+}
+
+bool get_kv_batch(napi_env env, napi_value o, brik_kv_batch* b)
+{
+    void* p[4] = {};
+    static const char* const names[4] = {"rowOff", "kvLen", "table", "prefixTable"};
+    *b = brik_kv_batch{};
+    for (int i = 0; i < 4; ++i)
+        if (!opt_ptr(env, o, names[i], &p[i])) return false;
+    b->row_off = (const int32_t*)p[0];
+    b->kv_len = (const int32_t*)p[1];
+    b->table = (const int32_t*)p[2];
+    b->prefix_table = (const int32_t*)p[3];
+    return opt_i32(env, o, "seqs", &b->seqs) && opt_i32(env, o, "rows", &b->rows) && opt_i32(env, o, "tableCols", &b->table_cols) &&
+           opt_i32(env, o, "maxLen", &b->max_len) && opt_i32(env, o, "maxRows", &b->max_rows) &&
+           opt_i32(env, o, "prefixLen", &b->prefix_len);
+}
+
+bool get_qkv_rows(napi_env env, napi_value o, brik_qkv_rows* r)
+{
+    void* p[9] = {};
+    static const char* const names[9] = {"q", "k", "v", "qOut", "kOut", "qNorm", "kNorm", "invFreq", "positions"};
+    *r = brik_qkv_rows{};
+    r->eps = 1e-6f;
+    for (int i = 0; i < 9; ++i)
+        if (!opt_ptr(env, o, names[i], &p[i])) return false;
+    r->q = (const float*)p[0];
+    r->k = (const float*)p[1];
+    r->v = (const float*)p[2];
+    r->q_out = (float*)p[3];
+    r->k_out = (float*)p[4];
+    r->q_norm = (const float*)p[5];
+    r->k_norm = (const float*)p[6];
+    r->inv_freq = (const float*)p[7];
+    r->positions = (const int32_t*)p[8];
+    return opt_i64(env, o, "qStride", &r->q_stride) && opt_i64(env, o, "kStride", &r->k_stride) &&
+           opt_i64(env, o, "vStride", &r->v_stride) && opt_i64(env, o, "qOutStride", &r->q_out_stride) &&
+           opt_i64(env, o, "kOutStride", &r->k_out_stride) && opt_i32(env, o, "heads", &r->heads) &&
+           opt_i32(env, o, "kvHeads", &r->kv_heads) && opt_i32(env, o, "headDim", &r->head_dim) &&
+           opt_i32(env, o, "rotDim", &r->rot_dim) && opt_i32(env, o, "flags", &r->flags) && opt_f32(env, o, "eps", &r->eps);
+}
+
+napi_value QkNormRope(napi_env env, napi_callback_info info)   // (ctx, batch, rows)
+{
+    Args a;
+    brik_ctx* c;
+    brik_kv_batch b;
+    brik_qkv_rows r;
+    if (!get_args(env, info, a, 3) || !get_ctx(env, a.v[0], &c) || !get_kv_batch(env, a.v[1], &b) || !get_qkv_rows(env, a.v[2], &r))
+        return nullptr;
+    if (check(env, c, brik_qk_norm_rope(c, &b, &r))) return nullptr;
+    return undefined(env);
+}
+
+napi_value KvWrite(napi_env env, napi_callback_info info)   // (ctx, cache, batch, rows)
+{
+    Args a;
+    brik_ctx* c;
+    brik_kv_cache k;
+    brik_kv_batch b;
+    brik_qkv_rows r;
+    if (!get_args(env, info, a, 4) || !get_ctx(env, a.v[0], &c) || !get_kv_cache(env, a.v[1], &k) || !get_kv_batch(env, a.v[2], &b) ||
+        !get_qkv_rows(env, a.v[3], &r))
+        return nullptr;
+    if (check(env, c, brik_kv_write(c, &k, &b, &r))) return nullptr;
+    return undefined(env);
+}
+
+napi_value KvRead(napi_env env, napi_callback_info info)   // (ctx, cache, batch, k, v)
+{
+    Args a;
+    brik_ctx* c;
+    brik_kv_cache kc;
+    brik_kv_batch b;
+    void *k, *v;
+    if (!get_args(env, info, a, 5) || !get_ctx(env, a.v[0], &c) || !get_kv_cache(env, a.v[1], &kc) || !get_kv_batch(env, a.v[2], &b) ||
+        !get_ptr(env, a.v[3], &k) || !get_ptr(env, a.v[4], &v))
+        return nullptr;
+    if (check(env, c, brik_kv_read(c, &kc, &b, (float*)k, (float*)v))) return nullptr;
+    return undefined(env);
+}
+
+napi_value Attention(napi_env env, napi_callback_info info)   // (ctx, cache, batch, {q, out, heads, scale, ...})
+{
+    Args a;
+    brik_ctx* c;
+    brik_kv_cache k;
+    brik_kv_batch b;
+    brik_attn_args t{};
+    void *q = nullptr, *out = nullptr;
+    if (!get_args(env, info, a, 4) || !get_ctx(env, a.v[0], &c) || !get_kv_cache(env, a.v[1], &k) || !get_kv_batch(env, a.v[2], &b) ||
+        !opt_ptr(env, a.v[3], "q", &q) || !opt_ptr(env, a.v[3], "out", &out) || !opt_i64(env, a.v[3], "qStride", &t.q_stride) ||
+        !opt_i64(env, a.v[3], "outStride", &t.out_stride) || !opt_i32(env, a.v[3], "heads", &t.heads) ||
+        !opt_i32(env, a.v[3], "window", &t.window) || !opt_f32(env, a.v[3], "scale", &t.scale) ||
+        !opt_f32(env, a.v[3], "softcap", &t.softcap))
+        return nullptr;
+    t.q = (const float*)q;
+    t.out = (float*)out;
+    if (check(env, c, brik_attention(c, &k, &b, &t))) return nullptr;
+    return undefined(env);
+}
+
 // ---- sampling pre-work -------------------------------------------------------------------------
 
 // logitsTopK(ctx, logits, recent, ids, vals, n, nRecent, k, penalty, softcap)
@@ -1031,6 +1206,11 @@ napi_value Init(napi_env env, napi_value exports)
         {"liveBuffers", nullptr, LiveBuffers, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
         {"readbackAsync", nullptr, ReadbackAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
         {"selfValidate", nullptr, SelfValidate, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
+        // reached through the facade's methods of the same names; not among the keys of the addon
+        {"qkNormRope", nullptr, QkNormRope, nullptr, nullptr, nullptr, napi_default, nullptr},
+        {"kvWrite", nullptr, KvWrite, nullptr, nullptr, nullptr, napi_default, nullptr},
+        {"kvRead", nullptr, KvRead, nullptr, nullptr, nullptr, napi_default, nullptr},
+        {"attention", nullptr, Attention, nullptr, nullptr, nullptr, napi_default, nullptr},
     };
     napi_define_properties(env, exports, sizeof(props) / sizeof(props[0]), props);
     return exports;

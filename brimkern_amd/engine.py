@@ -26,6 +26,9 @@ data,n,dtype)``            equal to the CPU ``encodeTensor``)
 wF16)``                    (MATMUL_T_F16W)                                      shaders.ts:2240-2259
 session ``conv2d`` with a  :meth:`Engine.conv2d` (q8 / q4 handle)              kernels.ts:1233-1256,
 q8 / q4 weight                                                                  1369-1374
+rope, quantize_kv and the  :meth:`Engine.kv_cache`, :meth:`Engine.qk_norm_rope`,   shaders.ts:1361, 1673
+attention over the         :meth:`Engine.kv_write`, :meth:`Engine.kv_read`,
+quantized cache            :meth:`Engine.attention` (device resident)
 .brik container            :mod:`brimkern_amd.container`,                        container.ts:30-87
                            :meth:`Engine.weight_from_container`
 =========================  ===================================================  ==================
@@ -41,7 +44,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import container, layout
-from .capi import BrikError, Context, DeviceBuffer, BRIK_EINVAL
+from .capi import BrikError, Context, DeviceBuffer, KvBatch, KvCache, BRIK_EINVAL
 
 
 class QWeight(dict):
@@ -256,6 +259,53 @@ class Engine:
         return out
 
     # ---- sampling pre-work ---------------------------------------------------------------
+    # ---- attention over a cache of quantized keys and values ---------------------------------
+    def kv_cache(self, dtype: str, heads: int, head_dim: int, page: int, pages: int) -> KvCache:
+        """A paged cache of its own memory: keys and values one packed .brik tensor [pages, heads, page, head_dim] each."""
+        if dtype not in ("q8", "q4"):
+            raise BrikError(BRIK_EINVAL, f"kv_cache: dtype {dtype!r} is not q8 or q4")
+        n = pages * heads * page * head_dim
+        if n <= 0 or n % 512:
+            raise BrikError(BRIK_EINVAL, "kv_cache: pages * heads * page * head_dim must be a multiple of 512")
+        offs = layout.plane_offsets(dtype, n)
+        bufs = [self.ctx.alloc(layout.byte_length(dtype, n)) for _ in range(2)]
+        planes = [[b.offset(offs[p][0]) for p in self._PLANES[dtype]] for b in bufs]
+        cache = self.ctx.kv_cache(dtype, heads, head_dim, page, pages, *planes)
+        cache.buffers = bufs
+        return cache
+
+    def free_kv_cache(self, cache: KvCache):
+        for b in cache.buffers:
+            self.ctx.free(b)
+        cache.buffers = []
+
+    def kv_batch(self, *args, **kw) -> KvBatch:
+        """The sequences of a step (:meth:`Context.kv_batch`)."""
+        return self.ctx.kv_batch(*args, **kw)
+
+    def qk_norm_rope(self, batch: KvBatch, **rows):
+        """Head norms and rotation of q and k; ``rows``: the arguments of :meth:`Context.qkv_rows`."""
+        self.ctx.qk_norm_rope(batch, self.ctx.qkv_rows(**rows))
+
+    def kv_write(self, cache: KvCache, batch: KvBatch, **rows):
+        """k and v into the cache, normed and rotated on the way (and q, into ``q_out``)."""
+        self.ctx.kv_write(cache, batch, self.ctx.qkv_rows(head_dim=cache.head_dim, kv_heads=cache.heads, **rows))
+
+    def kv_read(self, cache: KvCache, batch: KvBatch, k=None, v=None):
+        """The batch's tokens back as f32 rows in ``k`` and ``v``."""
+        self.ctx.kv_read(cache, batch, k, v)
+
+    def attention(self, cache: KvCache, batch: KvBatch, q, heads: int, out=None, scale: float | None = None, **args):
+        """Attention of the batch's rows; ``out`` (allocated when not given). ``scale``: 1 / sqrt(head_dim) by default."""
+        y = self.ctx.alloc(max(4 * batch.rows * (args.get("out_stride") or heads * cache.head_dim), 4)) if out is None else out
+        try:
+            self.ctx.attention(cache, batch, self.ctx.attn_args(q, y, heads, cache.head_dim ** -0.5 if scale is None else scale, **args))
+        except BrikError:
+            if out is None:
+                self.ctx.free(y)
+            raise
+        return y
+
     def _top_k(self, run, recent, k):
         ids = list(dict.fromkeys(int(i) for i in (recent or [])))      # each id once, as the callers pass them
         rb = self.ctx.upload(np.asarray(ids, np.int32)) if ids else None

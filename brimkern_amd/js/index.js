@@ -27,6 +27,8 @@
 //   (MATMUL_T_F16W, shaders.ts:2240)                 (w: f16 bits on the device); engine.mmF16(a, w, m, k, n[, out])
 //   session conv2d with a q8 / q4 weight :1369-1374  engine.conv2d(inp, w, bias, Cin, H, W, Cout, kh, kw, st, pd[, out])
 //   (recConv2dDirectQ8 / Q4)            :1233-1256  (device resident; inputs may be Float32Arrays)
+//   rope / quantize_kv and the attention    shaders.ts   engine.kvCache(dtype, ...), qkNormRope, kvWrite, kvRead,
+//   passes over the quantized cache     :1361, 1673  attention (device resident, pages and batches)
 //   .brik container (container.ts)                   require('./container'): parseBrik, serializeBrik, ...;
 //                                                    engine.weightFromContainer(parsed, name)
 //
@@ -66,6 +68,11 @@ function jobSpec(j) {
   if (j.eps !== undefined) s.eps = j.eps;
   s.flags = (j.onePlus ? 1 : 0) | (j.act === 'gelu' ? 2 : 0);
   return s;
+}
+
+// The native rows object: its flags from {onePlus, interleaved}.
+function qkvRows(r) {
+  return Object.assign({}, r, { flags: (r.onePlus ? 1 : 0) | (r.interleaved ? 2 : 0) });
 }
 
 function planHandle(nat, plan) {
@@ -397,6 +404,46 @@ class Engine {
     } finally {
       if (xb) xb.destroy();
     }
+  }
+
+  // ---- attention over a cache of quantized keys and values (include/brik.h: brik_kv_*, brik_attention) ----
+  // A paged cache: `pages` pages of `page` tokens, keys and values one packed .brik tensor each
+  // [pages, heads, page, headDim] (q8 or q4). The counterpart of the reference's quantized session cache
+  // (quantize_kv and its attention, shaders.ts:1673); destroy() frees it.
+  kvCache(dtype, heads, headDim, page, pages) {
+    if (dtype !== 'q8' && dtype !== 'q4') throw einval('kvCache: dtype must be q8 or q4');
+    const n = pages * heads * page * headDim;
+    if (!(Number.isInteger(n) && n > 0 && n % 512 === 0)) throw einval('kvCache: pages * heads * page * headDim must be a multiple of 512');
+    const offs = planes.planeOffsets(dtype, n), size = planes.byteLength(dtype, n);
+    const kb = this.alloc(size), vb = this.alloc(size);
+    const at = function (b, p) { return offs[p] ? b.view(offs[p][0]) : null; };
+    return { dtype: dtype, fmt: FMT[dtype], heads: heads, headDim: headDim, page: page, pages: pages, keys: kb, values: vb,
+      k: kb, v: vb, kScales: at(kb, 'sc'), vScales: at(vb, 'sc'), kMins: at(kb, 'mn'), vMins: at(vb, 'mn'),
+      destroy: function () { kb.destroy(); vb.destroy(); } };
+  }
+
+  // batch: {seqs, rows, kvLen, table, tableCols, maxLen[, rowOff, maxRows, prefixTable, prefixLen]}, kvLen, table, rowOff and
+  // prefixTable int32 device buffers. rows: {heads, kvHeads, headDim, q, k, v, qOut, kOut, qNorm, kNorm, eps, onePlus, invFreq,
+  // rotDim, positions, interleaved, qStride, ...}, what is not needed left out. Head norms and rotation of q and k:
+  qkNormRope(batch, rows) { this.native.qkNormRope(this.ctx, batch, qkvRows(rows)); }
+
+  // k and v into the cache, normed and rotated on the way (and q, into qOut).
+  kvWrite(cache, batch, rows) { this.native.kvWrite(this.ctx, cache, batch, qkvRows(rows)); }
+
+  // The batch's tokens back as f32 rows [rows, heads, headDim]; k or v may be null.
+  kvRead(cache, batch, k, v) { this.native.kvRead(this.ctx, cache, batch, k, v); }
+
+  // args: {q, heads[, out, scale = 1 / sqrt(headDim), window, softcap, qStride, outStride]}. Returns out (allocated when not given).
+  attention(cache, batch, args) {
+    const t = Object.assign({ scale: 1 / Math.sqrt(cache.headDim) }, args);
+    if (!t.out) t.out = this.alloc(Math.max(4 * batch.rows * (t.outStride || t.heads * cache.headDim), 4));
+    try {
+      this.native.attention(this.ctx, cache, batch, t);
+    } catch (e) {
+      if (!args.out) t.out.destroy();
+      throw e;
+    }
+    return t.out;
   }
 
   dequant(fmt, w, out, nElems) {
