@@ -54,13 +54,15 @@ inline int batch(Why& w, const char* who, const brik_kv_batch* b, bool tokens, b
     if (b->seqs < 0 || b->rows < 0 || b->table_cols < 0 || b->max_len < 0 || b->max_rows < 0 || b->prefix_len < 0)
         return no(w, BRIK_EINVAL, "%s: negative size in the batch", who);
     if (b->rows > (1 << 24) - 1) return no(w, BRIK_EINVAL, "%s: %d rows exceed 2^24 - 1 in one call", who, b->rows);
-    if (b->rows == 0 || (!tokens && !lens)) return BRIK_OK;
+    if (b->rows == 0) return BRIK_OK;
+    if (off(b->row_off, 4)) return no(w, BRIK_EALIGN, "%s: row_off must be 4-byte aligned", who);
+    if (!tokens && !lens) return BRIK_OK;
     if (b->seqs == 0) return no(w, BRIK_EINVAL, "%s: %d rows of no sequences", who, b->rows);
     if (!b->row_off && b->rows % b->seqs)
         return no(w, BRIK_EINVAL, "%s: %d rows do not divide over %d sequences and row_off is null", who, b->rows, b->seqs);
     if (!b->kv_len) return no(w, BRIK_EINVAL, "%s: kv_len is null", who);
-    if (off(b->row_off, 4) || off(b->kv_len, 4) || off(b->table, 4) || off(b->prefix_table, 4))
-        return no(w, BRIK_EALIGN, "%s: row_off, kv_len and the tables must be 4-byte aligned", who);
+    if (off(b->kv_len, 4) || off(b->table, 4) || off(b->prefix_table, 4))
+        return no(w, BRIK_EALIGN, "%s: kv_len and the tables must be 4-byte aligned", who);
     if (!tokens) return BRIK_OK;
     if (b->table_cols > 0 && !b->table) return no(w, BRIK_EINVAL, "%s: table is null", who);
     if (b->prefix_len > 0 && !b->prefix_table) return no(w, BRIK_EINVAL, "%s: prefix_table is null", who);

@@ -2470,8 +2470,8 @@ void brik_graph_destroy(brik_ctx* c, brik_graph* g)
 static int refuse(brik_ctx* c, int code, const brik_check::Why& w) { return fail(c, code, "%s", w.text); }
 
 // Blocks per row: one row's heads in one block where the rows alone fill the device several times over, else more, up to a
-// block per 256 / lanes heads (40 heads of one row 4.8 us, in one block 7.8; 48 of 64 rows 9.1 and 12.3; three prompts of up to 777 rows 12.5,
-// by twice as many blocks 13.8).
+// block per 256 / lanes heads (40 heads of one row 4.8 us, in one block 7.8; 48 of 64 rows 9.1 and 12.3; three prompts of up to
+// 777 rows 12.5, by twice as many blocks 13.8).
 static unsigned row_blocks(int rows, int units, int per_block)
 {
     const int most = (units + per_block - 1) / per_block, want = (int)((4 * kCUs + rows - 1) / rows);
@@ -2576,7 +2576,8 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     // that the call finds. (Splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for the longest. Up to
     // 1024 keys a block per sequence is as fast, and one that begins a second sequence pays 4 us for it.)
     const long blocks32 = (std::max(0l, own_keys) + 31) / 32;
-    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32 && !c->opt_attn_splits) {
+    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32 && a.s.seqs * blocks32 < (1l << 30) &&
+        !c->opt_attn_splits) {
         a.own_blocks = (int)std::max(1l, std::min<long>((2 * kCUs + KV - 1) / KV, a.s.seqs * ((blocks32 + 3) / 4)));
         tiles = a.own_blocks;
         a.own_splits = 1;

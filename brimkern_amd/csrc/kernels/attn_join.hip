@@ -17,6 +17,7 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
         if (b >= a.s.seqs) return;                                   // behind the last sequence
         const Seq q = Share::find(a, b, 0, start);
         const int G = a.a.heads / a.c.heads, kvh = h / G;
+        if ((t - q.row + 1) * G > 16) return;                        // more rows than the call was said to have
         const int first = start / share.each, count = q.n ? (start + q.n - 1) / share.each - first + 1 : 0;
         if (count == 1 && a.prefix_splits == 0) return;              // written by its block
         slots = a.prefix_splits + count;

@@ -156,6 +156,8 @@ __device__ __forceinline__ void rows_body(const brik_rows_launch& a)
         b = seq_of_row(a.s, t);
         if (b >= a.s.seqs) return;                       // behind the last sequence
         pos = row_position(a.s, b, t);
+    } else if (a.s.row_off && t >= a.s.row_off[a.s.seqs]) {
+        return;
     }
     if (FMT && pos >= a.s.prefix_len) page = brik_page_of(a.s, b, pos);
     if (turn) {

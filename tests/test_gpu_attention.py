@@ -601,3 +601,15 @@ def test_option_refusals(ctx):
             with pytest.raises(BrikError) as e:
                 ctx.set_option(option, value)
             assert e.value.code == BRIK_EINVAL
+
+
+@pytest.mark.parametrize("fmt,B", [("q8", 700), ("q4", 1030)])
+def test_many_sequences_behind_a_prefix(dev, fmt, B):
+    """So many rows share the prefix that it goes to tiles of 128 rows and more, the sequences' own keys to tiles of 16, in one
+    call: shared out where there are up to 1024 sequences and one is long."""
+    rng = np.random.default_rng(B)
+    own = [int(x) for x in rng.integers(1, 20, B)]
+    own[5], own[B - 1] = 1100, 40
+    c = Case(dev, fmt, 32, 8, 64, 16, [1] * B, [45 + n for n in own], prefix=45, seed=B)
+    c.check()
+    assert dev.ctx.last_kernel() == "attn_few"

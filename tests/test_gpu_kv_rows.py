@@ -302,3 +302,18 @@ def test_refusals(dev):
         refused(BRIK_EINVAL, ctx.kv_read, cache, wrong, out, out)
     refused(BRIK_EALIGN, ctx.kv_read, cache, batch, out.offset(4), None)
     refused(BRIK_EINVAL, ctx.qk_norm_rope, batch, ctx.qkv_rows(head_dim=64, heads=2, q=x))
+
+
+def test_rows_behind_the_last_sequence_with_positions_of_their_own(dev):
+    """A padded batch: with given positions, or without rotation, the lengths are not looked at, and still those rows stay."""
+    rng = np.random.default_rng(8)
+    H, D, T = 2, 64, 9
+    q, w, pos = rows_of(rng, T, H, D), rng.standard_normal(D).astype(f32), np.arange(T, dtype=np.int32) * 3
+    for rot in (D, 0):
+        out = dev.room(T, H, D)
+        rows = dev.ctx.qkv_rows(head_dim=D, heads=H, q=dev.up(q), q_out=out, q_norm=dev.up(w), inv_freq=dev.up(freqs(D)) if rot else None,
+                                rot_dim=rot, positions=dev.i32(pos) if rot else None)
+        dev.ctx.qk_norm_rope(dev.ctx.kv_batch(seqs=2, rows=T, row_off=dev.i32(np.array([0, 4, 6]))), rows)
+        got = dev.down(out, T, H, D)
+        near(got[:6], R.norm_rope(q[:6], w, 1e-6, False, pos[:6], freqs(D) if rot else None, False))
+        assert np.isnan(got[6:]).all()
