@@ -26,10 +26,12 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
         return;
     }
     auto vec = [&](int s) { return a.own_blocks && s >= a.prefix_splits ? own + (size_t)(s - a.prefix_splits) * 16 : s * all + row; };
-    // every wave: the reference exponent, then the weights (they stay in the cache: read twice rather than kept)
-    float M = ATTN_NONE;
+    // every wave: the reference exponent, then the weights (64 slots in a register, more are read twice)
+    f32x2_t ml0 = {ATTN_NONE, 0.f};
+    if (lane < slots) ml0 = *(const f32x2_t*)(a.ml + 2 * vec(lane));
+    float M = ml0.x;
 #pragma unroll 1
-    for (int s = lane; s < slots; s += 64) M = fmaxf(M, a.ml[2 * vec(s)]);
+    for (int s = lane + 64; s < slots; s += 64) M = fmaxf(M, a.ml[2 * vec(s)]);
     M = half_max(M);
     float p, q;
     half_pair(M, p, q);
@@ -41,16 +43,25 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
     for (int s0 = 0; s0 < slots; s0 += 64) {                         // 64 slots at a time, one a lane
         float l = 0.f, f = 0.f;
         if (s0 + lane < slots) {
-            const f32x2_t ml = *(const f32x2_t*)(a.ml + 2 * vec(s0 + lane));
+            const f32x2_t ml = s0 ? *(const f32x2_t*)(a.ml + 2 * vec(s0 + lane)) : ml0;
             l = ml.y;
             f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
         }
         L += quarters_sum(sum16(l * f));
         const int n = min(64, slots - s0);
-        for (int s1 = 0; s1 < n; s1 += groups) {                     // as often in every lane: weights come from other lanes
-            const int s = s1 + g;
-            const float w = __shfl(f, min(s, 63));
-            if (g < groups && s < n && w != 0.f) v += *(const f32x4_t*)(a.part + vec(s0 + s) * D + d) * w;
+#pragma unroll 1
+        // four loads at once, whatever their weights (decoding one sequence 13.8 -> 12.7 and 65.7 -> 63.5 us; a slot that was not written has
+        // weight 0 and is not added); as often in every lane: weights come from other lanes
+        for (int s1 = 0; s1 < n; s1 += 4 * groups) {
+            f32x4_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = *(const f32x4_t*)(a.part + vec(s0 + min(s1 + i * groups + g, n - 1)) * D + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = s1 + i * groups + g;
+                const float w = __shfl(f, min(s, 63));
+                if (g < groups && s < n && w != 0.f) v += x[i] * w;
+            }
         }
     }
     sums[tid] = v;
