@@ -2537,12 +2537,14 @@ int brik_kv_read(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* b
                      256, 0, args);
 }
 
-// Splits of a section's keys (at most `keys` of them): enough blocks to fill the device, each with at least four blocks
-// of 32 keys, one per wave.
+// Splits of a section's keys (at most `keys` of them): as many as the device takes at once, each of at least four blocks of
+// 32 keys, one per wave. (108 rows over a prefix of 2001 keys by 56 tiles: 8 splits 18.2 us; 10, a few blocks in a second
+// round, 23.9. One sequence of 4095 keys over 8 heads: 32 splits 12.6, 16 splits 14.4, 8 splits 17.9; of 131072: 64 splits 63,
+// 32 and 128 both 70.)
 static int attn_splits(const brik_ctx* c, long blocks, long keys)
 {
     if (c->opt_attn_splits) return c->opt_attn_splits;
-    const long most = std::max(1l, (keys + 127) / 128), want = (2 * kCUs + blocks - 1) / std::max(1l, blocks);
+    const long most = std::max(1l, (keys + 127) / 128), want = 2 * kCUs / std::max(1l, blocks);
     return (int)std::min({most, std::max(1l, want), 64l});
 }
 
@@ -2578,7 +2580,7 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     const long blocks32 = (std::max(0l, own_keys) + 31) / 32;
     if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32 && a.s.seqs * blocks32 < (1l << 30) &&
         !c->opt_attn_splits) {
-        a.own_blocks = (int)std::max(1l, std::min<long>((2 * kCUs + KV - 1) / KV, a.s.seqs * ((blocks32 + 3) / 4)));
+        a.own_blocks = (int)std::max(1l, std::min<long>(2 * kCUs / KV, a.s.seqs * ((blocks32 + 3) / 4)));
         tiles = a.own_blocks;
         a.own_splits = 1;
     } else {

@@ -345,14 +345,14 @@ __device__ __forceinline__ size_t part_at(const brik_attn_launch& a, const Work&
 }
 
 // The key blocks [t0, t1) of 32 keys that this split works on: those of the keys [lo, hi) that any row sees, divided over
-// the splits in pieces of at least `least`.
+// the splits in whole multiples of `least`.
 __device__ __forceinline__ void find_keys(const Work& w, int lo, int hi, int least, int& t0, int& t1)
 {
     t0 = w.t0;
     t1 = w.t1;
     if (t1 || lo >= hi) return;
     const int first = lo >> 5, n = ((hi + 31) >> 5) - first;
-    const int each = max(least, (n + w.splits - 1) / w.splits);
+    const int each = (n + least * w.splits - 1) / (least * w.splits) * least;
     t0 = first + min(n, w.split * each);
     t1 = first + min(n, (w.split + 1) * each);
 }
