@@ -57,7 +57,7 @@ const char* const kKernelNames[K_COUNT] = {
 // Kernels of the attention side's code object. Teams of 8, 16, 32, 64 lanes: brik_rows_<rope, q8, q4>_<lanes>.
 // Attention by tiles of 16 rows, brik_attn_few_<fmt>_<head_dim>, and of 128 and 256, brik_attn_tile<waves>_<fmt>_<head_dim>
 // (256: up to head_dim 128).
-enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE4 = A_FEW + 10, A_TILE8 = A_TILE4 + 10, A_JOIN = A_TILE8 + 10, A_COUNT };
+enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE4 = A_FEW + 10, A_TILE8 = A_TILE4 + 10, A_JOIN = A_TILE8 + 10, A_JOIN_FEW, A_COUNT };
 constexpr int kAttnDims[5] = {64, 96, 128, 192, 256};
 
 // GEMV variants {team, r, u, d}, in the order of BRIK_GEMV_FMT in gemv.hip: TEAM lanes per row team,
@@ -1448,7 +1448,7 @@ int brik_create(int device, brik_ctx** out)
         else if (k < A_FEW) snprintf(name, sizeof name, "brik_kv_read_%s", kFmtNames[k - A_READ]);
         else if (k < A_JOIN) snprintf(name, sizeof name, "brik_attn_%s_%s_%d", k < A_TILE4 ? "few" : k < A_TILE8 ? "tile4" : "tile8",
                                     kFmtNames[(k - A_FEW) % 10 / 5], kAttnDims[(k - A_FEW) % 5]);
-        else snprintf(name, sizeof name, "brik_attn_join");
+        else snprintf(name, sizeof name, k == A_JOIN ? "brik_attn_join" : "brik_attn_join_few");
         if (k >= A_TILE8 && k < A_JOIN && kAttnDims[(k - A_FEW) % 5] > 128) continue;
         if (hipModuleGetFunction(&c->attn_fn[k], c->attn_module, name) != hipSuccess) return bail(BRIK_EMODULE);
     }
@@ -2537,15 +2537,65 @@ int brik_kv_read(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch* b
                      256, 0, args);
 }
 
-// Splits of a section's keys (at most `keys` of them): as many as the device takes at once, each of at least four blocks of
-// 32 keys, one per wave. (108 rows over a prefix of 2001 keys by 56 tiles: 8 splits 18.2 us; 10, a few blocks in a second
-// round, 23.9. One sequence of 4095 keys over 8 heads: 32 splits 12.6, 16 splits 14.4, 8 splits 17.9; of 131072: 64 splits 63,
-// 32 and 128 both 70.)
-static int attn_splits(const brik_ctx* c, long blocks, long keys)
+// Row tiles and splits of a section of keys (the own ones, or the prefix's): those with the least time by a model of the kernels,
+// fitted to measured times (us). A block takes `start`, then steps of `alone` where the device is not full and of `full` where its
+// `slots` are; a step of 16-row tiles is 128 keys (32 a wave), of the others 32 keys. Partial results are written and read
+// again at 4.5 TB/s and joined by a launch of 5. What it weighs, 32 heads over 8 of 128, q8, by 16, 128 and 256 rows unsplit:
+// a prompt of 1024 rows 68, 89, 93; of 2048 190, 170, 175 (256 in 2 splits 137); of 4096 639, 439, 384; eight prompts of 256
+// 80, 41, 37 (65 and more in 2 splits); 512 rows behind 8192 292, 617, 644 (256 in 4 splits 200). One row of 4095: 32 splits
+// 12.3, 16 splits 14.4, 8 splits 17.9; of 131072: 64 splits 63, 32 or 128 70.
+struct AttnPlan {
+    int rows = 16, splits = 1;
+    double us = 1e30;
+};
+struct AttnSection {
+    long KV, G, D, rows, seqs, most;      // most: rows of a sequence
+    long keys, window;
+    bool prefix, ragged;
+    long tiles(int bm) const
+    {
+        const long bound = (rows * G + bm - 1) / bm;
+        if (prefix) return bound;
+        const long each = (most * G + bm - 1) / bm * seqs;
+        return ragged ? std::min(each, bound + seqs) : each;
+    }
+};
+static AttnPlan attn_plan(const brik_ctx* c, const AttnSection& x, bool joined, int beside)
 {
-    if (c->opt_attn_splits) return c->opt_attn_splits;
-    const long most = std::max(1l, (keys + 127) / 128), want = 2 * kCUs / std::max(1l, blocks);
-    return (int)std::min({most, std::max(1l, want), 64l});
+    static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64};
+    AttnPlan best;
+    for (int bm : {16, 128, 256}) {
+        if (c->opt_attn_rows ? bm != (x.D > 128 && c->opt_attn_rows > 16 ? 128 : c->opt_attn_rows)
+                             : bm > 16 && (x.most * x.G <= 16 || (bm == 256 && x.D > 128)))
+            continue;
+        const double D = (double)x.D, slots = kCUs * (bm == 16 ? x.D <= 64 ? 3 : x.D <= 128 ? 2 : 1 : bm == 128 && x.D <= 128 ? 2 : 1);
+        const double start = bm == 16 ? 3.8 : 4, alone = bm == 16 ? 0.65 + 0.0086 * D : bm == 128 ? 0.6 + 0.0145 * D : 0.9 + 0.0133 * D;
+        const double full = bm == 16 ? 3.3e-5 * D * slots : bm == 256 ? 0.9 + 0.0155 * D : x.D <= 128 ? 1 + 0.018 * D : alone;
+        // keys of the tile that sees the most, and of the middle one
+        const long far = x.window ? std::min(x.keys, x.window + bm / x.G + 32) : x.keys;
+        const long mid = x.prefix ? far : std::min(far, std::max(1l, x.keys - x.most / 2 + bm / x.G));
+        const double blocks = (double)x.KV * x.tiles(bm), vectors = (double)x.rows * x.KV * x.G;
+        const long most = std::max(1l, std::min(64l, (far + 127) / 128));
+        double last = 0;
+        for (int q : kSplits) {
+            if (c->opt_attn_splits) q = c->opt_attn_splits;
+            else if (q > most) break;
+            // steps of the longest split (four of a tile's, or one of a 16-row tile's, at a time) and of the middle tile's
+            const double unit = bm == 16 ? 1 : 4, f = unit * ((far + 128 * q - 1) / (128 * q));
+            const double m = mid == far ? f : std::min(f, unit * mid / (128 * q) + 0.5);
+            if (f == last && !c->opt_attn_splits) continue;      // more splits, none of them shorter
+            last = f;
+            // rounds that blocks of one length do not fill last as long as full ones (half that with several blocks on a CU);
+            // where lengths differ the long ones go first, and short ones fill the gaps
+            const double rounds = blocks * q / slots, even = std::max(0.0, 2.0 * mid / std::max(1l, far) - 1) * (bm == 256 ? 1 : 0.5);
+            double us = std::max(start + f * alone, std::max(1.0, rounds + (std::ceil(rounds) - rounds) * even) * (start + m * full));
+            if (q > 1 || joined) us += (joined ? 0 : 5) + vectors * (2 * q + 1) * 4 * D / 4.5e6;
+            if (beside && beside != bm) us += 10;            // another kernel's launch
+            if (us < best.us) best = AttnPlan{bm, q, us};
+            if (c->opt_attn_splits) break;
+        }
+    }
+    return best;
 }
 
 static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
@@ -2557,15 +2607,9 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     int dim = 0;
     while (kAttnDims[dim] != a.c.head_dim) ++dim;
     const int which = 5 * (a.c.fmt == BRIK_FMT_Q4) + dim;
-    // Row tiles of 256 or 128 where they fill the device without splitting keys, else of 16 (a 32-key step of a tile takes 3 us
-    // however few blocks there are: 805 rows of 7 heads behind a window of 1024 keys 71 us by 256, 31 us by 16 rows).
-    auto tile_rows = [&](long most_rows, long all_rows) {
-        if (c->opt_attn_rows) return a.c.head_dim > 128 ? std::min(c->opt_attn_rows, 128) : c->opt_attn_rows;
-        const long fill = KV * ((all_rows * G + 255) / 256);
-        if (most_rows * G <= 16 || fill < kCUs / 2) return 16;
-        return a.c.head_dim > 128 || most_rows * G <= 128 ? 128 : 256;
-    };
-    const int own_bm = tile_rows(most, rows), prefix_bm = tile_rows(rows, rows);
+    AttnSection own{KV, G, a.c.head_dim, rows, a.s.seqs, most, std::max(0l, own_keys), a.a.window, false, a.s.row_off != nullptr};
+    const AttnPlan own_plan = attn_plan(c, own, prefix_keys > 0, 0);
+    const int own_bm = own_plan.rows;
     // row tiles of the sequences: the same number for each where that is not many more than there can be
     const long per_seq = (most * G + own_bm - 1) / own_bm, bound = (rows * G + own_bm - 1) / own_bm + a.s.seqs;
     long tiles = per_seq * a.s.seqs;
@@ -2584,11 +2628,18 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         tiles = a.own_blocks;
         a.own_splits = 1;
     } else {
-        a.own_splits = attn_splits(c, KV * tiles, own_keys);
+        a.own_splits = own_plan.splits;
     }
+    int prefix_bm = own_bm;
     if (prefix_keys > 0) {
+        AttnSection pre = own;
+        pre.prefix = true;
+        pre.most = rows;
+        pre.keys = prefix_keys;
+        const AttnPlan plan = attn_plan(c, pre, true, own_bm);
+        prefix_bm = plan.rows;
         a.prefix_tiles = (int)((rows * G + prefix_bm - 1) / prefix_bm);
-        a.prefix_splits = attn_splits(c, KV * a.prefix_tiles, prefix_keys);
+        a.prefix_splits = plan.splits;
     }
     a.whole = a.prefix_splits == 0 && a.own_splits == 1 && a.own_blocks == 0;
     if (!a.whole) {
@@ -2616,6 +2667,13 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
     }
     if (a.whole) return BRIK_OK;
     void* args[] = {&a};
+    // few slots, or rows and heads for every CU: each group of lanes joins a row and head by itself; else a block shares the slots
+    // out (32 heads of one row: 16 slots 15.0 us the one way, 12.9 the other, 4 slots 12.5 and 12.8; 1024 rows by 2 slots 68 and 102)
+    const int slots = a.prefix_splits + a.own_splits;
+    if (!a.own_blocks && (slots <= 4 || (slots <= 16 && rows * a.a.heads >= 2 * kCUs))) {
+        const int each = 256 / (a.c.head_dim / 4);
+        return launch_fn(c, c->attn_fn[A_JOIN_FEW], (unsigned)rows, (unsigned)((a.a.heads + each - 1) / each), 256, 0, args);
+    }
     return launch_fn(c, c->attn_fn[A_JOIN], (unsigned)rows, (unsigned)a.a.heads, 256, 0, args);
 }
 

@@ -72,3 +72,37 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
     for (int k = 1; k < groups; ++k) v += sums[k * quads + tid];
     *(f32x4_t*)(a.a.out + t * a.a.out_stride + (size_t)h * D + d) = L == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : v / L;
 }
+
+// The same for up to 16 static slots: a group of D / 4 lanes per row and head, which loops over the slots by itself. (2048 rows
+// of 32 heads by 2 slots, 170 MB: with the kernels before it 138 us, 200 by a block for each.)
+extern "C" __global__ __launch_bounds__(256) void brik_attn_join_few(brik_attn_launch a)
+{
+    const int D = a.c.head_dim, quads = D / 4, g = threadIdx.x / quads, d = 4 * (threadIdx.x - g * quads);
+    const int t = blockIdx.x, h = blockIdx.y * (256 / quads) + g, slots = a.prefix_splits + a.own_splits;
+    if (g >= 256 / quads || h >= a.a.heads || (a.s.row_off && t >= a.s.row_off[a.s.seqs])) return;
+    const size_t all = (size_t)a.s.rows * a.a.heads, row = (size_t)t * a.a.heads + h;
+    float M = ATTN_NONE;
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) M = fmaxf(M, a.ml[2 * (s * all + row)]);
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+#pragma unroll 1
+    for (int s0 = 0; s0 < slots; s0 += 4) {
+        f32x4_t x[4];
+        f32x2_t ml[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const size_t at = min(s0 + i, slots - 1) * all + row;
+            x[i] = *(const f32x4_t*)(a.part + at * D + d);
+            ml[i] = *(const f32x2_t*)(a.ml + 2 * at);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i >= slots || ml[i].y == 0.f) continue;        // nothing was written there
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - M);
+            L += ml[i].y * f;
+            v += x[i] * f;
+        }
+    }
+    *(f32x4_t*)(a.a.out + t * a.a.out_stride + (size_t)h * D + d) = L == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : v / L;
+}
