@@ -2618,13 +2618,15 @@ static int attention(brik_ctx* c, brik_attn_launch& a, int max_rows)
         a.tiles_per_seq = 0;
         tiles = bound;
     }
-    // One tile a sequence and several sequences: their keys in a row, shared out evenly over two blocks per CU, by the lengths
-    // that the call finds. (Splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for the longest. Up to
-    // 1024 keys a block per sequence is as fast, and one that begins a second sequence pays 4 us for it.)
-    const long blocks32 = (std::max(0l, own_keys) + 31) / 32;
-    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32 && a.s.seqs * blocks32 < (1l << 30) &&
-        !c->opt_attn_splits) {
-        a.own_blocks = (int)std::max(1l, std::min<long>(2 * kCUs / KV, a.s.seqs * ((blocks32 + 3) / 4)));
+    // One tile a sequence and several sequences: their keys in a row, shared out evenly over the blocks that the device takes at
+    // once, by the lengths that the call finds. (Splits of the longest length left 32 sequences of 1 to 8192 tokens waiting for
+    // the longest.) Only where a block gets 16 blocks of keys and a sequence has over 1024: one that begins a second sequence
+    // pays 4 us for it (17 sequences behind a window of 635 tokens, one head of 128: 20 us shared out, 13 by splits).
+    const long far = a.a.window ? std::min(own_keys, a.a.window + most) : own_keys, blocks32 = (std::max(0l, far) + 31) / 32;
+    const long share = std::max(1l, (a.c.head_dim <= 128 ? 2 : 1) * kCUs / KV);
+    if (own_bm == 16 && per_seq == 1 && a.s.seqs > 1 && a.s.seqs <= 1024 && blocks32 > 32 && a.s.seqs * blocks32 >= 16 * share &&
+        a.s.seqs * blocks32 < (1l << 30) && !c->opt_attn_splits) {
+        a.own_blocks = (int)share;
         tiles = a.own_blocks;
         a.own_splits = 1;
     } else {

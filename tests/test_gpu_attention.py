@@ -613,3 +613,26 @@ def test_many_sequences_behind_a_prefix(dev, fmt, B):
     c = Case(dev, fmt, 32, 8, 64, 16, [1] * B, [45 + n for n in own], prefix=45, seed=B)
     c.check()
     assert dev.ctx.last_kernel() == "attn_few"
+
+
+@pytest.mark.parametrize("fmt,D,window", [("q8", 64, 1100), ("q4", 256, 0), ("q4", 128, 1030)])
+def test_shared_out_keys_behind_a_window(dev, fmt, D, window):
+    rng = np.random.default_rng(D)
+    lens = [int(x) for x in rng.integers(1, 2500, 40)]
+    lens[0], lens[7], lens[39] = 2500, 1, 0
+    rows = [1] * 40
+    rows[39] = 0
+    Case(dev, fmt, 8, 8, D, 16, rows, lens, seed=D, window=window, behind=2).check()
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+@pytest.mark.parametrize("H,KV,D,rows,lens", [(8, 2, 128, [300], [1500]), (6, 2, 64, [256] * 4, [256] * 4), (4, 1, 96, [130, 1, 64], [900, 700, 64]),
+                                              (2, 2, 256, [200], [2000]), (16, 1, 192, [40, 50], [600, 1000])])
+def test_prompts_by_the_choice_of_the_call(dev, fmt, H, KV, D, rows, lens):
+    """Rows and splits as the sizes choose them, eager and again in other batches on the same workspace."""
+    a = Case(dev, fmt, H, KV, D, 32, rows, lens, seed=1)
+    a.check()
+    b = Case(dev, fmt, H, KV, D, 32, [1] * len(rows), lens, seed=2)
+    b.check()
+    a = Case(dev, fmt, H, KV, D, 32, rows, lens, seed=1)
+    a.check()
