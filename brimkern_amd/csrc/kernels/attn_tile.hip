@@ -16,7 +16,7 @@
 // rows that see a token with an infinite or NaN scale (its values are 0 in LDS, so that other rows are not touched).
 //
 // Bound by the five products of halves that two f32 products take, and the conversion and softmax between them (4096 rows of
-// 32 heads over 8 of 128, q8: 377 to 390 us, 0.36 PFLOP/s of the formula, 0.9 of products; without the output's products 122
+// 32 heads over 8 of 128, q8: 377 to 393 us, 0.36 PFLOP/s of the formula, 0.9 of products; without the output's products 122
 // less, the scores' 83, the conversion 31). 256 rows a block against 128: 423 and 451 us at that stage. Waves 4 to 7
 // converting after the products instead of before, to run beside the others' products: 408 against 389.
 #include "attn_common.h"
