@@ -63,6 +63,12 @@ BRIK_HD void brik_rows_of(const brik_step& s, int b, int32_t& first, int32_t& co
     count = end > first ? end - first : 0;
 }
 
+// Rows before the first sequence's and behind the last one's belong to none.
+BRIK_HD bool brik_row_taken(const brik_step& s, int32_t t)
+{
+    return !s.row_off || (t >= s.row_off[0] && t < s.row_off[s.seqs]);
+}
+
 // Index of the vector (token's head) in a cache plane: planes are [pages, heads, page, head_dim].
 BRIK_HD size_t brik_vector(const brik_step& s, int heads, int32_t page, int head, int32_t slot)
 {

@@ -95,18 +95,20 @@ __device__ __forceinline__ int wave_sum(int v)
     return uniform((int)(h[0] + h[1]));
 }
 
-// The sequence of row t: how many of row_off[1..seqs] are at most t. One load round trip per 64 sequences.
+// The sequence of row t: how many of row_off[1..seqs] are at most t, or seqs where the row belongs to none (behind the last
+// sequence, or before row_off[0]). One load round trip per 64 sequences.
 __device__ __forceinline__ int seq_of_row(const brik_step& s, int t)
 {
     if (!s.row_off) return t / s.per_seq;
     const int lane = threadIdx.x & 63;
+    const int32_t first = s.row_off[0];
     int count = 0;
     for (int base = 0; base < s.seqs; base += 64) {
         const int i = base + lane;
         const int32_t end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
         count += __popcll(__ballot(end <= t));
     }
-    return count;
+    return t < first ? s.seqs : count;
 }
 
 // The same for a row per lane, whose rows are t0 + (0 .. count - 1) over the wave: every candidate row is compared with 64 ends
@@ -115,6 +117,7 @@ __device__ __forceinline__ int seq_of_lane(const brik_step& s, int t, int t0, in
 {
     if (!s.row_off) return t / s.per_seq;
     const int lane = threadIdx.x & 63;
+    const int32_t first = s.row_off[0];
     int mine = 0;
     for (int base = 0; base < s.seqs; base += 64) {
         const int i = base + lane;
@@ -124,7 +127,7 @@ __device__ __forceinline__ int seq_of_lane(const brik_step& s, int t, int t0, in
             if (t == t0 + k) mine += c;
         }
     }
-    return mine;
+    return t < first ? s.seqs : mine;
 }
 
 // The position of row t of sequence b.

@@ -453,7 +453,7 @@ __device__ __forceinline__ void few_part(const brik_attn_launch& a, const Work& 
         const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
         const int rel = (w.r0 + r) / G;
         if (rel >= w.count) continue;
-        if (w.prefix && a.s.row_off && w.first + rel >= a.s.row_off[a.s.seqs]) continue;
+        if (w.prefix && !brik_row_taken(a.s, w.first + rel)) continue;
         const int tok = w.first + rel, h = w.head * G + w.r0 + r - rel * G;
         float Mr = joinm[0][r], L = 0.f;
 #pragma unroll

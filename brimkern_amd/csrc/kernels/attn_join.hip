@@ -16,15 +16,15 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
     if (a.own_blocks) {
         const Share share(a);                                        // first: its loads and the search's go together
         int b = uniform(seq_of_row(a.s, t)), start;
-        if (b >= a.s.seqs) return;                                   // behind the last sequence
+        if (b >= a.s.seqs) return;                                   // of no sequence
         const Seq q = Share::find(a, b, 0, start);
         const int G = a.a.heads / a.c.heads, kvh = h / G;
-        if ((t - q.row + 1) * G > 16) return;                        // more rows than the call was said to have
+        if (t < q.row || (t - q.row + 1) * G > 16) return;           // more rows than the call was said to have
         const int first = start / share.each, count = q.n ? (start + q.n - 1) / share.each - first + 1 : 0;
         if (count == 1 && a.prefix_splits == 0) return;              // written by its block
         slots = a.prefix_splits + count;
         own = a.prefix_splits * all + ((size_t)kvh * (a.own_blocks + a.s.seqs) + first + b) * 16 + (t - q.row) * G + (h - kvh * G);
-    } else if (a.s.row_off && t >= a.s.row_off[a.s.seqs]) {
+    } else if (!brik_row_taken(a.s, t)) {
         return;
     }
     auto vec = [&](int s) { return a.own_blocks && s >= a.prefix_splits ? own + (size_t)(s - a.prefix_splits) * 16 : s * all + row; };
@@ -79,7 +79,7 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join_few(brik_attn_l
 {
     const int D = a.c.head_dim, quads = D / 4, g = threadIdx.x / quads, d = 4 * (threadIdx.x - g * quads);
     const int t = blockIdx.x, h = blockIdx.y * (256 / quads) + g, slots = a.prefix_splits + a.own_splits;
-    if (g >= 256 / quads || h >= a.a.heads || (a.s.row_off && t >= a.s.row_off[a.s.seqs])) return;
+    if (g >= 256 / quads || h >= a.a.heads || !brik_row_taken(a.s, t)) return;
     const size_t all = (size_t)a.s.rows * a.a.heads, row = (size_t)t * a.a.heads + h;
     float M = ATTN_NONE;
 #pragma unroll 4

@@ -155,9 +155,9 @@ __device__ __forceinline__ void rows_body(const brik_rows_launch& a)
     int32_t pos = 0, page = -1;
     if (FMT || (turn && !r.positions)) {
         b = seq_of_row(a.s, t);
-        if (b >= a.s.seqs) return;                       // behind the last sequence
+        if (b >= a.s.seqs) return;                       // of no sequence
         pos = row_position(a.s, b, t);
-    } else if (a.s.row_off && t >= a.s.row_off[a.s.seqs]) {
+    } else if (!brik_row_taken(a.s, t)) {
         return;
     }
     if (FMT && pos >= a.s.prefix_len) page = brik_page_of(a.s, b, pos);

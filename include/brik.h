@@ -374,8 +374,9 @@ typedef struct brik_kv_cache {
  * row_off, kv_len, table, prefix_table: DEVICE arrays, read when the call runs (a recorded call reads what they hold
  * at the replay). max_len and max_rows bound kv_len and the rows of a sequence and size the launch. Tokens at or past
  * max_len, tokens past the table and tokens on a page outside [0, pages) do not exist: they are not written, read as
- * zeros and not attended to. A row past row_off[seqs] is left as it is, what a row past
- * max_rows of its sequence holds is not said; row_off must not decrease. */
+ * zeros and not attended to. row_off must not decrease; it may begin above 0 and end below `rows` (a part of a larger
+ * batch): the rows before row_off[0] and from row_off[seqs] on belong to no sequence, nothing is done for them and what
+ * their outputs hold stays. What a row past max_rows of its sequence holds is not said. */
 typedef struct brik_kv_batch {
     int32_t seqs, rows;
     const int32_t *row_off;      /* [seqs + 1], or NULL */
