@@ -279,8 +279,10 @@ __device__ __forceinline__ bool find_work(const brik_attn_launch& a, Work& w)
     }
     brik_rows_of(a.s, w.b, w.first, w.count);
     w.pos = row_position(a.s, w.b, w.first);
-    // the last tiles see the most keys: they come first
-    const int tiles = (int)(((long long)w.count * G + BM - 1) / BM);
+    // the last tiles see the most keys: they come first. Of a sequence with more rows than the call was said to have, the first
+    // ones are done.
+    int tiles = (int)(((long long)w.count * G + BM - 1) / BM);
+    if (a.tiles_per_seq) tiles = min(tiles, a.tiles_per_seq);
     if (j >= tiles) return false;
     w.r0 = (tiles - 1 - j) * BM;
     return true;
