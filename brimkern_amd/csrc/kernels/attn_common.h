@@ -176,6 +176,13 @@ struct Work {
     bool whole;                // nothing to join: the block writes the output
 };
 
+// The first key that the window of a row at `pos` shows, counted from token `first` on. (In 64 bits: a window of 2^31 - 1 and a
+// position before `first` leave 32.)
+__device__ __forceinline__ int first_seen(const brik_attn_launch& a, int32_t pos, int32_t first)
+{
+    return a.a.window ? (int)max(0ll, (long long)pos - a.a.window + 1 - first) : 0;
+}
+
 // A sequence's rows, and the blocks of 32 of its own keys that they see (first, count).
 struct Seq {
     int32_t row, rows, pos;      // first row, how many, the first row's position
@@ -189,7 +196,7 @@ __device__ __forceinline__ Seq find_seq(const brik_attn_launch& a, int b)
     q.pos = a.s.kv_len[b] - end_row + q.row;
     const int32_t before = a.s.prefix_len;
     const int32_t end = (int32_t)min((long long)a.s.max_len - before, min((long long)a.s.table_cols << a.s.shift, 0x7fffffc0ll));
-    const int hi = min(q.pos + q.rows - before, end), lo = a.a.window ? max(0, q.pos - a.a.window + 1 - before) : 0;
+    const int hi = min(q.pos + q.rows - before, end), lo = first_seen(a, q.pos, before);
     q.first = lo >> 5;
     q.n = q.rows > 0 && lo < hi ? ((hi + 31) >> 5) - q.first : 0;
     return q;
@@ -337,7 +344,7 @@ __device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w
     const int32_t end = w.prefix ? min(a.s.prefix_len, a.s.max_len)
                                  : (int32_t)min((long long)a.s.max_len - first, min((long long)a.s.table_cols << a.s.shift, 0x7fffffc0ll));
     r.hi = max(0, min(pos + 1 - first, end));
-    r.lo = a.a.window ? max(0, pos - a.a.window + 1 - first) : 0;
+    r.lo = first_seen(a, pos, first);
     return r;
 }
 
