@@ -43,17 +43,17 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
     float L = 0.f;
 #pragma unroll 1
     for (int s0 = 0; s0 < slots; s0 += 64) {                         // 64 slots at a time, one a lane
-        float l = 0.f, f = 0.f;
+        float l = 0.f, f = -1.f;
         if (s0 + lane < slots) {
             const f32x2_t ml = s0 ? *(const f32x2_t*)(a.ml + 2 * vec(s0 + lane)) : ml0;
             l = ml.y;
-            f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+            f = l == 0.f ? -1.f : __builtin_amdgcn_exp2f(ml.x - M);  // -1: nothing was written there
         }
         L += quarters_sum(sum16(l * f));
         const int n = min(64, slots - s0);
 #pragma unroll 1
-        // four loads at once, whatever their weights (decoding one sequence 13.8 -> 12.7 and 65.7 -> 63.5 us; a slot that was not written has
-        // weight 0 and is not added); as often in every lane: weights come from other lanes
+        // four loads at once, whatever their weights (decoding one sequence 13.8 -> 12.7 and 65.7 -> 63.5 us; a slot that was not written
+        // is not added, one whose weight is 0 is: it may hold NaN); as often in every lane: weights come from other lanes
         for (int s1 = 0; s1 < n; s1 += 4 * groups) {
             f32x4_t x[4];
 #pragma unroll
@@ -62,7 +62,7 @@ extern "C" __global__ __launch_bounds__(256) void brik_attn_join(brik_attn_launc
             for (int i = 0; i < 4; ++i) {
                 const int s = s1 + i * groups + g;
                 const float w = __shfl(f, min(s, 63));
-                if (g < groups && s < n && w != 0.f) v += x[i] * w;
+                if (g < groups && s < n && !(w < 0.f)) v += x[i] * w;
             }
         }
     }
