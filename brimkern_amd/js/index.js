@@ -435,7 +435,8 @@ class Engine {
 
   // args: {q, heads[, out, scale = 1 / sqrt(headDim), window, softcap, qStride, outStride]}. Returns out (allocated when not given).
   attention(cache, batch, args) {
-    const t = Object.assign({ scale: 1 / Math.sqrt(cache.headDim) }, args);
+    const t = Object.assign({}, args);
+    if (t.scale === undefined || t.scale === null) t.scale = 1 / Math.sqrt(cache.headDim);
     if (!t.out) t.out = this.alloc(Math.max(4 * batch.rows * (t.outStride || t.heads * cache.headDim), 4));
     try {
       this.native.attention(this.ctx, cache, batch, t);
