@@ -268,7 +268,12 @@ class Engine:
         if n <= 0 or n % 512:
             raise BrikError(BRIK_EINVAL, "kv_cache: pages * heads * page * head_dim must be a multiple of 512")
         offs = layout.plane_offsets(dtype, n)
-        bufs = [self.ctx.alloc(layout.byte_length(dtype, n)) for _ in range(2)]
+        bufs = [self.ctx.alloc(layout.byte_length(dtype, n))]
+        try:
+            bufs.append(self.ctx.alloc(layout.byte_length(dtype, n)))
+        except BrikError:
+            self.ctx.free(bufs[0])
+            raise
         planes = [[b.offset(offs[p][0]) for p in self._PLANES[dtype]] for b in bufs]
         cache = self.ctx.kv_cache(dtype, heads, head_dim, page, pages, *planes)
         cache.buffers = bufs

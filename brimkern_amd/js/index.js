@@ -415,7 +415,14 @@ class Engine {
     const n = pages * heads * page * headDim;
     if (!(Number.isInteger(n) && n > 0 && n % 512 === 0)) throw einval('kvCache: pages * heads * page * headDim must be a multiple of 512');
     const offs = planes.planeOffsets(dtype, n), size = planes.byteLength(dtype, n);
-    const kb = this.alloc(size), vb = this.alloc(size);
+    const kb = this.alloc(size);
+    let vb;
+    try {
+      vb = this.alloc(size);
+    } catch (e) {
+      kb.destroy();
+      throw e;
+    }
     const at = function (b, p) { return offs[p] ? b.view(offs[p][0]) : null; };
     return { dtype: dtype, fmt: FMT[dtype], heads: heads, headDim: headDim, page: page, pages: pages, keys: kb, values: vb,
       k: kb, v: vb, kScales: at(kb, 'sc'), vScales: at(vb, 'sc'), kMins: at(kb, 'mn'), vMins: at(vb, 'mn'),

@@ -39,3 +39,12 @@ for (const a of [{}, { scale: undefined }, { scale: null }, { scale: 0 }, { scal
 console.log(JSON.stringify(seen.map(a => a.scale)));
 """)
     assert got == [0.125, 0.125, 0.125, 0, 0.5]
+
+
+def test_second_allocation_of_a_cache_fails():
+    got = run("""
+let said = null;
+try { engine.kvCache('q8', 2, 64, 16, 4); } catch (e) { said = e.message; }
+console.log(JSON.stringify([said, freed]));
+""", left=1)
+    assert got[0] == "out of memory" and len(got[1]) == 1
