@@ -1206,7 +1206,8 @@ napi_value Init(napi_env env, napi_value exports)
         {"liveBuffers", nullptr, LiveBuffers, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
         {"readbackAsync", nullptr, ReadbackAsync, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
         {"selfValidate", nullptr, SelfValidate, nullptr, nullptr, nullptr, napi_enumerable, nullptr},
-        // reached through the facade's methods of the same names; not among the keys of the addon
+        // reached through the facade's methods of the same names; own properties of the addon, but not enumerable: Object.keys is the
+        // matmul path's surface, which callers may compare
         {"qkNormRope", nullptr, QkNormRope, nullptr, nullptr, nullptr, napi_default, nullptr},
         {"kvWrite", nullptr, KvWrite, nullptr, nullptr, nullptr, napi_default, nullptr},
         {"kvRead", nullptr, KvRead, nullptr, nullptr, nullptr, napi_default, nullptr},

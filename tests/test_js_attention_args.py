@@ -48,3 +48,12 @@ try { engine.kvCache('q8', 2, 64, 16, 4); } catch (e) { said = e.message; }
 console.log(JSON.stringify([said, freed]));
 """, left=1)
     assert got[0] == "out of memory" and len(got[1]) == 1
+
+
+def test_whole_surface_of_the_addon():
+    """Every own property of the addon, whether its keys list it or not."""
+    from test_js_host import EXPORTS
+    r = subprocess.run([NODE, "-e", "console.log(JSON.stringify(Object.getOwnPropertyNames(require('./brimkern_amd/js/brik.node'))))"],
+                       cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    assert sorted(json.loads(r.stdout)) == sorted(EXPORTS + ["qkNormRope", "kvWrite", "kvRead", "attention"])
