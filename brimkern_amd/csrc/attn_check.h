@@ -86,12 +86,17 @@ inline int stride(Why& w, const char* who, const char* name, int64_t& s, int64_t
         if (r_ != BRIK_OK) return r_; \
     } while (0)
 
+// Whether rows of aw values, as apart, and of bw values, bs apart, share memory. Of the same stride they may lie side by side in the
+// rows of one buffer; of others only their ranges are compared.
 inline bool overlap(const float* a, int64_t as, int64_t aw, const float* b, int64_t bs, int64_t bw, int rows)
 {
     if (rows <= 0) return false;
     const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
     const uintptr_t a1 = a0 + 4 * (uintptr_t)((rows - 1) * as + aw), b1 = b0 + 4 * (uintptr_t)((rows - 1) * bs + bw);
-    return a0 < b1 && b0 < a1;
+    if (!(a0 < b1 && b0 < a1)) return false;
+    if (as != bs || a0 % 4 != b0 % 4) return true;
+    const int64_t apart = ((int64_t)(b0 - a0) / 4 % as + as) % as;       // b's first column, counted from a's
+    return apart < aw || apart + bw > as;
 }
 
 // write: into a cache (else only norm and rotation). `r` comes back with its strides filled in.

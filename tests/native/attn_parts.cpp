@@ -1,6 +1,6 @@
-// Host test of the rows that a step leaves alone (attn_abi.h), without a device. Prints "ok" and returns 0 when every check
-// holds.
-#include "../../brimkern_amd/csrc/kernels/attn_abi.h"
+// Host test of the rows that a step leaves alone (attn_abi.h) and of rows that share a buffer (attn_check.h), without a device.
+// Prints "ok" and returns 0 when every check holds.
+#include "../../brimkern_amd/csrc/attn_check.h"
 
 #include <cstdio>
 #include <vector>
@@ -37,6 +37,24 @@ int main()
     s.seqs = s.per_seq = 2;
     s.rows = 4;
     for (int32_t t = 0; t < 4; ++t) EXPECT(brik_row_taken(s, t));
+
+    // rows of two kinds in one buffer: overlapping exactly where they share a float
+    for (int64_t as : {8, 12, 16})
+        for (int64_t bs : {8, 12, 16})
+            for (int64_t aw : {4, 8})
+                for (int64_t bw : {4, 8})
+                    for (int rows : {1, 2, 3})
+                        for (int64_t at = 0; at < 120; at += 4) {
+                            const float* const p = reinterpret_cast<const float*>((uintptr_t)0x10000);
+                            bool meet = false;
+                            for (int i = 0; i < rows; ++i)
+                                for (int j = 0; j < rows; ++j) {
+                                    const int64_t a0 = 60 + i * as, b0 = at + j * bs;
+                                    meet = meet || (a0 < b0 + bw && b0 < a0 + aw);
+                                }
+                            const bool said = brik_check::overlap(p + 60, as, aw, p + at, bs, bw, rows);
+                            EXPECT(as == bs ? said == meet : said || !meet);      // of unlike strides: never missed
+                        }
     std::printf(failures ? "%d failure(s)\n" : "ok\n", failures);
     return failures != 0;
 }

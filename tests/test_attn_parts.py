@@ -1,4 +1,4 @@
-"""Which rows of a step belong to a sequence, on the host: the function that the kernels call, compiled into a small driver
+"""Which rows of a step belong to a sequence, and which buffers overlap, on the host: the functions themselves in a small driver
 (tests/native/attn_parts.cpp)."""
 import os
 import subprocess
@@ -6,7 +6,7 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-def test_rows_of_no_sequence(tmp_path):
+def test_parts(tmp_path):
     exe = str(tmp_path / "attn_parts")
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Wextra", "-fsanitize=undefined", "-fno-sanitize-recover=undefined",
                     os.path.join(HERE, "native", "attn_parts.cpp"), "-o", exe], check=True)
