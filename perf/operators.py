@@ -15,6 +15,10 @@ A cache is ``.brik`` q8 or q4 planes of ``[pages, kv heads, page, head dim]`` va
 sequence's tokens lie in the pages of its row of the table, in order. The rows of a step are the last tokens of their
 sequences: row t of the n rows of a sequence of L tokens has position L - n + t and sees the keys up to its own
 position (``window``: only that many of them, its own included). A row that sees no key gives zeros.
+
+The library's context has a stream of its own, which does not wait for torch's and which torch's does not wait for. So with
+``own`` true ``prepare`` returns when its inputs are there; what ``run`` returns is there after ``context().sync()`` (or
+``torch.cuda.synchronize()``, which waits for every stream), and a state is kept until then.
 """
 import math
 
@@ -274,6 +278,7 @@ def prepare(case, seed):
         s["q_out"] = torch.zeros(T, c["H"], c["D"], device=DEV) if c["kind"] != "write" else None
     if own:
         s["h"] = _handles(s)
+        torch.cuda.synchronize()                         # the library's stream does not wait for torch's
     return s
 
 
