@@ -430,7 +430,8 @@ __device__ __forceinline__ half8_t halves_q8(uint32_t w0, uint32_t w1)
 }
 
 // Codes in the low nibbles of each 16 bits as f16 less 8. The products of values have to be of both signs: the matrix
-// cores' sums cut the bits that do not fit, and over sums of nearly equal terms that shows (7e-5 with codes from 0).
+// cores' sums cut the bits that do not fit, and over sums of nearly equal terms that shows (32 sequences of up to 8192: 2.6e-6 of the
+// output's norm with codes from 0, 3.9e-7 so).
 __device__ __forceinline__ half8_t centred_q4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
     const half2_t off = {(_Float16)-1032.f, (_Float16)-1032.f};
@@ -465,7 +466,7 @@ __device__ __forceinline__ float residual(half2_t h, float v)
     return r;
 }
 
-// tanh in f32: the exponential, and near 0, where that cancels, the odd series (next term below 2^-28 of the value).
+// tanh in f32: the exponential, and near 0, where that cancels, the odd series (next term below 2^-26 of the value).
 __device__ __forceinline__ float attn_tanh(float u)
 {
     const float z = u * u;

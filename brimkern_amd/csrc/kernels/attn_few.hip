@@ -12,7 +12,10 @@
 //           the keys within the product follows from that; V's transposed operand is read in it (ds_read_b64_tr_b8).
 //   q4:     s n + m is taken as s (n - 8) + (m + 8 s), the second sum on the vector units.
 // p s may be far from 1 (scales of any size), and a half holds 2^-24 to 65504. So M bounds x_j + e_j, e_j the exponent of the
-// key's largest value scale, within 2^8; p is 2^7 times exp2(x - M) and P' stays below 2^15.
+// key's largest value scale, within 2^8; p is 2^7 times exp2(x - M) and P' stays below 2^15. Its second half ends at 2^-24, which
+// is 2^-31 of the largest p_j 2^e_j: terms of groups whose scales lie far below the largest (of their key, or of one that
+// weighs as much) are rounded to that, not to 2^-22 of themselves. A second pass by group where the sums are low keeps them
+// too, but looking at the sums costs every call 1 to 5 %. Scores stay below 2^22, where M's last place is half a bit.
 //
 // Keys and values go through the wave's own LDS: whole 16-byte chunks of rows are loaded a block ahead into registers, and
 // written rotated by row so that reading a column of chunks meets every bank once.

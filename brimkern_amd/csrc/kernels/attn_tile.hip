@@ -1,13 +1,14 @@
 // Attention of many rows over the quantized cache: prefill, and the rows of all sequences over a shared prefix.
 //
-// 128 or 256 rows a block, 32 a wave (a row: a query head of the key / value head, of a token); 32 keys a step, in LDS for all
-// four waves, two buffers. As in attn_few.hip the products keep f32 accuracy on the f16 matrix cores, here with
+// 128 or 256 rows a block, 32 a wave (a row: a query head of the key / value head, of a token); 32 keys a step, in LDS for all of
+// its waves, two buffers. As in attn_few.hip the products keep f32 accuracy on the f16 matrix cores, here with
 // 32x32x16 products and the conversion done once per block:
 //   scores: S^T = K Q^T; codes exact in f16 (q4: less 8), q as two halves; per group one f32 result, times the key's scale.
 //           q4: the mins' part, sum over groups of (m + 8 s)_jg sum(q)_g, is a product of its own: both as two halves.
 //   output: O^T = V^T P^T with V dequantized to two halves, times 2^-e_j (e_j: exponent of the key's largest scale, so
-//           that its halves are well inside their range), P''_j = p_j 2^e_j as two halves, and the three products
-//           that are above 2^-22. With the scales in V instead of in P the split of P is done once instead of per group.
+//           that its halves are well inside their range, exact to 2^-25, which groups far below the key's largest feel),
+//           P''_j = p_j 2^e_j as two halves, and the three products that are above 2^-22. With the scales in V instead of in
+//           P the split of P is done once instead of per group.
 // A lane holds 16 keys of one row of S^T, which is the layout that the second product wants of P; V's columns come
 // from its rows in LDS by transposed reads (ds_read_b64_tr_b16).
 //

@@ -431,7 +431,11 @@ int brik_kv_read(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batch 
  * position p sees the tokens j <= p, with window > 0 only those j > p - window; a row that sees none gives zeros, a
  * row of NaN gives NaN, and what lies in tokens that a row does not see (infinities, NaN) does not reach it. A shared
  * prefix is read once for all sequences. q and out: f32 [rows, heads, head_dim], a row every *_stride values (0: packed);
- * out must not overlap q. f32-accurate: every product takes the codes exactly and the other operand as two halves.
+ * out must not overlap q. Every product takes the codes exactly and the other operand as two halves, sums are f32. So an output is
+ * as accurate as an f32 sum is against the largest terms of its row: of n tokens it may also be off by 2^-27 sqrt(n) times the largest
+ * p_j |v_j| (p_j the weight, |v_j| the largest value of the token's head, 2^-10 at least). Values some 2^8 and more below the largest
+ * of their head, or of another token's that weighs as much, have fewer exact bits in the output than f32 has. The
+ * scores x_j stay below 2^22 in size; a row with larger ones may hold anything.
  * Workspace: partial results of split key ranges, grown on demand. */
 typedef struct brik_attn_args {
     const float *q;
