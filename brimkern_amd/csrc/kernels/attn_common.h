@@ -95,39 +95,39 @@ __device__ __forceinline__ int wave_sum(int v)
     return uniform((int)(h[0] + h[1]));
 }
 
-// The sequence of row t: how many of row_off[1..seqs] are at most t, or seqs where the row belongs to none (behind the last
-// sequence, or before row_off[0]). One load round trip per 64 sequences.
+// The sequence of row t, or seqs where the row belongs to none (behind the last sequence, or before row_off[0]): how many of
+// row_off[1..seqs] are at most t, where any of row_off[0..seqs) is. One load round trip per 64 sequences.
 __device__ __forceinline__ int seq_of_row(const brik_step& s, int t)
 {
     if (!s.row_off) return t / s.per_seq;
     const int lane = threadIdx.x & 63;
-    const int32_t first = s.row_off[0];
     int count = 0;
+    uint64_t begun = 0;
     for (int base = 0; base < s.seqs; base += 64) {
         const int i = base + lane;
-        const int32_t end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
+        const int32_t first = i < s.seqs ? s.row_off[i] : 0x7fffffff, end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
+        begun |= __ballot(first <= t);
         count += __popcll(__ballot(end <= t));
     }
-    return t < first ? s.seqs : count;
+    return begun ? count : s.seqs;
 }
 
-// The same for a row per lane, whose rows are t0 + (0 .. count - 1) over the wave: every candidate row is compared with 64 ends
-// at a time, so no lane follows a chain of dependent loads.
+// For a row per lane, whose rows are t0 + (0 .. count - 1) over the wave: the last sequence that begins at most at the row, or -1.
+// Every candidate row is compared with 64 sequences at a time, so no lane follows a chain of dependent loads.
 __device__ __forceinline__ int seq_of_lane(const brik_step& s, int t, int t0, int count)
 {
     if (!s.row_off) return t / s.per_seq;
     const int lane = threadIdx.x & 63;
-    const int32_t first = s.row_off[0];
-    int mine = 0;
+    int mine = -1;
     for (int base = 0; base < s.seqs; base += 64) {
         const int i = base + lane;
-        const int32_t end = i < s.seqs ? s.row_off[i + 1] : 0x7fffffff;
+        const int32_t first = i < s.seqs ? s.row_off[i] : 0x7fffffff;
         for (int k = 0; k < count; ++k) {
-            const int c = __popcll(__ballot(end <= t0 + k));
+            const int c = __popcll(__ballot(first <= t0 + k));
             if (t == t0 + k) mine += c;
         }
     }
-    return t < first ? s.seqs : mine;
+    return mine;
 }
 
 // The position of row t of sequence b.
@@ -333,14 +333,19 @@ __device__ __forceinline__ Row find_row(const brik_attn_launch& a, const Work& w
     r.h = w.head * G + i - rel * G;
     r.lo = 0;
     r.hi = 0x7fffffff;
-    int b = w.b;
+    int32_t pos = w.pos + rel;
     if (w.prefix) {
-        const int t0 = uniform(r0 / G), last = min((r0 + ROWS - 1) / G, a.s.rows - 1);
-        b = seq_of_lane(a.s, r.t, t0, uniform(last) - t0 + 1);
-        r.real = r.real && b < a.s.seqs;
+        const int t0 = uniform(r0 / G), last = min((r0 + ROWS - 1) / G, a.s.rows - 1), b = seq_of_lane(a.s, r.t, t0, uniform(last) - t0 + 1);
+        if (!r.real || b < 0) {
+            r.real = false;
+            return r;
+        }
+        const int32_t end = a.s.row_off ? a.s.row_off[b + 1] : (b + 1) * a.s.per_seq;
+        pos = a.s.kv_len[b] - end + r.t;
+        r.real = r.t < end;                                  // else behind the last sequence
     }
     if (!r.real) return r;
-    const int32_t pos = w.prefix ? row_position(a.s, b, r.t) : w.pos + rel, first = w.prefix ? 0 : a.s.prefix_len;
+    const int32_t first = w.prefix ? 0 : a.s.prefix_len;
     const int32_t end = w.prefix ? min(a.s.prefix_len, a.s.max_len)
                                  : (int32_t)min((long long)a.s.max_len - first, min((long long)a.s.table_cols << a.s.shift, 0x7fffffc0ll));
     r.hi = max(0, min(pos + 1 - first, end));

@@ -426,7 +426,7 @@ __device__ __forceinline__ void few_part(const brik_attn_launch& a, const Work& 
     bad |= (uint32_t)__shfl_xor((int)bad, 32);
     if (q == 0) {
         joinm[wave][m] = M;
-        joinl[wave][m] = l;
+        joinl[wave][m] = row.real ? l : -1.f;
     }
     __syncthreads();
     float Mb = fmaxf(fmaxf(joinm[0][m], joinm[1][m]), fmaxf(joinm[2][m], joinm[3][m]));
@@ -456,7 +456,7 @@ __device__ __forceinline__ void few_part(const brik_attn_launch& a, const Work& 
         const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
         const int rel = (w.r0 + r) / G;
         if (rel >= w.count) continue;
-        if (w.prefix && !brik_row_taken(a.s, w.first + rel)) continue;
+        if (joinl[0][r] < 0.f) continue;                     // a row of no sequence
         const int tok = w.first + rel, h = w.head * G + w.r0 + r - rel * G;
         float Mr = joinm[0][r], L = 0.f;
 #pragma unroll
