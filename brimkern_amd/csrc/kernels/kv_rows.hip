@@ -9,8 +9,9 @@
 // A team of TL lanes (head_dim / 4, rounded up to a power of two) holds one head of one row, four values a lane, so a
 // quantization group is 8 neighbouring lanes; sums over a head and the scales of a group are cross-lane reductions, and
 // no value passes through LDS. A block works on one row: its cosines and sines are computed once in LDS and serve
-// all its heads. Bound by memory for long prompts (2048 rows of 40 heads of 128 normed and rotated: 84 MB in 21 us, 4.0 TB/s;
-// 4096 tokens of 16 heads written as q8 14 us, read back 10), by the latency of the 64-bit arithmetic for single rows (4 us).
+// all its heads. Long prompts are bound by memory where rows are normed and rotated (2048 rows of 40 heads of 128: 84 MB in 21 us,
+// 4.0 TB/s) and read back (4096 tokens of 16 heads 10 us), by vector instructions where they are written (the same tokens as q8
+// 14 us, 90 % of the issue cycles), single rows by the latency of the 64-bit arithmetic (4 us).
 #include "attn_common.h"
 #include "encode.h"
 

@@ -258,7 +258,6 @@ class Engine:
                                          "outside this library)")
         return out
 
-    # ---- sampling pre-work ---------------------------------------------------------------
     # ---- attention over a cache of quantized keys and values ---------------------------------
     def kv_cache(self, dtype: str, heads: int, head_dim: int, page: int, pages: int) -> KvCache:
         """A paged cache of its own memory: keys and values one packed .brik tensor [pages, heads, page, head_dim] each."""
@@ -311,6 +310,7 @@ class Engine:
             raise
         return y
 
+    # ---- sampling pre-work ---------------------------------------------------------------
     def _top_k(self, run, recent, k):
         ids = list(dict.fromkeys(int(i) for i in (recent or [])))      # each id once, as the callers pass them
         rb = self.ctx.upload(np.asarray(ids, np.int32)) if ids else None

@@ -9,7 +9,9 @@
  * DEVICE pointer (from brik_alloc or any hipMalloc'd buffer of the same device).
  *
  * Execution model: one context = one device + one HIP stream (default priority). Compute entry
- * points enqueue on that stream and return; brik_sync() waits. Copies are synchronous.
+ * points enqueue on that stream and return; brik_sync() waits. Copies are synchronous. The stream is ordered with no
+ * other one: what another stream writes must be complete before a call reads it, and what a call writes is there for
+ * others after brik_sync or a fence.
  * A context is not thread-safe: use it from one thread at a time.
  *
  * Error model: every int-returning function returns BRIK_OK (0) or a negative BRIK_E* code and
@@ -436,7 +438,8 @@ int brik_kv_read(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batch 
  * p_j |v_j| (p_j the weight, |v_j| the largest value of the token's head, 2^-10 at least). Values some 2^8 and more below the largest
  * of their head, or of another token's that weighs as much, have fewer exact bits in the output than f32 has. The
  * scores x_j stay below 2^22 in size; a row with larger ones may hold anything.
- * Workspace: partial results of split key ranges, grown on demand. */
+ * Workspace: partial results of split key ranges, grown on demand. In one call at most 2^24 - 1 rows, rows times heads below 2^27,
+ * and 2^23 blocks of work (a refusal names their number: a call of very many sequences and key / value heads is made in parts). */
 typedef struct brik_attn_args {
     const float *q;
     float *out;
