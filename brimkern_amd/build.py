@@ -2,7 +2,8 @@
 
 1. ``csrc/kernels/brik_kernels.hip`` -> ``_build/brik_gfx950.hsaco``  (hipcc --genco, gfx950 only), then
    ``check_lds_reads.py`` on its disassembly (the GEMM's inline-asm LDS reads); beside it
-   ``csrc/kernels/brik_attn_kernels.hip`` -> ``_build/brik_attn_gfx950.hsaco`` (the attention side)
+   ``csrc/kernels/brik_attn_kernels.hip`` -> ``_build/brik_attn_gfx950.hsaco`` (the attention side) and
+   ``brik_moe_kernels.hip`` -> ``_build/brik_moe_gfx950.hsaco`` (experts, products of 8-bit integers)
 2. ``csrc/brik_scratch.hip`` -> ``_build/brik_scratch.o`` (hipcc -c: the no-allocation scratch array)
 3. ``csrc/brik_runtime.cpp`` + ``csrc/brik_embed.S`` (embeds the code objects) + that object ->
    ``libbrik.so`` (the C ABI declared in ``include/brik.h``)
@@ -29,6 +30,8 @@ NODE_INC = "/usr/include/node"
 
 HSACO = os.path.join(BUILD, "brik_gfx950.hsaco")
 ATTN_HSACO = os.path.join(BUILD, "brik_attn_gfx950.hsaco")
+MOE_HSACO = os.path.join(BUILD, "brik_moe_gfx950.hsaco")
+HSACO_DEFINES = [f'-DBRIK_HSACO_PATH="{HSACO}"', f'-DBRIK_ATTN_HSACO_PATH="{ATTN_HSACO}"', f'-DBRIK_MOE_HSACO_PATH="{MOE_HSACO}"']
 SCRATCH_OBJ = os.path.join(BUILD, "brik_scratch.o")
 LIB = os.path.join(PKG, "libbrik.so")
 ADDON = os.path.join(PKG, "js", "brik.node")
@@ -70,6 +73,10 @@ def build_attn_hsaco(verbose=False):
     return _genco("brik_attn_kernels.hip", ATTN_HSACO, [], verbose)
 
 
+def build_moe_hsaco(verbose=False):
+    return _genco("brik_moe_kernels.hip", MOE_HSACO, [], verbose)
+
+
 def build_scratch(verbose=False):
     """``csrc/brik_scratch.hip`` (the fixed device scratch of the no-allocation entry point and its
     address lookup) as a HIP object, linked into libbrik.so."""
@@ -85,7 +92,7 @@ def build_lib(verbose=False):
     tmp = LIB + ".tmp"
     _run(["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", "-Wextra",
           "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROCM, "include"),
-          f'-DBRIK_HSACO_PATH="{HSACO}"', f'-DBRIK_ATTN_HSACO_PATH="{ATTN_HSACO}"',
+          *HSACO_DEFINES,
           os.path.join(CSRC, "brik_runtime.cpp"), os.path.join(CSRC, "brik_embed.S"), SCRATCH_OBJ,
           "-L", os.path.join(ROCM, "lib"), "-lamdhip64", f"-Wl,-rpath,{os.path.join(ROCM, 'lib')}",
           "-Wl,--no-undefined", "-o", tmp], verbose)
@@ -120,7 +127,7 @@ def _build_sanitize(out, verbose):
         _run(["g++", "-O1", "-g", "-std=c++17", "-Wall", "-Wextra", "-fno-omit-frame-pointer",
               "-fsanitize=address,undefined", "-fno-sanitize-recover=undefined", "-static-libasan",
               "-D__HIP_PLATFORM_AMD__", "-I", os.path.join(ROCM, "include"), "-I", os.path.join(ROOT, "include"),
-              f'-DBRIK_HSACO_PATH="{HSACO}"', f'-DBRIK_ATTN_HSACO_PATH="{ATTN_HSACO}"', out + ".cpp",
+              *HSACO_DEFINES, out + ".cpp",
               os.path.join(CSRC, "brik_runtime.cpp"), os.path.join(CSRC, "brik_embed.S"), SCRATCH_OBJ,
               "-L", os.path.join(ROCM, "lib"), "-lamdhip64", f"-Wl,-rpath,{os.path.join(ROCM, 'lib')}",
               "-o", tmp], verbose)
@@ -144,8 +151,8 @@ def check_hsaco(verbose=False):
 
 
 def build(verbose=False):
-    with concurrent.futures.ThreadPoolExecutor(3) as pool:        # three compilers side by side
-        for job in [pool.submit(f, verbose) for f in (build_hsaco, build_attn_hsaco, build_scratch)]:
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:        # four compilers side by side
+        for job in [pool.submit(f, verbose) for f in (build_hsaco, build_attn_hsaco, build_moe_hsaco, build_scratch)]:
             job.result()
     check_hsaco(verbose)
     build_lib(verbose)

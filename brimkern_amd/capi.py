@@ -21,6 +21,7 @@ BRIK_GEMV_VARIANTS = 11
 BRIK_OPT_GEMM_TILE, BRIK_GEMM_TILES = 3, 23
 BRIK_OPT_PLAN_STAGE, BRIK_OPT_PLAN_SETS, BRIK_OPT_SPLITK, BRIK_OPT_GEMV_BLOCKS = 4, 5, 6, 7
 BRIK_OPT_ATTN_ROWS, BRIK_OPT_ATTN_SPLITS = 8, 9
+BRIK_OPT_I8_KERNEL, BRIK_OPT_I8_SPLITS = 10, 11
 PATH_AUTO, PATH_GEMV, PATH_GEMM = 0, 1, 2
 BRIK_PATH_GEMV, BRIK_PATH_GEMV_STAGED, BRIK_PATH_TILED, BRIK_PATH_SPLITK = 1, 2, 3, 4
 
@@ -83,6 +84,15 @@ SIGNATURES = {
     "brik_kv_write": (_I, [_P, _P, _P, _P]),
     "brik_kv_read": (_I, [_P, _P, _P, _P, _P]),
     "brik_attention": (_I, [_P, _P, _P, _P]),
+    "brik_moe_route": (_I, [_P, _P]),
+    "brik_moe_route_grad": (_I, [_P, _P, _P, _P]),
+    "brik_moe_sort": (_I, [_P, _P, _I, _I, _I, _P, _P, _P]),
+    "brik_moe_dispatch": (_I, [_P, _P, _P, _P, _P, _I, _I, _I]),
+    "brik_moe_combine": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I]),
+    "brik_moe_combine_grad": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I]),
+    "brik_quantize_i8": (_I, [_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _I, _P, _P, _I, _I]),
+    "brik_matmul_t_i8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I]),
+    "brik_moe_matmul_t_i8": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I]),
 }
 BRIK_TOPK_MAX = 64
 BRIK_NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -136,6 +146,16 @@ class AttnArgs(ctypes.Structure):
 
 
 BRIK_QKV_GAIN_ONE_PLUS, BRIK_QKV_INTERLEAVED = 1, 2
+
+
+class MoeRouteArgs(ctypes.Structure):
+    """``brik_moe_route_args`` of include/brik.h."""
+    _fields_ = [("logits", _P), ("bias", _P), ("logit_stride", _I64), ("ids", _P), ("weights", _P), ("row_off", _P), ("src", _P),
+                ("slot", _P), ("tokens", _I32), ("experts", _I32), ("k", _I32), ("flags", _I32), ("scale", _F32), ("reserved", _I32)]
+
+
+BRIK_ROUTE_SIGMOID, BRIK_ROUTE_RENORM = 1, 2
+BRIK_MOE_EXPERTS, BRIK_MOE_K, BRIK_I8_K = 1024, 64, 131040
 
 
 class BrikError(RuntimeError):
@@ -438,6 +458,59 @@ class Context:
     def attention(self, cache: KvCache, batch: KvBatch, args: AttnArgs):
         """Attention of the batch's rows over the cache (brik_attention)."""
         self._check(self.lib.brik_attention(self.handle, ctypes.addressof(cache), ctypes.addressof(batch), ctypes.addressof(args)))
+
+    # ---- experts: routing, tokens to their experts and back ---------------------------------------
+    @staticmethod
+    def moe_route_args(logits, tokens, experts, k, ids, weights, bias=None, row_off=None, src=None, slot=None, sigmoid=False, renorm=False,
+                       scale=1.0, logit_stride=0) -> MoeRouteArgs:
+        """The routing of a step, made once and used in every one (``brik_moe_route_args``)."""
+        flags = (BRIK_ROUTE_SIGMOID if sigmoid else 0) | (BRIK_ROUTE_RENORM if renorm else 0)
+        return MoeRouteArgs(_addr(logits), _addr(bias), logit_stride, _addr(ids), _addr(weights), _addr(row_off), _addr(src), _addr(slot),
+                            tokens, experts, k, flags, scale, 0)
+
+    def moe_route(self, args: MoeRouteArgs):
+        """The k experts of every token, their weights and, if asked for, the sorted assignments (brik_moe_route)."""
+        self._check(self.lib.brik_moe_route(self.handle, ctypes.addressof(args)))
+
+    def moe_route_grad(self, args: MoeRouteArgs, dweights, dlogits):
+        """The gradient of the logits from that of the weights (brik_moe_route_grad)."""
+        self._check(self.lib.brik_moe_route_grad(self.handle, ctypes.addressof(args), _addr(dweights), _addr(dlogits)))
+
+    def moe_sort(self, ids, tokens, k, experts, row_off, src, slot):
+        """Assignments ``ids`` [tokens, k] sorted by expert (brik_moe_sort)."""
+        self._check(self.lib.brik_moe_sort(self.handle, _addr(ids), tokens, k, experts, _addr(row_off), _addr(src), _addr(slot)))
+
+    def moe_dispatch(self, x, slot, weights, x_sorted, tokens, k, width):
+        """The tokens' rows to their experts' rows, times ``weights`` unless None (brik_moe_dispatch)."""
+        self._check(self.lib.brik_moe_dispatch(self.handle, _addr(x), _addr(slot), _addr(weights), _addr(x_sorted), tokens, k, width))
+
+    def moe_combine(self, y_sorted, slot, weights, res, out, tokens, k, width):
+        """The experts' rows back to the tokens, weighted and summed, plus ``res`` unless None (brik_moe_combine)."""
+        self._check(self.lib.brik_moe_combine(self.handle, _addr(y_sorted), _addr(slot), _addr(weights), _addr(res), _addr(out), tokens, k,
+                                              width))
+
+    def moe_combine_grad(self, dout, y_sorted, slot, weights, dy_sorted, dweights, tokens, k, width):
+        """The gradients of the experts' rows and of the weights (brik_moe_combine_grad)."""
+        self._check(self.lib.brik_moe_combine_grad(self.handle, _addr(dout), _addr(y_sorted), _addr(slot), _addr(weights), _addr(dy_sorted),
+                                                   _addr(dweights), tokens, k, width))
+
+    # ---- products of 8-bit integers ---------------------------------------------------------------
+    def quantize_i8(self, x, codes, scales, M, K, x_stride=0, gate=None, gate_stride=0, gelu=False):
+        """Rows of x, or of act(gate) * x, to int8 codes and a scale each (brik_quantize_i8)."""
+        self._check(self.lib.brik_quantize_i8(self.handle, _addr(x), x_stride, _addr(gate), gate_stride, BRIK_JOB_ACT_GELU if gelu else 0,
+                                              _addr(codes), _addr(scales), M, K))
+
+    def matmul_t_i8(self, x, x_scales, w, w_scales, y, M, K, N, res=None):
+        """y = x . w^T of int8 codes, scaled by row and channel, plus ``res`` unless None (brik_matmul_t_i8)."""
+        self._check(self.lib.brik_matmul_t_i8(self.handle, _addr(x), _addr(x_scales), _addr(w), _addr(w_scales), _addr(res), _addr(y), M, K, N))
+
+    def moe_matmul_t_i8(self, x, x_scales, row_off, w, w_scales, y_sorted, E, rows, K, N, src=None, k=1, x_rows=None):
+        """The same by experts (brik_moe_matmul_t_i8). x: the sorted rows or, with ``src`` and ``k``, the tokens (rows / k of them
+        unless ``x_rows`` says otherwise)."""
+        if x_rows is None:
+            x_rows = rows if src is None else rows // max(k, 1)
+        self._check(self.lib.brik_moe_matmul_t_i8(self.handle, _addr(x), _addr(x_scales), x_rows, _addr(src), k, _addr(row_off), _addr(w),
+                                                  _addr(w_scales), _addr(y_sorted), E, rows, K, N))
 
     def dequant_q8(self, codes, sc, out, n):
         self._check(self.lib.brik_dequant_q8_f32(self.handle, _addr(codes), _addr(sc), _addr(out), n))

@@ -14,4 +14,10 @@ brik_hsaco_end:
 brik_attn_hsaco_begin:
     .incbin BRIK_ATTN_HSACO_PATH
     .byte 0
+    .balign 4096
+    .globl brik_moe_hsaco_begin
+    .type brik_moe_hsaco_begin, @object
+brik_moe_hsaco_begin:
+    .incbin BRIK_MOE_HSACO_PATH
+    .byte 0
     .section .note.GNU-stack, "", @progbits

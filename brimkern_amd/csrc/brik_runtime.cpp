@@ -7,7 +7,10 @@
 #include "../../include/brik.h"
 #include "attn_check.h"
 #include "attn_plan.h"
+#include "moe_check.h"
+#include "moe_plan.h"
 #include "kernels/attn_abi.h"
+#include "kernels/moe_abi.h"
 #include "kernels/stage_abi.h"
 
 #include <hip/hip_runtime_api.h>
@@ -24,6 +27,7 @@
 extern "C" const unsigned char brik_hsaco_begin[];
 extern "C" const unsigned char brik_hsaco_end[];
 extern "C" const unsigned char brik_attn_hsaco_begin[];
+extern "C" const unsigned char brik_moe_hsaco_begin[];
 // brik_scratch.hip: device address of the fixed scratch array on the current device (a hipError_t)
 extern "C" int brik_scratch_resolve(int device, void** out, size_t* bytes);
 
@@ -60,6 +64,13 @@ const char* const kKernelNames[K_COUNT] = {
 // (256: up to head_dim 128).
 enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE4 = A_FEW + 10, A_TILE8 = A_TILE4 + 10, A_JOIN = A_TILE8 + 10, A_JOIN_FEW, A_COUNT };
 constexpr int kAttnDims[5] = {64, 96, 128, 192, 256};
+
+// Kernels of the experts' code object: routing of 1, 2, 4, 8, 16 experts a lane (brik_route_<n>, _bias_<n>, _grad_<n>), then the
+// others by name; quantization without and with a gate by a wave, 256 and 1024 threads a row.
+enum MoeKern {
+    E_ROUTE, E_BIAS = E_ROUTE + 5, E_GRAD = E_BIAS + 5, E_COUNT_IDS = E_GRAD + 5, E_SORT, E_DISPATCH, E_COMBINE, E_COMBINE_GRAD,
+    E_QUANT, E_I8_JOIN = E_QUANT + 6, E_I8, E_COUNT = E_I8 + brik_plan::kI8Count
+};
 
 // GEMV variants {team, r, u, d}, in the order of BRIK_GEMV_FMT in gemv.hip: TEAM lanes per row team,
 // R rows per team, U groups per pipeline step, pipeline depth D; kernels brik_gemv_<fmt>_t<T>_r<R>_u<U>_d<D>
@@ -236,6 +247,8 @@ struct brik_ctx {
     hipModule_t module = nullptr;
     hipModule_t attn_module = nullptr;
     hipFunction_t attn_fn[A_COUNT] = {};
+    hipModule_t moe_module = nullptr;
+    hipFunction_t moe_fn[E_COUNT] = {};
     hipFunction_t fn[K_COUNT] = {};
     hipFunction_t gemv[3][kNumGemvVariants] = {};
     hipFunction_t gemvg[3][kNumGemvVariants] = {};
@@ -263,6 +276,8 @@ struct brik_ctx {
     int opt_gemv_blocks = 0; // single-matrix GEMV: 0 auto, else grid cap
     int opt_attn_rows = 0;   // attention: 0 auto, else rows of a tile
     int opt_attn_splits = 0; // attention: 0 auto, else splits of every tile's keys
+    int opt_i8_kernel = 0;   // 8-bit products: 0 auto, else 1 + index into brik_plan::kI8Kernels
+    int opt_i8_splits = 0;   // 8-bit products: 0 auto, else splits of K over blocks (dense)
     void* ws = nullptr;    // GEMM workspace: f16 activation rows, then per-row scales (grow-only)
     size_t ws_bytes = 0;
     void* tws = nullptr;   // top-k workspace: lane maxima, then LM-head logits (grow-only)
@@ -275,6 +290,10 @@ struct brik_ctx {
     size_t pws_bytes = 0;
     void* aws = nullptr;   // attention: partial results of split keys (grow-only)
     size_t aws_bytes = 0;
+    void* ews = nullptr;   // routing: assignments by chunk and expert (one size, so it never moves)
+    size_t ews_bytes = 0;
+    void* iws = nullptr;   // 8-bit products: partial sums of split K (grow-only)
+    size_t iws_bytes = 0;
     void* qws = nullptr;   // few-row GEMM: partial tiles (fixed size, so graphs may hold its address)
     void* fws = nullptr;   // fragment GEMM: x panels and the f16 weight panels of one column slab (grow-only)
     size_t fws_bytes = 0;
@@ -1453,6 +1472,18 @@ int brik_create(int device, brik_ctx** out)
         if (k >= A_TILE8 && k < A_JOIN && kAttnDims[(k - A_FEW) % 5] > 128) continue;
         if (hipModuleGetFunction(&c->attn_fn[k], c->attn_module, name) != hipSuccess) return bail(BRIK_EMODULE);
     }
+    if (hipModuleLoadData(&c->moe_module, brik_moe_hsaco_begin) != hipSuccess) return bail(BRIK_EMODULE);
+    for (int k = 0; k < E_COUNT; ++k) {
+        char name[64];
+        const char* const route[3] = {"", "bias_", "grad_"};
+        const char* const others[] = {"brik_route_count", "brik_route_sort", "brik_rows_dispatch", "brik_rows_combine", "brik_rows_combine_grad"};
+        const char* const quant[3] = {"wave", "256", "1024"};
+        if (k < E_COUNT_IDS) snprintf(name, sizeof name, "brik_route_%s%d", route[k / 5], 1 << k % 5);
+        else if (k < E_QUANT) snprintf(name, sizeof name, "%s", others[k - E_COUNT_IDS]);
+        else if (k < E_I8_JOIN) snprintf(name, sizeof name, "brik_quant_i8_%s%s", k - E_QUANT >= 3 ? "glu_" : "", quant[(k - E_QUANT) % 3]);
+        else snprintf(name, sizeof name, "%s", k == E_I8_JOIN ? "brik_i8_join" : brik_plan::kI8Kernels[k - E_I8].name);
+        if (hipModuleGetFunction(&c->moe_fn[k], c->moe_module, name) != hipSuccess) return bail(BRIK_EMODULE);
+    }
     // the fixed scratch of brik_matmul_t_q4_noalloc, with this device current (once per device)
     c->scratch_err = brik_scratch_resolve(device, &c->scratch, &c->scratch_bytes);
     constexpr int kSkl[3] = {2, 4, 8};
@@ -1501,8 +1532,11 @@ void brik_destroy(brik_ctx* c)
     if (c->kws) (void)hipFree(c->kws);
     if (c->qws) (void)hipFree(c->qws);
     if (c->aws) (void)hipFree(c->aws);
+    if (c->ews) (void)hipFree(c->ews);
+    if (c->iws) (void)hipFree(c->iws);
     if (c->module) (void)hipModuleUnload(c->module);
     if (c->attn_module) (void)hipModuleUnload(c->attn_module);
+    if (c->moe_module) (void)hipModuleUnload(c->moe_module);
     delete c;
 }
 
@@ -2591,6 +2625,241 @@ int brik_attention(brik_ctx* c, const brik_kv_cache* cache, const brik_kv_batch*
     return attention(c, a, batch->max_rows);
 }
 
+// ---- experts ----
+
+// Assignments that one block routes and sorts by itself, and that one block sorts.
+constexpr int kRouteAlone = 512, kSortAlone = 4096;
+
+static int take_counts(brik_ctx* c, brik_route_launch& a)
+{
+    HIP_TRY_RC(ensure_buf(c, c->ews, c->ews_bytes, BRIK_MOE_WS_BYTES));
+    a.counts = static_cast<int32_t*>(c->ews);
+    return BRIK_OK;
+}
+
+int brik_moe_route(brik_ctx* c, const brik_moe_route_args* args)
+{
+    if (!c) return BRIK_EINVAL;
+    if (!args) return fail(c, BRIK_EINVAL, "moe_route: args is null");
+    brik_check::Why w;
+    brik_route_launch a{};
+    a.r = *args;
+    const int rc = brik_check::route(w, "moe_route", a.r, false);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (a.r.tokens == 0 || a.r.k == 0)
+        return a.r.row_off ? fill_zero(c, reinterpret_cast<float*>(a.r.row_off), (size_t)a.r.experts + 1) : BRIK_OK;
+    const bool sorted = a.r.row_off != nullptr;
+    brik_plan::moe_chunks(a, sorted ? kRouteAlone : 0);
+    if (sorted && a.chunks > 1) HIP_TRY_RC(take_counts(c, a));
+    void* route[] = {&a};
+    HIP_TRY_RC(launch_fn(c, c->moe_fn[(a.r.bias ? E_BIAS : E_ROUTE) + brik_plan::moe_lanes(a.r.experts)], (unsigned)a.chunks, 1, 1024, 0, route));
+    return sorted && a.chunks > 1 ? launch_fn(c, c->moe_fn[E_SORT], (unsigned)a.chunks, 1, 1024, 0, route) : BRIK_OK;
+}
+
+int brik_moe_route_grad(brik_ctx* c, const brik_moe_route_args* args, const float* dweights, float* dlogits)
+{
+    if (!c) return BRIK_EINVAL;
+    if (!args) return fail(c, BRIK_EINVAL, "moe_route_grad: args is null");
+    brik_check::Why w;
+    brik_route_launch a{};
+    a.r = *args;
+    const int rc = brik_check::route(w, "moe_route_grad", a.r, true);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (a.r.tokens == 0 || a.r.experts == 0) return BRIK_OK;
+    if (!dlogits || (!dweights && a.r.k > 0)) return fail(c, BRIK_EINVAL, "moe_route_grad: dweights or dlogits is null");
+    if (!aligned(dweights, 4) || !aligned(dlogits, 4)) return fail(c, BRIK_EALIGN, "moe_route_grad: dweights and dlogits must be 4-byte aligned");
+    void* grad[] = {&a, &dweights, &dlogits};
+    return launch_fn(c, c->moe_fn[E_GRAD + brik_plan::moe_lanes(a.r.experts)], (unsigned)((a.r.tokens + 3) / 4), 1, 256, 0, grad);
+}
+
+int brik_moe_sort(brik_ctx* c, const int32_t* ids, int tokens, int k, int experts, int32_t* row_off, int32_t* src, int32_t* slot)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    int rc = brik_check::places(w, "moe_sort", tokens, k);
+    if (rc == BRIK_OK) rc = brik_check::experts(w, "moe_sort", experts);
+    const bool any = rc == BRIK_OK && (long long)tokens * k > 0;
+    if (rc == BRIK_OK) rc = brik_check::sorted(w, "moe_sort", row_off, src, slot, any);
+    if (rc == BRIK_OK && any && !ids) rc = brik_check::no(w, BRIK_EINVAL, "moe_sort: ids is null");
+    if (rc == BRIK_OK && !aligned(ids, 4)) rc = brik_check::no(w, BRIK_EALIGN, "moe_sort: ids must be 4-byte aligned");
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (!any) return fill_zero(c, reinterpret_cast<float*>(row_off), (size_t)experts + 1);
+    brik_route_launch a{};
+    a.r.ids = const_cast<int32_t*>(ids);
+    a.r.tokens = tokens;
+    a.r.k = k;
+    a.r.experts = experts;
+    a.r.row_off = row_off;
+    a.r.src = src;
+    a.r.slot = slot;
+    brik_plan::moe_chunks(a, kSortAlone);
+    void* sort[] = {&a};
+    if (a.chunks > 1) {
+        HIP_TRY_RC(take_counts(c, a));
+        HIP_TRY_RC(launch_fn(c, c->moe_fn[E_COUNT_IDS], (unsigned)a.chunks, 1, 1024, 0, sort));
+    }
+    return launch_fn(c, c->moe_fn[E_SORT], (unsigned)a.chunks, 1, 1024, 0, sort);
+}
+
+// Blocks of a token's row: one where the tokens alone fill the device, else up to one for 256 quads.
+static unsigned spread_blocks(const brik_spread_launch& a)
+{
+    return row_blocks(a.tokens, a.quads, 256);
+}
+
+int brik_moe_dispatch(brik_ctx* c, const float* x, const int32_t* slot, const float* weights, float* x_sorted, int tokens, int k, int width)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    int rc = brik_check::spread(w, "moe_dispatch", tokens, k, width, slot, weights);
+    const bool any = rc == BRIK_OK && tokens > 0 && k > 0 && width > 0;
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_dispatch", "x", x, any);
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_dispatch", "x_sorted", x_sorted, any);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (!any) return BRIK_OK;
+    brik_spread_launch a{};
+    a.x = x;
+    a.slot = slot;
+    a.weights = weights;
+    a.rows = x_sorted;
+    a.tokens = tokens;
+    a.k = k;
+    a.quads = width / 4;
+    void* args[] = {&a};
+    return launch_fn(c, c->moe_fn[E_DISPATCH], (unsigned)tokens, spread_blocks(a), 256, 0, args);
+}
+
+int brik_moe_combine(brik_ctx* c, const float* y_sorted, const int32_t* slot, const float* weights, const float* res, float* out, int tokens,
+                     int k, int width)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    int rc = brik_check::spread(w, "moe_combine", tokens, k, width, slot, weights);
+    const bool any = rc == BRIK_OK && tokens > 0 && width > 0;
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_combine", "y_sorted", y_sorted, any && k > 0);
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_combine", "res", res, false);
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_combine", "out", out, any);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (!any) return BRIK_OK;
+    brik_spread_launch a{};
+    a.y = y_sorted;
+    a.slot = slot;
+    a.weights = weights;
+    a.res = res;
+    a.out = out;
+    a.tokens = tokens;
+    a.k = k;
+    a.quads = width / 4;
+    void* args[] = {&a};
+    return launch_fn(c, c->moe_fn[E_COMBINE], (unsigned)tokens, spread_blocks(a), 256, 0, args);
+}
+
+int brik_moe_combine_grad(brik_ctx* c, const float* dout, const float* y_sorted, const int32_t* slot, const float* weights, float* dy_sorted,
+                          float* dweights, int tokens, int k, int width)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    int rc = brik_check::spread(w, "moe_combine_grad", tokens, k, width, slot, weights);
+    const bool any = rc == BRIK_OK && tokens > 0 && k > 0;
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_combine_grad", "dout", dout, any && width > 0);
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_combine_grad", "y_sorted", y_sorted, any && width > 0 && dweights);
+    if (rc == BRIK_OK) rc = brik_check::rows16(w, "moe_combine_grad", "dy_sorted", dy_sorted, false);
+    if (rc == BRIK_OK && !aligned(dweights, 4)) rc = brik_check::no(w, BRIK_EALIGN, "moe_combine_grad: dweights must be 4-byte aligned");
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (!any || (!dy_sorted && !dweights)) return BRIK_OK;
+    brik_spread_launch a{};
+    a.x = dout;
+    a.y = y_sorted;
+    a.slot = slot;
+    a.weights = weights;
+    a.rows = dy_sorted;
+    a.dweights = dweights;
+    a.tokens = tokens;
+    a.k = k;
+    a.quads = width / 4;
+    void* args[] = {&a};
+    return launch_fn(c, c->moe_fn[E_COMBINE_GRAD], (unsigned)tokens, 1, 256, 0, args);
+}
+
+int brik_quantize_i8(brik_ctx* c, const float* x, int64_t x_stride, const float* gate, int64_t gate_stride, int flags, int8_t* codes,
+                     float* scales, int M, int K)
+{
+    if (!c) return BRIK_EINVAL;
+    brik_check::Why w;
+    brik_quant_launch a{x, gate, x_stride, gate_stride, codes, scales, M, K, flags & BRIK_JOB_ACT_GELU};
+    const int rc = brik_check::quantize_i8(w, "quantize_i8", a, flags);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (M == 0) return BRIK_OK;
+    const int size = K <= 1024 ? 0 : K <= 4096 ? 1 : 2;
+    void* args[] = {&a};
+    return launch_fn(c, c->moe_fn[E_QUANT + 3 * (gate != nullptr) + size], (unsigned)(size ? M : (M + 3) / 4), 1, size == 2 ? 1024 : 256, 0, args);
+}
+
+static int product_i8(brik_ctx* c, const char* who, brik_i8_launch& a, bool moe)
+{
+    if (!c) return BRIK_EINVAL;
+    c->last_path = 0;
+    c->last_kernel = "";
+    brik_check::Why w;
+    const int rc = brik_check::product_i8(w, who, a, moe);
+    if (rc != BRIK_OK) return refuse(c, rc, w);
+    if (a.M == 0 || a.N == 0 || (moe && (a.E == 0 || a.x_rows == 0))) return BRIK_OK;
+    const int t = brik_plan::i8_plan(a, c->opt_i8_kernel);
+    const brik_plan::I8Kernel& g = brik_plan::kI8Kernels[t];
+    if (c->opt_i8_splits && !moe) {
+        a.steps = std::max(1, (a.steps + c->opt_i8_splits - 1) / c->opt_i8_splits);
+        a.splits = std::max(1, ((a.K + 63) / 64 + a.steps - 1) / a.steps);
+    }
+    if (a.splits > 1) {
+        HIP_TRY_RC(ensure_buf(c, c->iws, c->iws_bytes, 4 * (size_t)a.splits * a.M * a.N));
+        a.part = static_cast<int32_t*>(c->iws);
+    }
+    const long blocks = (long)a.row_tiles * a.col_tiles * a.splits;
+    if (blocks >= (1l << 23)) return fail(c, BRIK_EINVAL, "%s: %ld blocks in one call", who, blocks);
+    c->last_kernel = g.few ? "i8_few" : "i8_tile";
+    void* args[] = {&a};
+    HIP_TRY_RC(launch_fn(c, c->moe_fn[E_I8 + t], (unsigned)blocks, 1, (unsigned)g.threads, 0, args));
+    if (a.splits == 1) return BRIK_OK;
+    const long join = std::min<long>(((long)a.M * a.N + 255) / 256, 16 * kCUs);
+    return launch_fn(c, c->moe_fn[E_I8_JOIN], (unsigned)join, 1, 256, 0, args);
+}
+
+int brik_matmul_t_i8(brik_ctx* c, const int8_t* x, const float* x_scales, const int8_t* w, const float* w_scales, const float* res, float* y,
+                     int M, int K, int N)
+{
+    brik_i8_launch a{};
+    a.x = x;
+    a.xs = x_scales;
+    a.w = w;
+    a.ws = w_scales;
+    a.res = res;
+    a.y = y;
+    a.M = M;
+    a.K = K;
+    a.N = N;
+    return product_i8(c, "matmul_t_i8", a, false);
+}
+
+int brik_moe_matmul_t_i8(brik_ctx* c, const int8_t* x, const float* x_scales, int x_rows, const int32_t* src, int k, const int32_t* row_off,
+                         const int8_t* w, const float* w_scales, float* y_sorted, int E, int rows, int K, int N)
+{
+    brik_i8_launch a{};
+    a.x = x;
+    a.xs = x_scales;
+    a.w = w;
+    a.ws = w_scales;
+    a.y = y_sorted;
+    a.src = src;
+    a.row_off = row_off;
+    a.k = k;
+    a.x_rows = x_rows;
+    a.E = E;
+    a.M = rows;
+    a.K = K;
+    a.N = N;
+    return product_i8(c, "moe_matmul_t_i8", a, true);
+}
+
 int brik_timer_begin(brik_ctx* c)
 {
     if (!c) return BRIK_EINVAL;
@@ -2738,6 +3007,14 @@ int brik_set_option(brik_ctx* c, int key, int value)
     case BRIK_OPT_ATTN_SPLITS:
         if (value < 0 || value > 256) return fail(c, BRIK_EINVAL, "BRIK_OPT_ATTN_SPLITS: %d not in 0..256", value);
         c->opt_attn_splits = value;
+        return BRIK_OK;
+    case BRIK_OPT_I8_KERNEL:
+        if (value < 0 || value > brik_plan::kI8Count) return fail(c, BRIK_EINVAL, "BRIK_OPT_I8_KERNEL: %d not in 0..%d", value, brik_plan::kI8Count);
+        c->opt_i8_kernel = value;
+        return BRIK_OK;
+    case BRIK_OPT_I8_SPLITS:
+        if (value < 0 || value > 64) return fail(c, BRIK_EINVAL, "BRIK_OPT_I8_SPLITS: %d not in 0..64", value);
+        c->opt_i8_splits = value;
         return BRIK_OK;
     default:
         return fail(c, BRIK_EINVAL, "unknown option %d", key);

@@ -451,6 +451,98 @@ typedef struct brik_attn_args {
 } brik_attn_args;
 int brik_attention(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batch *batch, const brik_attn_args *args);
 
+/* ---- experts: routing, tokens to their experts and back -----------------------------------------
+ * What a mixture-of-experts layer runs around its experts' products (brik_moe_matmul_t_q4 and _i8, on rows sorted by
+ * expert). No counterpart in the reference, which has no MoE. An assignment is a pair (token t, place j < k), numbered
+ * a = t * k + j; its expert is ids[a]. Assignments whose id is outside [0, experts) (none chosen, or another device's expert)
+ * have no row. Sorted rows are the others, by expert, those of an expert in the order of a: row_off[e] is the first row of
+ * expert e, row_off[experts] their number; src[r] is the assignment of row r (-1 from there on), slot[a] the row of an
+ * assignment (-1: none). All of them int32 DEVICE arrays: row_off [experts + 1], src and slot [tokens * k].
+ *
+ * brik_moe_route: the k experts of every token and their weights. With l the token's logits and s = softmax(l) over all
+ * experts or, with BRIK_ROUTE_SIGMOID, s = 1 / (1 + exp(-l)):
+ *   ids      the k largest s, with bias the k largest s + bias (in 64 bits), the largest first, ties by smaller id; a
+ *            logit (or sum) of -infinity or NaN is never chosen: where fewer are left the others are -1
+ *   weights  scale * s of the chosen ones (without the bias), with BRIK_ROUTE_RENORM divided by their sum; 0 for id -1
+ * A token all of whose logits are -infinity (padding) so goes nowhere. A NaN logit counts as -infinity; +infinity gives a
+ * softmax of NaN. row_off, src and slot: all three, and the assignments are sorted by the same call, or none.
+ * tokens below 2^24, tokens * k at most 2^30, experts at most BRIK_MOE_EXPERTS, k at most BRIK_MOE_K and at most experts. Logits are 4-byte aligned,
+ * [tokens, experts] with a row every logit_stride values (0: packed). Workspace: at most 1 MiB, taken once. */
+#define BRIK_MOE_EXPERTS 1024
+#define BRIK_MOE_K 64
+#define BRIK_ROUTE_SIGMOID 1
+#define BRIK_ROUTE_RENORM 2
+typedef struct brik_moe_route_args {
+    const float *logits;
+    const float *bias;           /* DEVICE [experts], or NULL */
+    int64_t logit_stride;
+    int32_t *ids;                /* [tokens, k] */
+    float *weights;              /* [tokens, k] */
+    int32_t *row_off, *src, *slot;
+    int32_t tokens, experts, k;
+    int32_t flags;
+    float scale;
+    int32_t reserved;            /* 0 */
+} brik_moe_route_args;
+int brik_moe_route(brik_ctx *ctx, const brik_moe_route_args *args);
+
+/* dlogits [tokens, experts] (packed) of a call of brik_moe_route whose weights have the gradient dweights [tokens, k]; ids are
+ * read as that call left them, weights and the sorted arrays are not looked at. The choice itself and the bias have no
+ * gradient. */
+int brik_moe_route_grad(brik_ctx *ctx, const brik_moe_route_args *args, const float *dweights, float *dlogits);
+
+/* row_off, src and slot of ids [tokens, k] that come from elsewhere. */
+int brik_moe_sort(brik_ctx *ctx, const int32_t *ids, int tokens, int k, int experts, int32_t *row_off, int32_t *src,
+                  int32_t *slot);
+
+/* The tokens' rows to their experts: x_sorted[slot[t, j]] = weights[t, j] * x[t] (weights NULL: x[t]). Rows are `width` f32
+ * values, a multiple of 4, packed and 16-byte aligned; rows of x_sorted that no slot names are left as they are. slot: as the
+ * calls above write it, no row named twice, rows below tokens * k (others are not written). */
+int brik_moe_dispatch(brik_ctx *ctx, const float *x, const int32_t *slot, const float *weights, float *x_sorted, int tokens,
+                      int k, int width);
+
+/* And back: out[t] = res[t] + sum over j, in order, of weights[t, j] * y_sorted[slot[t, j]] over the assignments that have a
+ * row; weights NULL: 1, res NULL: 0; out may be res. What lies in other rows, and weights of assignments without one, do not
+ * reach out. With weights NULL this is the gradient of brik_moe_dispatch without weights. */
+int brik_moe_combine(brik_ctx *ctx, const float *y_sorted, const int32_t *slot, const float *weights, const float *res,
+                     float *out, int tokens, int k, int width);
+
+/* The gradient of brik_moe_combine: dy_sorted[slot[t, j]] = weights[t, j] * dout[t] and dweights[t, j] = the sum of
+ * dout[t] * y_sorted[slot[t, j]] (0 without a row). dy_sorted or dweights may be NULL; dy_sorted may be y_sorted. (res: dout.) */
+int brik_moe_combine_grad(brik_ctx *ctx, const float *dout, const float *y_sorted, const int32_t *slot, const float *weights,
+                          float *dy_sorted, float *dweights, int tokens, int k, int width);
+
+/* ---- products of 8-bit integers ---------------------------------------------------------------
+ * y = x . w^T with both operands int8 and one f32 scale per row of x (token) and per row of w (channel): the products and sums
+ * are exact int32, so y has no error but that of its scaling. Weights in this form are made by brik_quantize_i8 too, from f32
+ * (of a .brik tensor: brik_dequant_* first).
+ *
+ * brik_quantize_i8: rows of x [M, K] to codes int8 [M, K] (packed) and scales [M]. With h = x, or h = act(gate) * x in 64 bits
+ * where gate is given (act: SiLU, with BRIK_JOB_ACT_GELU tanh-GELU):
+ *   scales[m] = the f32 nearest max|h[m]| / 127,   codes = floor(h / scale + 1/2)
+ * in exact arithmetic (ties upward, as the .brik encoders), within [-127, 127]. A row whose scale would be below 2^-126 gets scale 0
+ * and codes 0; a row with a NaN or an infinity gets scale NaN and codes 0, so that its products are NaN. Rows of x and gate
+ * every *_stride values (0: packed; multiples of 4), 16-byte aligned; M below 2^22. */
+int brik_quantize_i8(brik_ctx *ctx, const float *x, int64_t x_stride, const float *gate, int64_t gate_stride, int flags,
+                     int8_t *codes, float *scales, int M, int K);
+
+/* y[m, n] = (sum_k x[m, k] * w[n, k]) * w_scales[n] * x_scales[m] (+ res[m, n]): the sum exact, rounded to f32, then two
+ * roundings, and one for res. x int8 [M, K], w int8 [N, K], 16-byte aligned; K a multiple of 32 up to BRIK_I8_K (no sum passes 31 bits);
+ * any N; res f32 [M, N] or NULL, may be y. Codes of -128 are taken as they are. N * K below 2^32. Workspace: partial sums of split
+ * K, grown on demand. */
+#define BRIK_I8_K 131040
+int brik_matmul_t_i8(brik_ctx *ctx, const int8_t *x, const float *x_scales, const int8_t *w, const float *w_scales,
+                     const float *res, float *y, int M, int K, int N);
+
+/* The same by experts, w [E, N, K], w_scales [E, N]: y_sorted[r] for the rows r of [row_off[e], row_off[e + 1]) by expert e's weight.
+ * Row r is row r of x or, with src (as brik_moe_route writes it), row src[r] / k of x: the tokens quantized once, no sorted
+ * copy of them. rows: the rows of y_sorted (and src); x has x_rows rows (src NULL: at least `rows`). row_off: as above, not
+ * decreasing; rows behind row_off[E] are left as they are, and so are rows past `rows`, and rows whose src names no row of x.
+ * The launch is sized by rows and E alone, so routing stays on the device. */
+int brik_moe_matmul_t_i8(brik_ctx *ctx, const int8_t *x, const float *x_scales, int x_rows, const int32_t *src, int k,
+                         const int32_t *row_off, const int8_t *w, const float *w_scales, float *y_sorted, int E, int rows,
+                         int K, int N);
+
 /* ---- timing and tuning -------------------------------------------------------------------
  * The reference has no kernel timing (it times whole tokens with performance.now(),
  * src/app/page.tsx:1313-1376). brik_timer_begin/end record HIP events on the context stream
@@ -482,6 +574,8 @@ int brik_timer_end(brik_ctx *ctx, float *ms);
 #define BRIK_OPT_ATTN_ROWS 8       /* attention: 0 auto, else 16, 128 or 256 rows (row x query head of a key / value head) per
                                     tile (256: as 128 where head_dim > 128) */
 #define BRIK_OPT_ATTN_SPLITS 9     /* attention: 0 auto, else every tile's keys split over so many blocks (up to 256) */
+#define BRIK_OPT_I8_KERNEL 10      /* products of 8-bit integers: 0 auto, else 1 + index of a kernel (moe_plan.h) */
+#define BRIK_OPT_I8_SPLITS 11      /* products of 8-bit integers, dense: 0 auto, else K split over so many blocks (up to 64) */
 int brik_set_option(brik_ctx *ctx, int key, int value);
 
 /* The path the last brik_matmul_t_* / brik_matmul_t_q4_noalloc / brik_moe_matmul_t_q4* call on this
@@ -498,7 +592,7 @@ int brik_last_path(const brik_ctx *ctx);
  * gemv, gemm (tiled), gemmg (expert-grouped), gemm_sk (split-K), gemm_few (few rows), gemm_frag (fragments);
  * gemv_f16w, gemm_h, gemm_f16, gemm_f16w for f16 weights (and gemm_few); gemm_conv (tap by tap), gemm or
  * gemm_sk (im2col rows), conv2d_direct for convolutions; attn_few (16 rows a tile), attn_tile4 (128), attn_tile8 (256) for the
- * own keys of an attention. A diagnostic as brik_last_path. */
+ * own keys of an attention; i8_few, i8_tile for products of 8-bit integers. A diagnostic as brik_last_path. */
 const char *brik_last_kernel(const brik_ctx *ctx);
 
 #ifdef __cplusplus
