@@ -13,6 +13,12 @@
 namespace {
 
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
+struct Yes {
+    static constexpr bool value = true;
+};
+struct No {
+    static constexpr bool value = false;
+};
 
 // Orders LDS accesses of the block; global loads stay in flight.
 __device__ __forceinline__ void lds_barrier()
@@ -48,10 +54,11 @@ __device__ __forceinline__ bool expert_tile(const brik_i8_launch& a, int tile, i
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
             const int j = tile - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l));
-            r.m0 = __builtin_amdgcn_readlane(first, l) + j * BM;
-            r.m1 = min(__builtin_amdgcn_readlane(end, l), r.m0 + BM);
-            r.w = a.w + (size_t)(base + l) * a.N * a.K;
-            r.ws = a.ws + (size_t)(base + l) * a.N;
+            const int e1 = uniform(base + l);
+            r.m0 = uniform(__builtin_amdgcn_readlane(first, l) + j * BM);
+            r.m1 = uniform(min(__builtin_amdgcn_readlane(end, l), r.m0 + BM));
+            r.w = a.w + (size_t)e1 * a.N * a.K;
+            r.ws = a.ws + (size_t)e1 * a.N;
             return true;
         }
         before += __builtin_amdgcn_readlane(sum, 63);
@@ -166,23 +173,79 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
 
 // ---- tiles -----------------------------------------------------------------------------------------
 
-// WR x WC waves, each WA x WB blocks of 32 x 32.
-template <int WR_, int WC_, int WA_, int WB_>
+// WR x WC waves, each WA x WB blocks of 32 x 32; BK of K a step, double-buffered.
+template <int WR_, int WC_, int WA_, int WB_, int BK_>
 struct I8Tile {
-    static constexpr int WR = WR_, WC = WC_, WA = WA_, WB = WB_;
+    static constexpr int WR = WR_, WC = WC_, WA = WA_, WB = WB_, BK = BK_;
     static constexpr int NT = 64 * WR * WC, BM = 32 * WR * WA, BN = 32 * WC * WB;
-    static constexpr int CX = BM * 4 / NT, CW = BN * 4 / NT;     // 16-byte chunks of a thread and step
-    static constexpr int BUF = (BM + BN) * 64;
-    static_assert(BM * 4 % NT == 0 && BN * 4 % NT == 0, "whole chunks");
+    static constexpr int CH = BK / 16, ROWS = NT / CH;           // 16-byte chunks of a row, rows that the block loads at once
+    static constexpr int CX = BM / ROWS, CW = BN / ROWS;         // chunks of a thread and step
+    static constexpr int BUF = (BM + BN) * BK, H = BK / 32;
+    static_assert(BM % ROWS == 0 && BN % ROWS == 0 && ROWS % 16 == 0 && (BK == 64 || BK == 128), "whole chunks");
+    // Chunk c of row r lies at c ^ turn(r): of a column of chunks, 8 rows meet every bank of 128 bytes once, 16 rows of 256 bytes.
+    static __device__ __forceinline__ int turn(int r) { return BK == 128 ? (r & 7) ^ ((r >> 3) & 1) : ((r >> 1) ^ (r >> 3)) & 3; }
 };
 
-// Chunk c of row r lies at c ^ turn(r): 8 rows of a column of chunks meet every bank of 128 bytes once, 16 rows of 256 bytes.
-__device__ __forceinline__ int turn(int r) { return ((r >> 1) ^ (r >> 3)) & 3; }
+// Loads past `bytes` give zeros.
+__device__ __forceinline__ brsrc_t rest_of(const int8_t* p, size_t bytes) { return make_rsrc(p, (uint32_t)min(bytes, (size_t)0xffffffffu)); }
+
+// A row of accumulators, read out of the accumulation registers here and not before (the compiler would read all of them at the
+// first use of any, and has no room for them).
+template <class T>
+__device__ __forceinline__ void in_vector_registers(i32x16_t (&acc)[T::WB])
+{
+#pragma unroll
+    for (int j = 0; j < T::WB; ++j) asm volatile("" : "+v"(acc[j]));
+}
+
+// A wave's part of the tile into y. scale, ok: of this lane's rows; at0: index of its first value; left: columns from there on.
+template <class T, bool RES>
+__device__ __forceinline__ void i8_write(const brik_i8_launch& a, i32x16_t (&acc)[T::WA][T::WB], const float (&ws)[T::WB], const float* scale,
+                                         const int* ok, size_t at0, int left, bool whole)
+{
+    // the values to add, 16 rows ahead of their use (res may be y, so no load passes a store by itself)
+    float res[2][RES ? 8 : 1][T::WB];
+    auto add = [&](int part) {
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+            const int row = 16 * part + 8 * (v >> 2) + (v & 3);
+            const float* const from = a.res + at0 + (size_t)row * a.N;
+#pragma unroll
+            for (int j = 0; j < T::WB; ++j) res[part & 1][v][j] = whole || (ok[row] && 32 * j < left) ? from[32 * j] : 0.f;
+        }
+    };
+    if constexpr (RES) add(0);
+#pragma unroll
+    for (int part = 0; part < 2 * T::WA; ++part) {
+        if constexpr (RES) {
+            if (part + 1 < 2 * T::WA) add(part + 1);
+        }
+        if (part % 2 == 0) in_vector_registers<T>(acc[part / 2]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const f32x4_t xs = *(const f32x4_t*)(scale + 16 * part + 8 * q);
+            const i32x4_t is = *(const i32x4_t*)(ok + 16 * part + 8 * q);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                float* const to = a.y + at0 + (size_t)(16 * part + 8 * q + v) * a.N;
+                const bool row = whole || is[v];
+#pragma unroll
+                for (int j = 0; j < T::WB; ++j) {
+                    float y = (float)acc[part / 2][j][8 * (part & 1) + 4 * q + v] * ws[j] * xs[v];
+                    if constexpr (RES) y += res[part & 1][4 * q + v][j];
+                    if (row && (whole || 32 * j < left)) to[32 * j] = y;
+                }
+            }
+        }
+    }
+}
 
 template <class T>
 __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
 {
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * T::BUF];
+    __shared__ __attribute__((aligned(16))) float row_scale[T::BM];
+    __shared__ __attribute__((aligned(16))) int row_ok[T::BM];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), wr = wave / T::WC, wc = wave % T::WC;
     // blocks of one XCD (every eighth) take neighbouring tiles, 8 row tiles by as many columns as fit
     const int tiles = a.row_tiles * a.col_tiles * a.splits, xcd = blockIdx.x & 7, each = tiles >> 3, more = tiles & 7;
@@ -194,56 +257,48 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
     I8Rows r{rt * T::BM, min(a.M, (rt + 1) * T::BM), a.w, a.ws};
     if (a.E && !expert_tile(a, rt, T::BM, r)) return;
     const int n0 = ct * T::BN, K = a.K;
-    const int steps = (K + 63) >> 6, s0 = split * a.steps, s1 = min(steps, s0 + a.steps);
+    const int k0 = split * a.steps * 64, k1 = min(K, k0 + a.steps * 64);
 
-    const int part = tid & 3, trow = tid >> 2;
-    const int8_t *xp[T::CX], *wp[T::CW];
+    // the scales of the tile's rows, and whether they are rows
+    for (int i = tid; i < T::BM; i += T::NT) {
+        const int from = r.m0 + i < r.m1 ? x_row(a, r.m0 + i) : -1;
+        row_ok[i] = from >= 0;
+        row_scale[i] = from >= 0 ? a.xs[from] : 0.f;
+    }
+    // A chunk past K is zeros: its offset is past any buffer. (Rows past the tile's are other rows or zeros, and not used.)
+    const int part = tid % T::CH, trow = tid / T::CH;
+    uint32_t xo[T::CX], wo[T::CW];
+    const brsrc_t rx = a.src ? rest_of(a.x, (size_t)a.x_rows * K) : rest_of(a.x + (size_t)r.m0 * K, (size_t)(a.M - r.m0) * K);
+    const brsrc_t rw = rest_of(r.w + (size_t)n0 * K, (size_t)(a.N - n0) * K);
+    int k = k0 + 16 * part;
 #pragma unroll
     for (int i = 0; i < T::CX; ++i) {
-        const int row = x_row(a, min(r.m0 + i * (T::NT / 4) + trow, r.m1 - 1));
-        xp[i] = a.x + (size_t)max(row, 0) * K + 16 * part;
+        const int m = i * T::ROWS + trow;
+        const int row = a.src ? max(x_row(a, min(r.m0 + m, r.m1 - 1)), 0) : m;
+        xo[i] = (uint32_t)row * (uint32_t)K;
     }
 #pragma unroll
-    for (int i = 0; i < T::CW; ++i) wp[i] = r.w + (size_t)min(n0 + i * (T::NT / 4) + trow, a.N - 1) * K + 16 * part;
+    for (int i = 0; i < T::CW; ++i) wo[i] = (uint32_t)(i * T::ROWS + trow) * (uint32_t)K;
 
-    i32x4_t gx[T::CX], gw[T::CW];
-    auto load = [&](int s) {
-        const int k = 64 * s;
-        if (k + 64 <= K) {
-#pragma unroll
-            for (int i = 0; i < T::CX; ++i) gx[i] = *(const i32x4_t*)(xp[i] + k);
-#pragma unroll
-            for (int i = 0; i < T::CW; ++i) gw[i] = *(const i32x4_t*)(wp[i] + k);
-        } else {
-            // half a step: zeros of x behind the row's end (of w whatever lies there in the row)
-            const bool inside = part < 2;
-            const int at = inside ? k : k - 32;
-#pragma unroll
-            for (int i = 0; i < T::CX; ++i) {
-                const i32x4_t v = *(const i32x4_t*)(xp[i] + at);
-                gx[i] = inside ? v : i32x4_t{0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int i = 0; i < T::CW; ++i) gw[i] = *(const i32x4_t*)(wp[i] + at);
-        }
+    // chunk i of the thread: of x, then of w
+    constexpr int C = T::CX + T::CW;
+    i32x4_t chunk[C];
+    auto load = [&](int i) {
+        const bool of_x = i < T::CX;
+        chunk[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                               of_x ? rx : rw, k < k1 ? (of_x ? xo[of_x ? i : 0] : wo[of_x ? 0 : i - T::CX]) + k : 0xffffffffu, 0, 0));
     };
-    const int put = trow * 64 + 16 * (part ^ turn(trow));
-    auto store = [&](int buf) {
-        unsigned char* const to = smem + buf * T::BUF + put;
-#pragma unroll
-        for (int i = 0; i < T::CX; ++i) *(i32x4_t*)(to + i * T::NT * 16) = gx[i];
-#pragma unroll
-        for (int i = 0; i < T::CW; ++i) *(i32x4_t*)(to + T::BM * 64 + i * T::NT * 16) = gw[i];
-    };
-    const int lrow = lane & 31, get = lrow * 64 + 16 * ((lane >> 5) ^ turn(lrow));
-    const int xget = get + wr * T::WA * 2048, wget = get + T::BM * 64 + wc * T::WB * 2048;
+    const int put = trow * T::BK + 16 * (part ^ T::turn(trow));
+    // (rows of w follow those of x)
+    auto store = [&](int i, int buf) { *(i32x4_t*)(smem + buf * T::BUF + put + i * T::NT * 16) = chunk[i]; };
+    const int lrow = lane & 31, get = lrow * T::BK + 16 * ((lane >> 5) ^ T::turn(lrow));
+    const int xget = get + wr * T::WA * 32 * T::BK, wget = get + T::BM * T::BK + wc * T::WB * 32 * T::BK;
     i32x4_t fx[2][T::WA], fw[2][T::WB];
-    auto fetch = [&](int buf, int h) {
+    // operand i (of w, then of x) of part h, 32 of K, of a buffer
+    auto fetch = [&](int i, int buf, int h) {
         const unsigned char* const from = smem + buf * T::BUF;
-#pragma unroll
-        for (int i = 0; i < T::WA; ++i) fx[h][i] = *(const i32x4_t*)(from + (xget ^ (32 * h)) + i * 2048);
-#pragma unroll
-        for (int j = 0; j < T::WB; ++j) fw[h][j] = *(const i32x4_t*)(from + (wget ^ (32 * h)) + j * 2048);
+        if (i < T::WB) fw[h & 1][i < T::WB ? i : 0] = *(const i32x4_t*)(from + (wget ^ (32 * h)) + i * 32 * T::BK);
+        else fx[h & 1][i < T::WB ? 0 : i - T::WB] = *(const i32x4_t*)(from + (xget ^ (32 * h)) + (i - T::WB) * 32 * T::BK);
     };
     i32x16_t acc[T::WA][T::WB];
 #pragma unroll
@@ -252,54 +307,79 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
         for (int j = 0; j < T::WB; ++j)
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
-    auto multiply = [&](int h) {
-#pragma unroll
-        for (int i = 0; i < T::WA; ++i)
-#pragma unroll
-            for (int j = 0; j < T::WB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h][i], fw[h][j], acc[i][j], 0, 0, 0);
-    };
 
-    if (s0 < s1) {
-        load(s0);
-        store(0);
-        if (s0 + 1 < s1) load(s0 + 1);
-        lds_barrier();
-        fetch(0, 0);
-        for (int s = s0; s < s1; ++s) {
-            const int buf = (s - s0) & 1;
-            fetch(buf, 1);
-            multiply(0);
-            // (the other buffer's last reads were waited for before the last barrier)
-            if (s + 1 < s1) store(buf ^ 1);
-            if (s + 2 < s1) load(s + 2);
-            lds_barrier();
-            if (s + 1 < s1) fetch(buf ^ 1, 0);
-            multiply(1);
-        }
-    }
-
-    const int h = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < T::WA; ++i)
+    for (int i = 0; i < C; ++i) load(i);
+    k += T::BK;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int m = r.m0 + 32 * (wr * T::WA + i) + 8 * (v >> 2) + 4 * h + (v & 3);
-            if (m >= r.m1) continue;
-            const int from = x_row(a, m);
-            const float xs = from < 0 || a.part ? 0.f : a.xs[from];
+    for (int i = 0; i < C; ++i) store(i, 0);
 #pragma unroll
-            for (int j = 0; j < T::WB; ++j) {
-                const int n = n0 + 32 * (wc * T::WB + j) + lrow;
-                if (n >= a.N) continue;
-                const size_t at = (size_t)m * a.N + n;
-                if (a.part) {
-                    a.part[(size_t)split * a.M * a.N + at] = acc[i][j][v];
-                } else if (from >= 0) {
-                    const float y = (float)acc[i][j][v] * r.ws[n] * xs;
-                    a.y[at] = a.res ? y + a.res[at] : y;
+    for (int i = 0; i < C; ++i) load(i);
+    k += T::BK;
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < T::WA + T::WB; ++i) fetch(i, 0, 0);
+    // A step: parts of 32 of K. Between the products of a part go the next part's operands from LDS and, in the middle parts, the next
+    // step's chunks into the other buffer, whose last readers are past the barrier, each followed by the load of the step after.
+    // The barrier before the last part ends both: the next step's first operands come from the other buffer. The order is written
+    // out and held (left to itself the compiler moves the products together and waits for every operand where it is used).
+    constexpr int P = T::WA * T::WB, OPS = T::WA + T::WB, MID = T::H == 2 ? 1 : T::H - 2, PUT = C / MID;
+    static_assert(C % MID == 0, "whole parts");
+    int buf = 0;
+    for (int at = k0; at < k1; at += T::BK) {
+#pragma unroll
+        for (int h = 0; h < T::H; ++h) {
+            const bool last = h + 1 == T::H;
+            const int mid = T::H == 2 ? h : h - 1;               // number of this middle part
+            if (last) {
+                k += T::BK;
+                lds_barrier();
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const int i = p / T::WB, j = p % T::WB;
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h & 1][i], fw[h & 1][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int o = p * OPS / P; o < (p + 1) * OPS / P; ++o) fetch(o, last ? buf ^ 1 : buf, last ? 0 : h + 1);
+                if (!last && mid >= 0 && mid < MID) {
+#pragma unroll
+                    for (int o = p * PUT / P; o < (p + 1) * PUT / P; ++o) {
+                        store(mid * PUT + o, buf ^ 1);
+                        load(mid * PUT + o);
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        buf ^= 1;
+    }
+
+    // D layout of a 32 x 32 tile: lane holds column lane & 31, register 4 q + v row 8 q + 4 (lane >> 5) + v
+    const int rel = 32 * wr * T::WA + 4 * (lane >> 5), n1 = n0 + 32 * wc * T::WB + lrow;
+    const size_t at0 = (size_t)(r.m0 + rel) * a.N + n1;
+    if (a.part) {
+        int32_t* const to = a.part + (size_t)split * a.M * a.N + at0;
+#pragma unroll
+        for (int i = 0; i < T::WA; ++i) {
+            in_vector_registers<T>(acc[i]);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int row = 32 * i + 8 * (v >> 2) + (v & 3);
+                if (r.m0 + rel + row >= r.m1) continue;
+#pragma unroll
+                for (int j = 0; j < T::WB; ++j)
+                    if (n1 + 32 * j < a.N) (to + (size_t)row * a.N)[32 * j] = acc[i][j][v];
+            }
+        }
+        return;
+    }
+    float ws[T::WB];
+#pragma unroll
+    for (int j = 0; j < T::WB; ++j) ws[j] = r.ws[min(n1 + 32 * j, a.N - 1)];
+    // whole: every value of the tile is one of y
+    const bool whole = !a.src && r.m0 + T::BM <= r.m1 && n0 + T::BN <= a.N;
+    if (a.res) i8_write<T, true>(a, acc, ws, row_scale + rel, row_ok + rel, at0, a.N - n1, whole);
+    else i8_write<T, false>(a, acc, ws, row_scale + rel, row_ok + rel, at0, a.N - n1, whole);
 }
 
 }  // namespace
@@ -313,12 +393,17 @@ BRIK_I8_FEW(1, 2, 8)
 BRIK_I8_FEW(2, 2, 8)
 BRIK_I8_FEW(4, 2, 8)
 
-#define BRIK_I8_TILE(WR, WC, WA, WB, OCC) \
-    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##WR##WC##_##WA##x##WB(brik_i8_launch a) { i8_tile<I8Tile<WR, WC, WA, WB>>(a); }
-BRIK_I8_TILE(2, 2, 4, 4, 1)
-BRIK_I8_TILE(2, 2, 4, 2, 2)
-BRIK_I8_TILE(2, 2, 2, 2, 2)
-BRIK_I8_TILE(2, 2, 1, 2, 3)
+#define BRIK_I8_TILE(WR, WC, WA, WB, BK, OCC)                                                                             \
+    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##WR##WC##_##WA##x##WB##_##BK(brik_i8_launch a) \
+    {                                                                                                                    \
+        i8_tile<I8Tile<WR, WC, WA, WB, BK>>(a);                                                                          \
+    }
+BRIK_I8_TILE(2, 2, 4, 4, 128, 1)
+BRIK_I8_TILE(2, 2, 4, 4, 64, 1)
+BRIK_I8_TILE(2, 2, 4, 2, 64, 2)
+BRIK_I8_TILE(2, 2, 2, 2, 128, 2)
+BRIK_I8_TILE(2, 2, 2, 2, 64, 3)
+BRIK_I8_TILE(2, 2, 1, 2, 128, 2)
 
 // The splits' sums and the scaling: a thread per four neighbours of y.
 extern "C" __global__ __launch_bounds__(256) void brik_i8_join(brik_i8_launch a)

@@ -91,6 +91,8 @@ inline int product_i8(Why& w, const char* who, const brik_i8_launch& a, bool moe
     if (moe) {
         if (a.E < 0 || a.E > 65536) return no(w, BRIK_EINVAL, "%s: %d experts (0 to 65536)", who, a.E);
         if (a.src && a.k < 1) return no(w, BRIK_EINVAL, "%s: src with k=%d", who, a.k);
+        if (a.src && (long long)a.x_rows * a.K >= (1ll << 32))
+            return no(w, BRIK_EINVAL, "%s: x of %d rows of %d values found by src exceeds 2^32", who, a.x_rows, a.K);
         if (a.x_rows < 0 || (!a.src && a.x_rows < a.M)) return no(w, BRIK_EINVAL, "%s: x of %d rows for %d", who, a.x_rows, a.M);
     }
     if ((long long)a.N * a.K >= (1ll << 32)) return no(w, BRIK_EINVAL, "%s: N*K = %lld exceeds the 2^32 per-tensor limit", who, (long long)a.N * a.K);

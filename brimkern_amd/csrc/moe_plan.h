@@ -32,8 +32,9 @@ struct I8Kernel {
 constexpr I8Kernel kI8Kernels[] = {
     {true, 16, 16, 512, "brik_i8_few_1_1_8"},      {true, 32, 16, 512, "brik_i8_few_2_1_8"},      {true, 64, 16, 512, "brik_i8_few_4_1_8"},
     {true, 16, 32, 512, "brik_i8_few_1_2_8"},      {true, 32, 32, 512, "brik_i8_few_2_2_8"},      {true, 64, 32, 512, "brik_i8_few_4_2_8"},
-    {false, 256, 256, 256, "brik_i8_tile_22_4x4"}, {false, 256, 128, 256, "brik_i8_tile_22_4x2"}, {false, 128, 128, 256, "brik_i8_tile_22_2x2"},
-    {false, 64, 128, 256, "brik_i8_tile_22_1x2"},
+    {false, 256, 256, 256, "brik_i8_tile_22_4x4_128"}, {false, 256, 256, 256, "brik_i8_tile_22_4x4_64"},
+    {false, 256, 128, 256, "brik_i8_tile_22_4x2_64"},  {false, 128, 128, 256, "brik_i8_tile_22_2x2_128"},
+    {false, 128, 128, 256, "brik_i8_tile_22_2x2_64"},  {false, 64, 128, 256, "brik_i8_tile_22_1x2_128"},
 };
 constexpr int kI8Count = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
 
@@ -46,8 +47,8 @@ inline int i8_plan(brik_i8_launch& a, int forced)
     if (a.K == 0) t = kI8Count - 1;                             // (a tile without steps: sums of 0)
     else if (forced) t = forced - 1;
     else if (rows <= 64) t = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
-    else if (a.E) t = 8;
-    else t = a.M >= 2048 ? 6 : 8;
+    else if (a.E) t = 9;
+    else t = a.M >= 2048 && (long)a.M * a.N >= 32l << 20 ? 6 : 9;
     const I8Kernel& g = kI8Kernels[t];
     a.col_tiles = (a.N + g.bn - 1) / g.bn;
     a.splits = 1;

@@ -8,7 +8,7 @@ from brimkern_amd.capi import BrikError, BRIK_EALIGN, BRIK_EINVAL, BRIK_I8_K, BR
 from test_gpu_moe import Dev, dev, run_route        # noqa: F401
 
 pytestmark = pytest.mark.gpu
-KERNELS = 10
+KERNELS = 12
 
 
 def run_quantize(dev, x, gate=None, gelu=False, x_stride=0, gate_stride=0, K=None):
