@@ -2816,7 +2816,7 @@ static int product_i8(brik_ctx* c, const char* who, brik_i8_launch& a, bool moe)
     }
     const long blocks = (long)a.row_tiles * a.col_tiles * a.splits;
     if (blocks >= (1l << 23)) return fail(c, BRIK_EINVAL, "%s: %ld blocks in one call", who, blocks);
-    c->last_kernel = g.few ? "i8_few" : "i8_tile";
+    c->last_kernel = g.kind == brik_plan::I8_FEW ? "i8_few" : g.kind == brik_plan::I8_TILE ? "i8_tile" : "i8_moe";
     void* args[] = {&a};
     HIP_TRY_RC(launch_fn(c, c->moe_fn[E_I8 + t], (unsigned)blocks, 1, (unsigned)g.threads, 0, args));
     if (a.splits == 1) return BRIK_OK;

@@ -181,13 +181,14 @@ struct I8Tile {
     static constexpr int CH = BK / 16, ROWS = NT / CH;           // 16-byte chunks of a row, rows that the block loads at once
     static constexpr int CX = BM / ROWS, CW = BN / ROWS;         // chunks of a thread and step
     static constexpr int BUF = (BM + BN) * BK, H = BK / 32;
-    static_assert(BM % ROWS == 0 && BN % ROWS == 0 && ROWS % 16 == 0 && (BK == 64 || BK == 128), "whole chunks");
-    // Chunk c of row r lies at c ^ turn(r): of a column of chunks, 8 rows meet every bank of 128 bytes once, 16 rows of 256 bytes.
-    static __device__ __forceinline__ int turn(int r) { return BK == 128 ? (r & 7) ^ ((r >> 3) & 1) : ((r >> 1) ^ (r >> 3)) & 3; }
+    static_assert(BM % ROWS == 0 && BN % ROWS == 0 && ROWS % 32 == 0 && (BK == 64 || BK == 128), "whole chunks");
+    // Chunk c of row r lies at c ^ turn(r): a column of chunks is read in groups of the rows 4 a .. 4 a + 3 and 4 (a ^ 5) .. 4 (a ^ 5) + 3,
+    // which then meet every bank once (no conflicts counted).
+    static __device__ __forceinline__ int turn(int r) { return BK == 128 ? (r & 7) ^ ((r >> 3) & 1) : ((r >> 1) & 1) | ((r >> 3) & 2); }
 };
 
 // Loads past `bytes` give zeros.
-__device__ __forceinline__ brsrc_t rest_of(const int8_t* p, size_t bytes) { return make_rsrc(p, (uint32_t)min(bytes, (size_t)0xffffffffu)); }
+__device__ __forceinline__ brsrc_t rest_of(const void* p, size_t bytes) { return make_rsrc(p, (uint32_t)min(bytes, (size_t)0xffffffffu)); }
 
 // A row of accumulators, read out of the accumulation registers here and not before (the compiler would read all of them at the
 // first use of any, and has no room for them).
@@ -198,27 +199,31 @@ __device__ __forceinline__ void in_vector_registers(i32x16_t (&acc)[T::WB])
     for (int j = 0; j < T::WB; ++j) asm volatile("" : "+v"(acc[j]));
 }
 
-// A wave's part of the tile into y. scale, ok: of this lane's rows; at0: index of its first value; left: columns from there on.
-template <class T, bool RES>
-__device__ __forceinline__ void i8_write(const brik_i8_launch& a, i32x16_t (&acc)[T::WA][T::WB], const float (&ws)[T::WB], const float* scale,
-                                         const int* ok, size_t at0, int left, bool whole)
+// A wave's part of the tile into y: row v of register r, column block j. Offsets from the tile's first value, past any buffer for
+// what is no value of y (no store waits for another, as it would behind branches). WHOLE: every value of the tile is one of y.
+template <class T, bool RES, bool WHOLE>
+__device__ __forceinline__ void i8_write(i32x16_t (&acc)[T::WA][T::WB], brsrc_t y, brsrc_t res, const float (&ws)[T::WB], const float* scale,
+                                         const int* ok, uint32_t at0, uint32_t pitch, int left)
 {
     // the values to add, 16 rows ahead of their use (res may be y, so no load passes a store by itself)
-    float res[2][RES ? 8 : 1][T::WB];
-    auto add = [&](int part) {
+    float add[2][RES ? 8 : 1][T::WB];
+    auto offset = [&](uint32_t row, bool is, int j) {
+        return WHOLE || (is && 32 * j < left) ? at0 + row * pitch + 128 * j : 0xffffffffu;
+    };
+    auto read = [&](int part) {
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
             const int row = 16 * part + 8 * (v >> 2) + (v & 3);
-            const float* const from = a.res + at0 + (size_t)row * a.N;
 #pragma unroll
-            for (int j = 0; j < T::WB; ++j) res[part & 1][v][j] = whole || (ok[row] && 32 * j < left) ? from[32 * j] : 0.f;
+            for (int j = 0; j < T::WB; ++j)
+                add[part & 1][v][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(res, offset(row, ok[row], j), 0, 0));
         }
     };
-    if constexpr (RES) add(0);
+    if constexpr (RES) read(0);
 #pragma unroll
     for (int part = 0; part < 2 * T::WA; ++part) {
         if constexpr (RES) {
-            if (part + 1 < 2 * T::WA) add(part + 1);
+            if (part + 1 < 2 * T::WA) read(part + 1);
         }
         if (part % 2 == 0) in_vector_registers<T>(acc[part / 2]);
 #pragma unroll
@@ -226,21 +231,19 @@ __device__ __forceinline__ void i8_write(const brik_i8_launch& a, i32x16_t (&acc
             const f32x4_t xs = *(const f32x4_t*)(scale + 16 * part + 8 * q);
             const i32x4_t is = *(const i32x4_t*)(ok + 16 * part + 8 * q);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                float* const to = a.y + at0 + (size_t)(16 * part + 8 * q + v) * a.N;
-                const bool row = whole || is[v];
+            for (int v = 0; v < 4; ++v)
 #pragma unroll
                 for (int j = 0; j < T::WB; ++j) {
-                    float y = (float)acc[part / 2][j][8 * (part & 1) + 4 * q + v] * ws[j] * xs[v];
-                    if constexpr (RES) y += res[part & 1][4 * q + v][j];
-                    if (row && (whole || 32 * j < left)) to[32 * j] = y;
+                    float val = (float)acc[part / 2][j][8 * (part & 1) + 4 * q + v] * ws[j] * xs[v];
+                    if constexpr (RES) val += add[part & 1][4 * q + v][j];
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, val), y, offset(16 * part + 8 * q + v, is[v], j), 0, 0);
                 }
-            }
         }
     }
 }
 
-template <class T>
+// MOE: by experts, the rows of x perhaps found by src; else dense, with values to add or K split.
+template <class T, bool MOE>
 __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
 {
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * T::BUF];
@@ -255,26 +258,33 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
     const int group = 8 * a.col_tiles, g = id / group, rows = min(8, a.row_tiles - 8 * g), in = id - g * group;
     const int rt = 8 * g + in % rows, ct = in / rows;
     I8Rows r{rt * T::BM, min(a.M, (rt + 1) * T::BM), a.w, a.ws};
-    if (a.E && !expert_tile(a, rt, T::BM, r)) return;
+    if (MOE && !expert_tile(a, rt, T::BM, r)) return;
     const int n0 = ct * T::BN, K = a.K;
     const int k0 = split * a.steps * 64, k1 = min(K, k0 + a.steps * 64);
 
     // the scales of the tile's rows, and whether they are rows
     for (int i = tid; i < T::BM; i += T::NT) {
-        const int from = r.m0 + i < r.m1 ? x_row(a, r.m0 + i) : -1;
+        const int from = r.m0 + i < r.m1 ? MOE ? x_row(a, r.m0 + i) : r.m0 + i : -1;
         row_ok[i] = from >= 0;
         row_scale[i] = from >= 0 ? a.xs[from] : 0.f;
     }
+    // D layout of a 32 x 32 tile: lane holds column lane & 31, register 4 q + v row 8 q + 4 (lane >> 5) + v. The columns' scales are
+    // there before the first chunk is.
+    const int lrow = lane & 31, rel = 32 * wr * T::WA + 4 * (lane >> 5), n1 = n0 + 32 * wc * T::WB + lrow;
+    const size_t first = (size_t)r.m0 * a.N + n0;
+    float ws[T::WB];
+#pragma unroll
+    for (int j = 0; j < T::WB; ++j) ws[j] = r.ws[min(n1 + 32 * j, a.N - 1)];
     // A chunk past K is zeros: its offset is past any buffer. (Rows past the tile's are other rows or zeros, and not used.)
     const int part = tid % T::CH, trow = tid / T::CH;
     uint32_t xo[T::CX], wo[T::CW];
-    const brsrc_t rx = a.src ? rest_of(a.x, (size_t)a.x_rows * K) : rest_of(a.x + (size_t)r.m0 * K, (size_t)(a.M - r.m0) * K);
+    const brsrc_t rx = MOE && a.src ? rest_of(a.x, (size_t)a.x_rows * K) : rest_of(a.x + (size_t)r.m0 * K, (size_t)(a.M - r.m0) * K);
     const brsrc_t rw = rest_of(r.w + (size_t)n0 * K, (size_t)(a.N - n0) * K);
     int k = k0 + 16 * part;
 #pragma unroll
     for (int i = 0; i < T::CX; ++i) {
         const int m = i * T::ROWS + trow;
-        const int row = a.src ? max(x_row(a, min(r.m0 + m, r.m1 - 1)), 0) : m;
+        const int row = MOE && a.src ? max(x_row(a, min(r.m0 + m, r.m1 - 1)), 0) : m;
         xo[i] = (uint32_t)row * (uint32_t)K;
     }
 #pragma unroll
@@ -291,7 +301,7 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
     const int put = trow * T::BK + 16 * (part ^ T::turn(trow));
     // (rows of w follow those of x)
     auto store = [&](int i, int buf) { *(i32x4_t*)(smem + buf * T::BUF + put + i * T::NT * 16) = chunk[i]; };
-    const int lrow = lane & 31, get = lrow * T::BK + 16 * ((lane >> 5) ^ T::turn(lrow));
+    const int get = lrow * T::BK + 16 * ((lane >> 5) ^ T::turn(lrow));
     const int xget = get + wr * T::WA * 32 * T::BK, wget = get + T::BM * T::BK + wc * T::WB * 32 * T::BK;
     i32x4_t fx[2][T::WA], fw[2][T::WB];
     // operand i (of w, then of x) of part h, 32 of K, of a buffer
@@ -354,32 +364,31 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
         buf ^= 1;
     }
 
-    // D layout of a 32 x 32 tile: lane holds column lane & 31, register 4 q + v row 8 q + 4 (lane >> 5) + v
-    const int rel = 32 * wr * T::WA + 4 * (lane >> 5), n1 = n0 + 32 * wc * T::WB + lrow;
-    const size_t at0 = (size_t)(r.m0 + rel) * a.N + n1;
-    if (a.part) {
-        int32_t* const to = a.part + (size_t)split * a.M * a.N + at0;
+    const uint32_t pitch = 4u * (uint32_t)a.N, at = (uint32_t)rel * pitch + 4u * (uint32_t)(n1 - n0);
+    if (!MOE && a.part) {
+        const brsrc_t to = rest_of(a.part + (size_t)split * a.M * a.N + first, 4 * ((size_t)a.M * a.N - first));
 #pragma unroll
         for (int i = 0; i < T::WA; ++i) {
             in_vector_registers<T>(acc[i]);
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const int row = 32 * i + 8 * (v >> 2) + (v & 3);
-                if (r.m0 + rel + row >= r.m1) continue;
 #pragma unroll
                 for (int j = 0; j < T::WB; ++j)
-                    if (n1 + 32 * j < a.N) (to + (size_t)row * a.N)[32 * j] = acc[i][j][v];
+                    __builtin_amdgcn_raw_buffer_store_b32((uint32_t)acc[i][j][v], to,
+                                                          r.m0 + rel + row < r.m1 && n1 + 32 * j < a.N ? at + row * pitch + 128 * j : 0xffffffffu, 0, 0);
             }
         }
         return;
     }
-    float ws[T::WB];
-#pragma unroll
-    for (int j = 0; j < T::WB; ++j) ws[j] = r.ws[min(n1 + 32 * j, a.N - 1)];
-    // whole: every value of the tile is one of y
-    const bool whole = !a.src && r.m0 + T::BM <= r.m1 && n0 + T::BN <= a.N;
-    if (a.res) i8_write<T, true>(a, acc, ws, row_scale + rel, row_ok + rel, at0, a.N - n1, whole);
-    else i8_write<T, false>(a, acc, ws, row_scale + rel, row_ok + rel, at0, a.N - n1, whole);
+    const brsrc_t y = rest_of(a.y + first, 4 * ((size_t)a.M * a.N - first));
+    const bool whole = !(MOE && a.src) && r.m0 + T::BM <= r.m1 && n0 + T::BN <= a.N;
+    auto write = [&](auto added, brsrc_t res) {
+        if (whole) i8_write<T, decltype(added)::value, true>(acc, y, res, ws, row_scale + rel, row_ok + rel, at, pitch, a.N - n1);
+        else i8_write<T, decltype(added)::value, false>(acc, y, res, ws, row_scale + rel, row_ok + rel, at, pitch, a.N - n1);
+    };
+    if (!MOE && a.res) write(Yes(), rest_of(a.res + first, 4 * ((size_t)a.M * a.N - first)));
+    else write(No(), y);
 }
 
 }  // namespace
@@ -393,17 +402,24 @@ BRIK_I8_FEW(1, 2, 8)
 BRIK_I8_FEW(2, 2, 8)
 BRIK_I8_FEW(4, 2, 8)
 
-#define BRIK_I8_TILE(WR, WC, WA, WB, BK, OCC)                                                                             \
-    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##WR##WC##_##WA##x##WB##_##BK(brik_i8_launch a) \
-    {                                                                                                                    \
-        i8_tile<I8Tile<WR, WC, WA, WB, BK>>(a);                                                                          \
+#define BRIK_I8_TILE(NAME, WR, WC, WA, WB, BK, OCC)                                                             \
+    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##NAME(brik_i8_launch a)         \
+    {                                                                                                           \
+        i8_tile<I8Tile<WR, WC, WA, WB, BK>, false>(a);                                                          \
     }
-BRIK_I8_TILE(2, 2, 4, 4, 128, 1)
-BRIK_I8_TILE(2, 2, 4, 4, 64, 1)
-BRIK_I8_TILE(2, 2, 4, 2, 64, 2)
-BRIK_I8_TILE(2, 2, 2, 2, 128, 2)
-BRIK_I8_TILE(2, 2, 2, 2, 64, 3)
-BRIK_I8_TILE(2, 2, 1, 2, 128, 2)
+#define BRIK_I8_MOE(NAME, WR, WC, WA, WB, BK, OCC)                                                              \
+    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_moe_##NAME(brik_i8_launch a)          \
+    {                                                                                                           \
+        i8_tile<I8Tile<WR, WC, WA, WB, BK>, true>(a);                                                           \
+    }
+BRIK_I8_TILE(256x256, 2, 2, 4, 4, 128, 1)
+BRIK_I8_TILE(256x128, 2, 2, 4, 2, 64, 2)
+BRIK_I8_TILE(128x128, 2, 2, 2, 2, 128, 2)
+BRIK_I8_TILE(64x128, 2, 2, 1, 2, 128, 3)
+BRIK_I8_MOE(256x128, 2, 2, 4, 2, 64, 2)
+BRIK_I8_MOE(128x128, 2, 2, 2, 2, 64, 4)
+BRIK_I8_MOE(128x128k, 2, 2, 2, 2, 128, 2)
+BRIK_I8_MOE(64x128, 2, 2, 1, 2, 128, 3)
 
 // The splits' sums and the scaling: a thread per four neighbours of y.
 extern "C" __global__ __launch_bounds__(256) void brik_i8_join(brik_i8_launch a)

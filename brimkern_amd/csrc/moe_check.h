@@ -96,6 +96,7 @@ inline int product_i8(Why& w, const char* who, const brik_i8_launch& a, bool moe
         if (a.x_rows < 0 || (!a.src && a.x_rows < a.M)) return no(w, BRIK_EINVAL, "%s: x of %d rows for %d", who, a.x_rows, a.M);
     }
     if ((long long)a.N * a.K >= (1ll << 32)) return no(w, BRIK_EINVAL, "%s: N*K = %lld exceeds the 2^32 per-tensor limit", who, (long long)a.N * a.K);
+    if (a.N >= 1 << 22) return no(w, BRIK_EINVAL, "%s: N=%d exceeds 2^22 - 1 channels", who, a.N);
     if (a.M == 0 || a.N == 0 || (moe && a.E == 0)) return BRIK_OK;
     if (!a.y) return no(w, BRIK_EINVAL, "%s: y is null", who);
     if (off(a.y, 4) || off(a.res, 4)) return no(w, BRIK_EALIGN, "%s: y and res must be 4-byte aligned", who);

@@ -528,7 +528,7 @@ int brik_quantize_i8(brik_ctx *ctx, const float *x, int64_t x_stride, const floa
 
 /* y[m, n] = (sum_k x[m, k] * w[n, k]) * w_scales[n] * x_scales[m] (+ res[m, n]): the sum exact, rounded to f32, then two
  * roundings, and one for res. x int8 [M, K], w int8 [N, K], 16-byte aligned; K a multiple of 32 up to BRIK_I8_K (no sum passes 31 bits);
- * any N; res f32 [M, N] or NULL, may be y. Codes of -128 are taken as they are. N * K below 2^32. Workspace: partial sums of split
+ * N below 2^22; res f32 [M, N] or NULL, may be y. Codes of -128 are taken as they are. N * K below 2^32. Workspace: partial sums of split
  * K, grown on demand. */
 #define BRIK_I8_K 131040
 int brik_matmul_t_i8(brik_ctx *ctx, const int8_t *x, const float *x_scales, const int8_t *w, const float *w_scales,
@@ -592,7 +592,8 @@ int brik_last_path(const brik_ctx *ctx);
  * gemv, gemm (tiled), gemmg (expert-grouped), gemm_sk (split-K), gemm_few (few rows), gemm_frag (fragments);
  * gemv_f16w, gemm_h, gemm_f16, gemm_f16w for f16 weights (and gemm_few); gemm_conv (tap by tap), gemm or
  * gemm_sk (im2col rows), conv2d_direct for convolutions; attn_few (16 rows a tile), attn_tile4 (128), attn_tile8 (256) for the
- * own keys of an attention; i8_few, i8_tile for products of 8-bit integers. A diagnostic as brik_last_path. */
+ * own keys of an attention; i8_few, i8_tile, i8_moe (tiles by experts) for products of
+ * 8-bit integers. A diagnostic as brik_last_path. */
 const char *brik_last_kernel(const brik_ctx *ctx);
 
 #ifdef __cplusplus
