@@ -2804,12 +2804,8 @@ static int product_i8(brik_ctx* c, const char* who, brik_i8_launch& a, bool moe)
     const int rc = brik_check::product_i8(w, who, a, moe);
     if (rc != BRIK_OK) return refuse(c, rc, w);
     if (a.M == 0 || a.N == 0 || (moe && (a.E == 0 || a.x_rows == 0))) return BRIK_OK;
-    const int t = brik_plan::i8_plan(a, c->opt_i8_kernel);
+    const int t = brik_plan::i8_plan(a, c->opt_i8_kernel, c->opt_i8_splits);
     const brik_plan::I8Kernel& g = brik_plan::kI8Kernels[t];
-    if (c->opt_i8_splits && !moe) {
-        a.steps = std::max(1, (a.steps + c->opt_i8_splits - 1) / c->opt_i8_splits);
-        a.splits = std::max(1, ((a.K + 63) / 64 + a.steps - 1) / a.steps);
-    }
     if (a.splits > 1) {
         HIP_TRY_RC(ensure_buf(c, c->iws, c->iws_bytes, 4 * (size_t)a.splits * a.M * a.N));
         a.part = static_cast<int32_t*>(c->iws);

@@ -174,9 +174,9 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
 // ---- tiles -----------------------------------------------------------------------------------------
 
 // WR x WC waves, each WA x WB blocks of 32 x 32; BK of K a step, double-buffered.
-template <int WR_, int WC_, int WA_, int WB_, int BK_>
+template <int WR_, int WC_, int WA_, int WB_, int BK_, int AHEAD_, int FD_>
 struct I8Tile {
-    static constexpr int WR = WR_, WC = WC_, WA = WA_, WB = WB_, BK = BK_;
+    static constexpr int WR = WR_, WC = WC_, WA = WA_, WB = WB_, BK = BK_, AHEAD = AHEAD_, FD = FD_;
     static constexpr int NT = 64 * WR * WC, BM = 32 * WR * WA, BN = 32 * WC * WB;
     static constexpr int CH = BK / 16, ROWS = NT / CH;           // 16-byte chunks of a row, rows that the block loads at once
     static constexpr int CX = BM / ROWS, CW = BN / ROWS;         // chunks of a thread and step
@@ -292,23 +292,25 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
 
     // chunk i of the thread: of x, then of w
     constexpr int C = T::CX + T::CW;
-    i32x4_t chunk[C];
-    auto load = [&](int i) {
+    i32x4_t chunk[T::AHEAD][C];
+    auto load = [&](int i, int set) {
         const bool of_x = i < T::CX;
-        chunk[i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+        chunk[set][i] = __builtin_bit_cast(i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
                                                of_x ? rx : rw, k < k1 ? (of_x ? xo[of_x ? i : 0] : wo[of_x ? 0 : i - T::CX]) + k : 0xffffffffu, 0, 0));
     };
     const int put = trow * T::BK + 16 * (part ^ T::turn(trow));
     // (rows of w follow those of x)
-    auto store = [&](int i, int buf) { *(i32x4_t*)(smem + buf * T::BUF + put + i * T::NT * 16) = chunk[i]; };
+    auto store = [&](int i, int buf, int set) { *(i32x4_t*)(smem + buf * T::BUF + put + i * T::NT * 16) = chunk[set][i]; };
     const int get = lrow * T::BK + 16 * ((lane >> 5) ^ T::turn(lrow));
     const int xget = get + wr * T::WA * 32 * T::BK, wget = get + T::BM * T::BK + wc * T::WB * 32 * T::BK;
-    i32x4_t fx[2][T::WA], fw[2][T::WB];
+    constexpr int NF = T::FD == 1 ? 2 : 4;                       // sets of operands
+    static_assert(T::H % NF == 0 && T::FD < T::H, "parts");
+    i32x4_t fx[NF][T::WA], fw[NF][T::WB];
     // operand i (of w, then of x) of part h, 32 of K, of a buffer
     auto fetch = [&](int i, int buf, int h) {
         const unsigned char* const from = smem + buf * T::BUF;
-        if (i < T::WB) fw[h & 1][i < T::WB ? i : 0] = *(const i32x4_t*)(from + (wget ^ (32 * h)) + i * 32 * T::BK);
-        else fx[h & 1][i < T::WB ? 0 : i - T::WB] = *(const i32x4_t*)(from + (xget ^ (32 * h)) + (i - T::WB) * 32 * T::BK);
+        if (i < T::WB) fw[h % NF][i < T::WB ? i : 0] = *(const i32x4_t*)(from + (wget ^ (32 * h)) + i * 32 * T::BK);
+        else fx[h % NF][i < T::WB ? 0 : i - T::WB] = *(const i32x4_t*)(from + (xget ^ (32 * h)) + (i - T::WB) * 32 * T::BK);
     };
     i32x16_t acc[T::WA][T::WB];
 #pragma unroll
@@ -319,52 +321,66 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
 
 #pragma unroll
-    for (int i = 0; i < C; ++i) load(i);
+    for (int i = 0; i < C; ++i) load(i, T::AHEAD - 1);
     k += T::BK;
+    if constexpr (T::AHEAD == 2) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) store(i, 0);
+        for (int i = 0; i < C; ++i) load(i, 0);
+        k += T::BK;
+    }
 #pragma unroll
-    for (int i = 0; i < C; ++i) load(i);
+    for (int i = 0; i < C; ++i) {
+        store(i, 0, T::AHEAD - 1);
+        load(i, T::AHEAD - 1);
+    }
     k += T::BK;
     lds_barrier();
 #pragma unroll
-    for (int i = 0; i < T::WA + T::WB; ++i) fetch(i, 0, 0);
+    for (int h = 0; h < T::FD; ++h)
+#pragma unroll
+        for (int i = 0; i < T::WA + T::WB; ++i) fetch(i, 0, h);
     // A step: parts of 32 of K. Between the products of a part go the next part's operands from LDS and, in the middle parts, the next
     // step's chunks into the other buffer, whose last readers are past the barrier, each followed by the load of the step after.
     // The barrier before the last part ends both: the next step's first operands come from the other buffer. The order is written
     // out and held (left to itself the compiler moves the products together and waits for every operand where it is used).
-    constexpr int P = T::WA * T::WB, OPS = T::WA + T::WB, MID = T::H == 2 ? 1 : T::H - 2, PUT = C / MID;
-    static_assert(C % MID == 0, "whole parts");
-    int buf = 0;
-    for (int at = k0; at < k1; at += T::BK) {
+    constexpr int P = T::WA * T::WB, OPS = T::WA + T::WB, MID = T::H - T::FD, SLOTS = MID * P;
+    auto step = [&](int buf, int set) {
 #pragma unroll
         for (int h = 0; h < T::H; ++h) {
-            const bool last = h + 1 == T::H;
-            const int mid = T::H == 2 ? h : h - 1;               // number of this middle part
-            if (last) {
+            const bool other = h >= MID;                         // operands of the next step from here on
+            if (h == MID) {
                 k += T::BK;
                 lds_barrier();
             }
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const int i = p / T::WB, j = p % T::WB;
-                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h & 1][i], fw[h & 1][j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h % NF][i], fw[h % NF][j], acc[i][j], 0, 0, 0);
 #pragma unroll
-                for (int o = p * OPS / P; o < (p + 1) * OPS / P; ++o) fetch(o, last ? buf ^ 1 : buf, last ? 0 : h + 1);
-                if (!last && mid >= 0 && mid < MID) {
+                for (int o = p * OPS / P; o < (p + 1) * OPS / P; ++o) fetch(o, other ? buf ^ 1 : buf, other ? h - MID : h + T::FD);
+                if (!other) {
 #pragma unroll
-                    for (int o = p * PUT / P; o < (p + 1) * PUT / P; ++o) {
-                        store(mid * PUT + o, buf ^ 1);
-                        load(mid * PUT + o);
+                    for (int o = (h * P + p) * C / SLOTS; o < (h * P + p + 1) * C / SLOTS; ++o) {
+                        store(o, buf ^ 1, set);
+                        load(o, set);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        buf ^= 1;
+    };
+    int at = k0;
+    if constexpr (T::AHEAD == 2) {
+        for (; at + T::BK < k1; at += 2 * T::BK) {
+            step(0, 0);
+            step(1, 1);
+        }
+        if (at < k1) step(0, 0);
+    } else {
+        for (int buf = 0; at < k1; at += T::BK, buf ^= 1) step(buf, 0);
     }
 
-    const uint32_t pitch = 4u * (uint32_t)a.N, at = (uint32_t)rel * pitch + 4u * (uint32_t)(n1 - n0);
+    const uint32_t pitch = 4u * (uint32_t)a.N, at0 = (uint32_t)rel * pitch + 4u * (uint32_t)(n1 - n0);
     if (!MOE && a.part) {
         const brsrc_t to = rest_of(a.part + (size_t)split * a.M * a.N + first, 4 * ((size_t)a.M * a.N - first));
 #pragma unroll
@@ -376,7 +392,7 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
 #pragma unroll
                 for (int j = 0; j < T::WB; ++j)
                     __builtin_amdgcn_raw_buffer_store_b32((uint32_t)acc[i][j][v], to,
-                                                          r.m0 + rel + row < r.m1 && n1 + 32 * j < a.N ? at + row * pitch + 128 * j : 0xffffffffu, 0, 0);
+                                                          r.m0 + rel + row < r.m1 && n1 + 32 * j < a.N ? at0 + row * pitch + 128 * j : 0xffffffffu, 0, 0);
             }
         }
         return;
@@ -384,8 +400,8 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
     const brsrc_t y = rest_of(a.y + first, 4 * ((size_t)a.M * a.N - first));
     const bool whole = !(MOE && a.src) && r.m0 + T::BM <= r.m1 && n0 + T::BN <= a.N;
     auto write = [&](auto added, brsrc_t res) {
-        if (whole) i8_write<T, decltype(added)::value, true>(acc, y, res, ws, row_scale + rel, row_ok + rel, at, pitch, a.N - n1);
-        else i8_write<T, decltype(added)::value, false>(acc, y, res, ws, row_scale + rel, row_ok + rel, at, pitch, a.N - n1);
+        if (whole) i8_write<T, decltype(added)::value, true>(acc, y, res, ws, row_scale + rel, row_ok + rel, at0, pitch, a.N - n1);
+        else i8_write<T, decltype(added)::value, false>(acc, y, res, ws, row_scale + rel, row_ok + rel, at0, pitch, a.N - n1);
     };
     if (!MOE && a.res) write(Yes(), rest_of(a.res + first, 4 * ((size_t)a.M * a.N - first)));
     else write(No(), y);
@@ -395,31 +411,29 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
 
 #define BRIK_I8_FEW(MB, CB, NW) \
     extern "C" __global__ __launch_bounds__(64 * NW) void brik_i8_few_##MB##_##CB##_##NW(brik_i8_launch a) { i8_few<MB, CB, NW>(a); }
+BRIK_I8_FEW(1, 1, 4)
 BRIK_I8_FEW(1, 1, 8)
 BRIK_I8_FEW(2, 1, 8)
-BRIK_I8_FEW(4, 1, 8)
-BRIK_I8_FEW(1, 2, 8)
-BRIK_I8_FEW(2, 2, 8)
-BRIK_I8_FEW(4, 2, 8)
+BRIK_I8_FEW(1, 1, 16)
+BRIK_I8_FEW(2, 1, 16)
 
-#define BRIK_I8_TILE(NAME, WR, WC, WA, WB, BK, OCC)                                                             \
+#define BRIK_I8_TILE(NAME, WR, WC, WA, WB, BK, AHEAD, FD, OCC)                                                  \
     extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##NAME(brik_i8_launch a)         \
     {                                                                                                           \
-        i8_tile<I8Tile<WR, WC, WA, WB, BK>, false>(a);                                                          \
+        i8_tile<I8Tile<WR, WC, WA, WB, BK, AHEAD, FD>, false>(a);                                               \
     }
-#define BRIK_I8_MOE(NAME, WR, WC, WA, WB, BK, OCC)                                                              \
+#define BRIK_I8_MOE(NAME, WR, WC, WA, WB, BK, AHEAD, FD, OCC)                                                   \
     extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_moe_##NAME(brik_i8_launch a)          \
     {                                                                                                           \
-        i8_tile<I8Tile<WR, WC, WA, WB, BK>, true>(a);                                                           \
+        i8_tile<I8Tile<WR, WC, WA, WB, BK, AHEAD, FD>, true>(a);                                                \
     }
-BRIK_I8_TILE(256x256, 2, 2, 4, 4, 128, 1)
-BRIK_I8_TILE(256x128, 2, 2, 4, 2, 64, 2)
-BRIK_I8_TILE(128x128, 2, 2, 2, 2, 128, 2)
-BRIK_I8_TILE(64x128, 2, 2, 1, 2, 128, 3)
-BRIK_I8_MOE(256x128, 2, 2, 4, 2, 64, 2)
-BRIK_I8_MOE(128x128, 2, 2, 2, 2, 64, 4)
-BRIK_I8_MOE(128x128k, 2, 2, 2, 2, 128, 2)
-BRIK_I8_MOE(64x128, 2, 2, 1, 2, 128, 3)
+BRIK_I8_TILE(256x256, 2, 2, 4, 4, 128, 1, 1, 1)
+BRIK_I8_TILE(256x128, 2, 2, 4, 2, 128, 2, 2, 1)
+BRIK_I8_TILE(128x128, 2, 2, 2, 2, 128, 2, 2, 2)
+BRIK_I8_TILE(64x128, 2, 2, 1, 2, 128, 2, 2, 2)
+BRIK_I8_MOE(256x256, 2, 2, 4, 4, 128, 1, 1, 1)
+BRIK_I8_MOE(128x128, 2, 2, 2, 2, 128, 2, 2, 2)
+BRIK_I8_MOE(64x128, 2, 2, 1, 2, 128, 2, 2, 3)
 
 // The splits' sums and the scaling: a thread per four neighbours of y.
 extern "C" __global__ __launch_bounds__(256) void brik_i8_join(brik_i8_launch a)

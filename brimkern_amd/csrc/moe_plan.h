@@ -4,6 +4,7 @@
 #include "kernels/moe_abi.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace brik_plan {
 
@@ -23,8 +24,7 @@ inline int moe_lanes(int E)
     return v;
 }
 
-// Kernels of the 8-bit product: few rows (16 rows x 1, 2, 4 at once, by 16 x 1, 2 channels), tiles of dense products, tiles by
-// experts.
+// Kernels of the 8-bit product: few rows (16 rows x 1 or 2 at once, 16 channels a block), tiles of dense products, tiles by experts.
 enum I8Kind { I8_FEW, I8_TILE, I8_MOE };
 struct I8Kernel {
     I8Kind kind;
@@ -32,33 +32,96 @@ struct I8Kernel {
     const char* name;
 };
 constexpr I8Kernel kI8Kernels[] = {
-    {I8_FEW, 16, 16, 512, "brik_i8_few_1_1_8"},        {I8_FEW, 32, 16, 512, "brik_i8_few_2_1_8"},
-    {I8_FEW, 64, 16, 512, "brik_i8_few_4_1_8"},        {I8_FEW, 16, 32, 512, "brik_i8_few_1_2_8"},
-    {I8_FEW, 32, 32, 512, "brik_i8_few_2_2_8"},        {I8_FEW, 64, 32, 512, "brik_i8_few_4_2_8"},
-    {I8_TILE, 256, 256, 256, "brik_i8_tile_256x256"},  {I8_TILE, 256, 128, 256, "brik_i8_tile_256x128"},
-    {I8_TILE, 128, 128, 256, "brik_i8_tile_128x128"},  {I8_TILE, 64, 128, 256, "brik_i8_tile_64x128"},
-    {I8_MOE, 256, 128, 256, "brik_i8_moe_256x128"},    {I8_MOE, 128, 128, 256, "brik_i8_moe_128x128"},
-    {I8_MOE, 128, 128, 256, "brik_i8_moe_128x128k"},   {I8_MOE, 64, 128, 256, "brik_i8_moe_64x128"},
+    {I8_FEW, 16, 16, 256, "brik_i8_few_1_1_4"},       {I8_FEW, 16, 16, 512, "brik_i8_few_1_1_8"},
+    {I8_FEW, 32, 16, 512, "brik_i8_few_2_1_8"},       {I8_FEW, 16, 16, 1024, "brik_i8_few_1_1_16"},
+    {I8_FEW, 32, 16, 1024, "brik_i8_few_2_1_16"},     {I8_TILE, 256, 256, 256, "brik_i8_tile_256x256"},
+    {I8_TILE, 256, 128, 256, "brik_i8_tile_256x128"}, {I8_TILE, 128, 128, 256, "brik_i8_tile_128x128"},
+    {I8_TILE, 64, 128, 256, "brik_i8_tile_64x128"},   {I8_MOE, 256, 256, 256, "brik_i8_moe_256x256"},
+    {I8_MOE, 128, 128, 256, "brik_i8_moe_128x128"},   {I8_MOE, 64, 128, 256, "brik_i8_moe_64x128"},
 };
 constexpr int kI8Count = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
+constexpr int kI8Few = 0, kI8Tiles = 5, kI8Moe = 9;
 
-// The kernel of a call, and its grid in `a`. forced: 0, or 1 + index of a kernel (one of the other kind's tiles: as 0).
-inline int i8_plan(brik_i8_launch& a, int forced)
+// A tile's times, fitted to measurements (us): `start` for a block, then for a step of 128 of K from `alone`, where few blocks run, to
+// `full` with one on every CU (the matrix cores' clock falls under load), and `two` where CUs have two, which share its paths.
+struct I8Times {
+    double start, alone, full, two;
+    bool square;                 // how the step's time grows with the blocks
+};
+constexpr I8Times kI8Times[4] = {{11.6, 1.0, 1.7, 0, true}, {7.1, 0.61, 1.1, 0, false}, {4.6, 0.37, 0.74, 1.3, false}, {3.7, 0.27, 0.52, 0.92, true}};
+constexpr int kI8CUs = 256;
+
+inline double i8_tile_us(const I8Times& t, double blocks, double steps)
 {
-    int t;
-    const long rows = a.E ? (a.M + a.E - 1) / a.E : a.M;       // of an expert, in the mean
-    const I8Kind other = a.E ? I8_TILE : I8_MOE;
-    if (a.K == 0) t = a.E ? 13 : 9;                             // (a tile without steps: sums of 0)
-    else if (forced && kI8Kernels[forced - 1].kind != other) t = forced - 1;
-    else if (a.E) t = rows <= 8 ? 0 : rows <= 64 ? 13 : 11;
-    else if (rows <= 64) t = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
-    else t = a.M >= 2048 && (long)a.M * a.N >= 32l << 20 ? 6 : 8;
-    const I8Kernel& g = kI8Kernels[t];
-    a.col_tiles = (a.N + g.bn - 1) / g.bn;
+    const double slots = t.two > 0 ? 2 * kI8CUs : kI8CUs, rounds = std::floor(blocks / slots), rest = blocks - rounds * slots, x = rest / kI8CUs;
+    const double last = rest == 0 ? 0 : x > 1 ? t.two : t.alone + (t.full - t.alone) * (t.square ? x * x : x);
+    return t.start + steps * (rounds * (t.two > 0 ? t.two : t.full) + last);
+}
+
+// Up to 64 rows by the few-row kernel: its launch, the waves' steps of 64 of K, w from memory, x from the L2 for every block, and more
+// waves than the device holds.
+inline double i8_few_us(long M, long K, long N, int waves)
+{
+    const long steps = (K + 63) / 64, blocks = (N + 15) / 16;
+    return 2.9 + 0.28 * ((steps + waves - 1) / waves) + N * (double)K / 7e6 + (double)M * K * blocks / 11e6 + (M > 16 ? 0.8 * ((M - 1) / 16) : 0) +
+           (blocks * waves > 32 * kI8CUs ? 2 : 0);
+}
+
+// The kernel of a dense product and the splits of its K, by these times. What it weighs (us): 1 x 2560 x 9728 few 7.7, tiles 9.1; 1 x
+// 9728 x 2560 few by 16 waves 9.7, by 8 11.1, tiles 23.7, in 8 splits 11.5; 64 x 2560 x 9728 few 20, 64 x 128 tiles 9.6; 128 x 9728 x
+// 2560 64 x 128 tiles 23.5, in 4 splits 13.2; 512 x 2560 x 9728 256 x 128 25, 128 x 128 30, 256 x 256 35; 1536 rows of it 54, 57, 45.
+inline int i8_dense(brik_i8_launch& a, int forced, int splits)
+{
+    const long M = a.M, K = a.K, N = a.N, steps = (K + 127) / 128;
+    int best = -1, best_splits = 1;
+    double us = 1e30;
+    for (int t = 0; t < kI8Moe; ++t) {
+        const I8Kernel& g = kI8Kernels[t];
+        if (forced ? t != forced - 1 : t == kI8Few || (g.kind == I8_FEW && (M > 64 || (M > 16) != (g.bm > 16)))) continue;
+        for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (splits) s = splits;
+            else if (s > 1 && (g.kind == I8_FEW || steps < 4 * s)) break;
+            const double tiles = (double)((M + g.bm - 1) / g.bm) * ((N + g.bn - 1) / g.bn);
+            double x = g.kind == I8_FEW ? i8_few_us(M, K, N, g.threads / 64) : i8_tile_us(kI8Times[t - kI8Tiles], tiles * s, (double)((steps + s - 1) / s));
+            if (s > 1) x += 2 + 0.45 * s + 8.0 * s * M * N / 5e6;        // the sums written and read again by a launch of its own
+            if (x < us) {
+                us = x;
+                best = t;
+                best_splits = s;
+            }
+            if (splits) break;
+        }
+    }
+    const long each = ((K + 63) / 64 + best_splits - 1) / best_splits;
+    a.steps = (int)std::max(1l, best_splits > 1 ? (each + 1) / 2 * 2 : each);        // whole steps of 128
+    a.splits = (int)std::max(1l, ((K + 63) / 64 + a.steps - 1) / a.steps);
+    return best;
+}
+
+// The kernel of a product by experts, by the mean of their rows. 64 experts, 8 a token, 2048 x 1536 and 768 x 2048 (us): 8 tokens few
+// 31 and 16, 64-row tiles 37 and 22, 128-row 44 and 28; 32 tokens 41 and 25, 40 and 25, 48 and 32; 256 tokens 66 and 38 (128 tokens),
+// 50 and 29, 52 and 35; 1024 tokens 79 and 55 by 64 rows, 78 and 57 by 128;
+// 8192 tokens by 2048 x 1536 374 by 64, 332 by 128, 322 by 256.
+inline int i8_experts(brik_i8_launch& a, int forced)
+{
     a.splits = 1;
     a.steps = (a.K + 63) / 64;
+    if (forced && kI8Kernels[forced - 1].kind != I8_TILE) return forced - 1;
+    const long rows = ((long)a.M + a.E - 1) / a.E;
+    if (rows <= 2) return a.K <= 2048 ? 0 : a.K <= 4096 ? 1 : 3;
+    return rows <= 160 ? kI8Moe + 2 : rows <= 768 || a.K < 1024 ? kI8Moe + 1 : kI8Moe;
+}
+
+// The kernel of a call, and its grid in `a`. forced: 0, or 1 + index of a kernel (a tile of the other kind: 0).
+inline int i8_plan(brik_i8_launch& a, int forced, int splits)
+{
+    if (a.K == 0) forced = a.E ? kI8Moe + 3 : kI8Tiles + 4, splits = 1;      // (a tile without steps: sums of 0)
+    if (!a.E && forced > kI8Moe) forced = 0;
+    const int t = a.E ? i8_experts(a, forced) : i8_dense(a, forced, splits);
+    const I8Kernel& g = kI8Kernels[t];
+    a.col_tiles = (a.N + g.bn - 1) / g.bn;
     if (g.kind == I8_FEW) a.row_tiles = std::max(1, a.E);
-    else a.row_tiles = (int)((a.M + g.bm - 1) / g.bm + (a.E ? std::min(a.E, a.M) : 0));
+    else a.row_tiles = (int)(((long)a.M + g.bm - 1) / g.bm + (a.E ? std::min(a.E, a.M) : 0));
     return t;
 }
 

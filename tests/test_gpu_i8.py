@@ -8,7 +8,7 @@ from brimkern_amd.capi import BrikError, BRIK_EALIGN, BRIK_EINVAL, BRIK_I8_K, BR
 from test_gpu_moe import Dev, dev, run_route        # noqa: F401
 
 pytestmark = pytest.mark.gpu
-KERNELS = 14
+KERNELS = 12
 
 
 def run_quantize(dev, x, gate=None, gelu=False, x_stride=0, gate_stride=0, K=None):
@@ -221,7 +221,7 @@ def test_malformed_offsets_stay_inside(dev):
     rng, E, rows, K, N = np.random.default_rng(4), 4, 40, 64, 32
     x, xs, w, ws = (rng.integers(-128, 128, (rows, K)).astype(np.int8), np.ones(rows, np.float32), rng.integers(-128, 128, (E, N, K)).astype(np.int8),
                     np.ones((E, N), np.float32))
-    for kernel in (1, 13):
+    for kernel in (1, 10, 12):
         y = dev.full((rows + 8, N), 7.0)
         dev.ctx.set_option(BRIK_OPT_I8_KERNEL, kernel)
         try:
