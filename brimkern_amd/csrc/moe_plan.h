@@ -42,20 +42,20 @@ constexpr I8Kernel kI8Kernels[] = {
 constexpr int kI8Count = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
 constexpr int kI8Few = 0, kI8Tiles = 5, kI8Moe = 9;
 
-// A tile's times, fitted to measurements (us): `start` for a block, then for a step of 128 of K from `alone`, where few blocks run, to
+// A tile's times, fitted to measurements (us): `start` for a block (twice where a CU has two), then for a step of 128 of K from `alone`, where few blocks run, to
 // `full` with one on every CU (the matrix cores' clock falls under load), and `two` where CUs have two, which share its paths.
 struct I8Times {
     double start, alone, full, two;
     bool square;                 // how the step's time grows with the blocks
 };
-constexpr I8Times kI8Times[4] = {{11.6, 1.0, 1.7, 0, true}, {7.1, 0.61, 1.1, 0, false}, {4.6, 0.37, 0.74, 1.3, false}, {3.7, 0.27, 0.52, 0.92, true}};
+constexpr I8Times kI8Times[4] = {{11.6, 1.0, 1.7, 0, true}, {7.1, 0.61, 1.0, 0, false}, {4.6, 0.37, 0.66, 0.95, false}, {3.7, 0.27, 0.45, 0.64, true}};
 constexpr int kI8CUs = 256;
 
 inline double i8_tile_us(const I8Times& t, double blocks, double steps)
 {
     const double slots = t.two > 0 ? 2 * kI8CUs : kI8CUs, rounds = std::floor(blocks / slots), rest = blocks - rounds * slots, x = rest / kI8CUs;
-    const double last = rest == 0 ? 0 : x > 1 ? t.two : t.alone + (t.full - t.alone) * (t.square ? x * x : x);
-    return t.start + steps * (rounds * (t.two > 0 ? t.two : t.full) + last);
+    const double whole = t.two > 0 ? 2 * t.start + steps * t.two : t.start + steps * t.full;
+    return rounds * whole + (rest == 0 ? 0 : x > 1 ? whole : t.start + steps * (t.alone + (t.full - t.alone) * (t.square ? x * x : x)));
 }
 
 // Up to 64 rows by the few-row kernel: its launch, the waves' steps of 64 of K, w from memory, x from the L2 for every block, and more
