@@ -65,10 +65,10 @@ const char* const kKernelNames[K_COUNT] = {
 enum AttnKern { A_ROWS, A_READ = A_ROWS + 12, A_FEW = A_READ + 2, A_TILE4 = A_FEW + 10, A_TILE8 = A_TILE4 + 10, A_JOIN = A_TILE8 + 10, A_JOIN_FEW, A_COUNT };
 constexpr int kAttnDims[5] = {64, 96, 128, 192, 256};
 
-// Kernels of the experts' code object: routing of 1, 2, 4, 8, 16 experts a lane (brik_route_<n>, _bias_<n>, _grad_<n>), then the
-// others by name; quantization without and with a gate by a wave, 256 and 1024 threads a row.
+// Kernels of the experts' code object: routing by teams of 16 lanes and by waves, 1, 2, 4, 8, 16 experts a lane (brik_route_<lanes>_<n>,
+// _bias_<lanes>_<n>), its gradient (brik_route_grad_<n>), then the others by name; quantization without and with a gate by a wave, 256 and 1024 threads a row.
 enum MoeKern {
-    E_ROUTE, E_BIAS = E_ROUTE + 5, E_GRAD = E_BIAS + 5, E_COUNT_IDS = E_GRAD + 5, E_SORT, E_DISPATCH, E_COMBINE, E_COMBINE_GRAD,
+    E_ROUTE, E_BIAS = E_ROUTE + 10, E_GRAD = E_BIAS + 10, E_COUNT_IDS = E_GRAD + 5, E_SORT, E_DISPATCH, E_COMBINE, E_COMBINE_GRAD,
     E_QUANT, E_I8_JOIN = E_QUANT + 6, E_I8, E_COUNT = E_I8 + brik_plan::kI8Count
 };
 
@@ -1475,10 +1475,10 @@ int brik_create(int device, brik_ctx** out)
     if (hipModuleLoadData(&c->moe_module, brik_moe_hsaco_begin) != hipSuccess) return bail(BRIK_EMODULE);
     for (int k = 0; k < E_COUNT; ++k) {
         char name[64];
-        const char* const route[3] = {"", "bias_", "grad_"};
         const char* const others[] = {"brik_route_count", "brik_route_sort", "brik_rows_dispatch", "brik_rows_combine", "brik_rows_combine_grad"};
         const char* const quant[3] = {"wave", "256", "1024"};
-        if (k < E_COUNT_IDS) snprintf(name, sizeof name, "brik_route_%s%d", route[k / 5], 1 << k % 5);
+        if (k < E_GRAD) snprintf(name, sizeof name, "brik_route_%s%d_%d", k < E_BIAS ? "" : "bias_", k % 10 < 5 ? 16 : 64, 1 << k % 5);
+        else if (k < E_COUNT_IDS) snprintf(name, sizeof name, "brik_route_grad_%d", 1 << (k - E_GRAD));
         else if (k < E_QUANT) snprintf(name, sizeof name, "%s", others[k - E_COUNT_IDS]);
         else if (k < E_I8_JOIN) snprintf(name, sizeof name, "brik_quant_i8_%s%s", k - E_QUANT >= 3 ? "glu_" : "", quant[(k - E_QUANT) % 3]);
         else snprintf(name, sizeof name, "%s", k == E_I8_JOIN ? "brik_i8_join" : brik_plan::kI8Kernels[k - E_I8].name);
@@ -2652,7 +2652,7 @@ int brik_moe_route(brik_ctx* c, const brik_moe_route_args* args)
     brik_plan::moe_chunks(a, sorted ? kRouteAlone : 0);
     if (sorted && a.chunks > 1) HIP_TRY_RC(take_counts(c, a));
     void* route[] = {&a};
-    HIP_TRY_RC(launch_fn(c, c->moe_fn[(a.r.bias ? E_BIAS : E_ROUTE) + brik_plan::moe_lanes(a.r.experts)], (unsigned)a.chunks, 1, 1024, 0, route));
+    HIP_TRY_RC(launch_fn(c, c->moe_fn[(a.r.bias ? E_BIAS : E_ROUTE) + brik_plan::moe_route(a.r.experts, a.r.k)], (unsigned)a.chunks, 1, 1024, 0, route));
     return sorted && a.chunks > 1 ? launch_fn(c, c->moe_fn[E_SORT], (unsigned)a.chunks, 1, 1024, 0, route) : BRIK_OK;
 }
 
@@ -2669,7 +2669,7 @@ int brik_moe_route_grad(brik_ctx* c, const brik_moe_route_args* args, const floa
     if (!dlogits || (!dweights && a.r.k > 0)) return fail(c, BRIK_EINVAL, "moe_route_grad: dweights or dlogits is null");
     if (!aligned(dweights, 4) || !aligned(dlogits, 4)) return fail(c, BRIK_EALIGN, "moe_route_grad: dweights and dlogits must be 4-byte aligned");
     void* grad[] = {&a, &dweights, &dlogits};
-    return launch_fn(c, c->moe_fn[E_GRAD + brik_plan::moe_lanes(a.r.experts)], (unsigned)((a.r.tokens + 3) / 4), 1, 256, 0, grad);
+    return launch_fn(c, c->moe_fn[E_GRAD + brik_plan::moe_lanes(a.r.experts, 64)], (unsigned)((a.r.tokens + 3) / 4), 1, 256, 0, grad);
 }
 
 int brik_moe_sort(brik_ctx* c, const int32_t* ids, int tokens, int k, int experts, int32_t* row_off, int32_t* src, int32_t* slot)

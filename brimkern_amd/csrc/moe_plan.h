@@ -12,17 +12,20 @@ namespace brik_plan {
 inline void moe_chunks(brik_route_launch& a, int alone)
 {
     const long n = (long)a.r.tokens * a.r.k;
-    a.chunk = n <= alone ? std::max(1, a.r.tokens) : (int)std::max(16l, ((long)a.r.tokens + BRIK_MOE_CHUNKS - 1) / BRIK_MOE_CHUNKS);
+    a.chunk = n <= alone ? std::max(1, a.r.tokens) : (int)std::max(64l, ((long)a.r.tokens + BRIK_MOE_CHUNKS - 1) / BRIK_MOE_CHUNKS);
     a.chunks = (a.r.tokens + a.chunk - 1) / a.chunk;
 }
 
-// Index of a kernel among those of 1, 2, 4, 8 and 16 experts a lane.
-inline int moe_lanes(int E)
+// Index of a kernel among those of 1, 2, 4, 8 and 16 experts a lane of a team of `lanes`.
+inline int moe_lanes(int E, int lanes)
 {
     int v = 0;
-    while ((64 << v) < E) ++v;
+    while ((lanes << v) < E) ++v;
     return v;
 }
+
+// Index of a routing kernel: by teams of 16 lanes, then by whole waves.
+inline int moe_route(int E, int k) { return E <= 256 && k <= 16 ? moe_lanes(E, 16) : 5 + moe_lanes(E, 64); }
 
 // Kernels of the 8-bit product: few rows (16 rows x 1 or 2 at once, 16 channels a block), tiles of dense products, tiles by experts.
 enum I8Kind { I8_FEW, I8_TILE, I8_MOE };
