@@ -7,7 +7,8 @@
 2. ``csrc/brik_scratch.hip`` -> ``_build/brik_scratch.o`` (hipcc -c: the no-allocation scratch array)
 3. ``csrc/brik_runtime.cpp`` + ``csrc/brik_embed.S`` (embeds the code objects) + that object ->
    ``libbrik.so`` (the C ABI declared in ``include/brik.h``)
-4. ``csrc/brik_napi.cc`` -> ``js/brik.node`` (Node N-API addon over libbrik.so, rpath $ORIGIN/..)
+4. ``csrc/brik_napi.cc`` -> ``js/brik.node`` (Node N-API addon over libbrik.so, rpath $ORIGIN/..), and
+   ``csrc/brik_napi_experts.cc`` -> ``js/brik_experts.node`` (experts, 8-bit products)
 5. ``tests/native/host_sanitize.cpp`` and ``attn_sanitize.cpp`` + the runtime sources, host code built with AddressSanitizer
    and UndefinedBehaviorSanitizer -> ``tests/native/host_sanitize``, ``attn_sanitize`` (test drivers, not part of the
    library; skipped when g++ cannot link the sanitizer runtimes)
@@ -35,6 +36,7 @@ HSACO_DEFINES = [f'-DBRIK_HSACO_PATH="{HSACO}"', f'-DBRIK_ATTN_HSACO_PATH="{ATTN
 SCRATCH_OBJ = os.path.join(BUILD, "brik_scratch.o")
 LIB = os.path.join(PKG, "libbrik.so")
 ADDON = os.path.join(PKG, "js", "brik.node")
+EXPERTS_ADDON = os.path.join(PKG, "js", "brik_experts.node")
 SANITIZE_BINS = [os.path.join(ROOT, "tests", "native", n) for n in ("host_sanitize", "attn_sanitize")]
 
 # Device flags. packed-fp32-ops is switched off: the compiler would otherwise fuse pairs of f32
@@ -100,16 +102,20 @@ def build_lib(verbose=False):
     return LIB
 
 
-def build_addon(verbose=False):
-    src = os.path.join(CSRC, "brik_napi.cc")
+def build_addons(verbose=False):
+    return [_build_addon(*a, verbose) for a in (("brik_napi.cc", ADDON), ("brik_napi_experts.cc", EXPERTS_ADDON))]
+
+
+def _build_addon(name, out, verbose):
+    src = os.path.join(CSRC, name)
     if not os.path.exists(src) or not os.path.exists(os.path.join(NODE_INC, "node_api.h")):
         return None
-    tmp = ADDON + ".tmp"
-    _run(["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", "-Wextra", "-DNODE_GYP_MODULE_NAME=brik",
+    tmp = out + ".tmp"
+    _run(["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", "-Wextra", f"-DNODE_GYP_MODULE_NAME={os.path.basename(out)[:-5]}",
           "-I", NODE_INC, "-I", os.path.join(ROOT, "include"), src,
           "-L", PKG, "-lbrik", "-Wl,-rpath,$ORIGIN/..", "-o", tmp], verbose)
-    os.replace(tmp, ADDON)
-    return ADDON
+    os.replace(tmp, out)
+    return out
 
 
 def build_host_sanitize(verbose=False):
@@ -156,7 +162,7 @@ def build(verbose=False):
             job.result()
     check_hsaco(verbose)
     build_lib(verbose)
-    build_addon(verbose)
+    build_addons(verbose)
     build_host_sanitize(verbose)
 
 

@@ -29,6 +29,10 @@ q8 / q4 weight                                                                  
 rope, quantize_kv and the  :meth:`Engine.kv_cache`, :meth:`Engine.qk_norm_rope`,   shaders.ts:1361, 1673
 attention over the         :meth:`Engine.kv_write`, :meth:`Engine.kv_read`,
 quantized cache            :meth:`Engine.attention` (device resident)
+(none)                     :meth:`Engine.moe_route` ... :meth:`Engine.moe_combine`
+                           (experts), :meth:`Engine.quantize_i8`,
+                           :meth:`Engine.mm_i8`, :meth:`Engine.moe_mm_i8` (8-bit
+                           integer products); device resident
 .brik container            :mod:`brimkern_amd.container`,                        container.ts:30-87
                            :meth:`Engine.weight_from_container`
 =========================  ===================================================  ==================
@@ -54,6 +58,11 @@ class QWeight(dict):
     @property
     def fmt(self) -> str:
         return "q3" if self.get("q3") else "q4" if "nib" in self else "q8"
+
+
+class I8Rows(dict):
+    """Rows of int8 codes with an f32 scale each, ``{i8, isc}`` of device addresses: an activation, or a weight of as many channels
+    (:meth:`Engine.quantize_i8`). Keys of its own: no product of .brik planes takes it for one of theirs."""
 
 
 class Engine:
@@ -309,6 +318,70 @@ class Engine:
                 self.ctx.free(y)
             raise
         return y
+
+    # ---- experts ---------------------------------------------------------------------------
+    def moe_route(self, logits, tokens: int, experts: int, k: int, **how) -> dict:
+        """The routing of a step (:meth:`Context.moe_route_args` for ``how``) into buffers of its own, sorted: ``ids``, ``weights``,
+        ``row_off``, ``src``, ``slot`` and the arguments of the call, ``args``, for further steps. :meth:`free_routing` frees it."""
+        sizes = {"ids": tokens * k, "weights": tokens * k, "row_off": experts + 1, "src": tokens * k, "slot": tokens * k}
+        at, total = {}, 0
+        for name, n in sizes.items():
+            at[name], total = total, total + (4 * max(n, 0) + 15) // 16 * 16
+        buf = self.ctx.alloc(max(total, 16))
+        r = {name: buf.offset(o) for name, o in at.items()}
+        r["args"] = self.ctx.moe_route_args(logits, tokens, experts, k, **r, **how)
+        try:
+            self.ctx.moe_route(r["args"])
+        except BrikError:
+            self.ctx.free(buf)
+            raise
+        r["_buf"] = buf
+        return r
+
+    def free_routing(self, routing: dict):
+        self.ctx.free(routing["_buf"])
+
+    def moe_dispatch(self, x, slot, x_sorted, tokens, k, width, weights=None):
+        """The tokens' rows to their experts' rows."""
+        self.ctx.moe_dispatch(x, slot, weights, x_sorted, tokens, k, width)
+
+    def moe_combine(self, y_sorted, slot, weights, out, tokens, k, width, res=None):
+        """The experts' rows back to the tokens, weighted, summed and added to ``res``."""
+        self.ctx.moe_combine(y_sorted, slot, weights, res, out, tokens, k, width)
+
+    # ---- products of 8-bit integers ----------------------------------------------------------
+    def quantize_i8(self, x, M: int, K: int, out: I8Rows | None = None, **how) -> I8Rows:
+        """Rows ``x`` [M, K] (device f32), or act(gate) * x, to a handle ``{i8, isc}`` of int8 codes and row scales: an activation,
+        or a weight of M channels. ``how``: :meth:`Context.quantize_i8`'s ``gate``, strides, ``gelu``."""
+        h = out
+        if h is None:
+            if M < 0 or K < 0:
+                raise BrikError(BRIK_EINVAL, f"quantize_i8: negative shape M={M} K={K}")
+            at = (M * K + 15) // 16 * 16
+            buf = self.ctx.alloc(max(at + 4 * M, 16))
+            h = I8Rows(i8=buf.offset(0), isc=buf.offset(at), _buf=buf)
+        try:
+            self.ctx.quantize_i8(x, h["i8"], h["isc"], M, K, **how)
+        except BrikError:
+            if out is None:
+                self.ctx.free(h["_buf"])
+            raise
+        return h
+
+    def mm_i8(self, x: I8Rows, w: I8Rows, m: int, k: int, n: int, out=None, res=None) -> DeviceBuffer:
+        """``x . w^T`` of two handles of :meth:`quantize_i8`, plus ``res``."""
+        y = self.ctx.alloc(max(m * n, 1) * 4) if out is None else out
+        try:
+            self.ctx.matmul_t_i8(x["i8"], x["isc"], w["i8"], w["isc"], y, m, k, n, res=res)
+        except BrikError:
+            if out is None:
+                self.ctx.free(y)
+            raise
+        return y
+
+    def moe_mm_i8(self, x: I8Rows, row_off, w: I8Rows, y_sorted, E: int, rows: int, K: int, N: int, src=None, k: int = 1):
+        """The same by experts, ``w`` a handle of [E, N, K]; with ``src``, ``x`` holds the tokens (rows / k of them)."""
+        self.ctx.moe_matmul_t_i8(x["i8"], x["isc"], row_off, w["i8"], w["isc"], y_sorted, E, rows, K, N, src=src, k=k)
 
     # ---- sampling pre-work ---------------------------------------------------------------
     def _top_k(self, run, recent, k):

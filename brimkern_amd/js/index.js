@@ -29,6 +29,8 @@
 //   (recConv2dDirectQ8 / Q4)            :1233-1256  (device resident; inputs may be Float32Arrays)
 //   rope / quantize_kv and the attention    shaders.ts   engine.kvCache(dtype, ...), qkNormRope, kvWrite, kvRead,
 //   passes over the quantized cache     :1361, 1673  attention (device resident, pages and batches)
+//   (none: the reference has no experts)             engine.moeRoute, moeRouteGrad, moeSort, moeDispatch, moeCombine,
+//                                                    moeCombineGrad; 8-bit products: quantizeI8, mmI8, moeMatmulI8
 //   .brik container (container.ts)                   require('./container'): parseBrik, serializeBrik, ...;
 //                                                    engine.weightFromContainer(parsed, name)
 //
@@ -47,6 +49,12 @@ let native = null;
 function loadNative() {
   if (native === null) native = require(path.join(__dirname, 'brik.node'));   // throws if not built
   return native;
+}
+
+let experts = null;                                  // experts and 8-bit products, an addon beside it
+function loadExperts() {
+  if (experts === null) experts = require(path.join(__dirname, 'brik_experts.node'));
+  return experts;
 }
 
 const FMT = { q8: 8, q4: 4, q3: 3 };
@@ -73,6 +81,11 @@ function jobSpec(j) {
 // The native rows object: its flags from {onePlus, interleaved}.
 function qkvRows(r) {
   return Object.assign({}, r, { flags: (r.onePlus ? 1 : 0) | (r.interleaved ? 2 : 0) });
+}
+
+// The native routing object: its flags from {sigmoid, renorm}.
+function routeArgs(r) {
+  return Object.assign({}, r, { flags: (r.sigmoid ? 1 : 0) | (r.renorm ? 2 : 0) });
 }
 
 function planHandle(nat, plan) {
@@ -342,6 +355,77 @@ class Engine {
   moeMatmulQ4x2(xSorted, rowOff, wa, ya, wb, yb, E, R, K, N) {
     this.native.moeMatmulQ4x2(this.ctx, xSorted, rowOff, wa.nib, wa.sc, wa.mn, ya, wb.nib, wb.sc, wb.mn, yb, E, R, K, N);
     return [ya, yb];
+  }
+
+  // ---- experts (include/brik.h: brik_moe_*): no reference counterpart -------------------------------------
+  // route: {logits, tokens, experts, k, ids, weights[, bias, logitStride, sigmoid, renorm, scale, rowOff, src, slot]}, device buffers:
+  // the k experts of every token and their weights and, with rowOff, src and slot, the assignments sorted by expert.
+  moeRoute(route) { loadExperts().moeRoute(this.ctx, routeArgs(route)); }
+
+  // The logits' gradient [tokens, experts] from the weights' [tokens, k].
+  moeRouteGrad(route, dweights, dlogits) {
+    loadExperts().moeRouteGrad(this.ctx, routeArgs(route), dweights, dlogits);
+    return dlogits;
+  }
+
+  // rowOff [experts + 1], src and slot [tokens * k] (int32 device buffers) of assignments ids [tokens, k].
+  moeSort(ids, rowOff, src, slot, tokens, k, experts) { loadExperts().moeSort(this.ctx, ids, rowOff, src, slot, tokens, k, experts); }
+
+  // The tokens' rows to their experts' rows (weights may be null), and back, weighted, summed and added to res (may be null).
+  moeDispatch(x, slot, weights, xSorted, tokens, k, width) {
+    loadExperts().moeDispatch(this.ctx, x, slot, weights, xSorted, tokens, k, width);
+    return xSorted;
+  }
+
+  moeCombine(ySorted, slot, weights, res, out, tokens, k, width) {
+    loadExperts().moeCombine(this.ctx, ySorted, slot, weights, res, out, tokens, k, width);
+    return out;
+  }
+
+  // The gradients of the experts' rows and of the weights (either may be null).
+  moeCombineGrad(dout, ySorted, slot, weights, dySorted, dweights, tokens, k, width) {
+    loadExperts().moeCombineGrad(this.ctx, dout, ySorted, slot, weights, dySorted, dweights, tokens, k, width);
+  }
+
+  // ---- products of 8-bit integers (brik_quantize_i8, brik_matmul_t_i8, brik_moe_matmul_t_i8) ----------------
+  // Rows x [M, K] (f32 device buffer), or act(opts.gate) * x, to int8 codes and a scale each: {i8, isc}, a weight or an activation
+  // handle (keys of its own: no product of .brik planes takes it). opts: {gate, act: 'gelu' (else SiLU), xStride, gateStride, out: a handle to fill}. destroyWeight frees it.
+  quantizeI8(x, M, K, opts) {
+    const o = opts || {};
+    let h = o.out;
+    if (!h) {
+      if (!(M >= 0 && K >= 0)) throw einval('quantizeI8: M = ' + M + ', K = ' + K);
+      const at = Math.ceil(M * K / 16) * 16, buf = this.alloc(Math.max(at + 4 * M, 16));
+      h = { i8: buf.view(0), isc: buf.view(at), _buf: buf };
+    }
+    try {
+      loadExperts().quantizeI8(this.ctx, { x: x, gate: o.gate || null, codes: h.i8, scales: h.isc, M: M, K: K,
+        xStride: o.xStride || 0, gateStride: o.gateStride || 0, flags: o.act === 'gelu' ? 2 : 0 });
+    } catch (e) {
+      if (!o.out) h._buf.destroy();
+      throw e;
+    }
+    return h;
+  }
+
+  // y [m, n] = x . w^T of handles of quantizeI8, plus opts.res; returns opts.out (allocated when not given).
+  mmI8(x, w, m, k, n, opts) {
+    const o = opts || {}, y = o.out || this.alloc(Math.max(m * n * 4, 4));
+    try {
+      loadExperts().matmulI8(this.ctx, x.i8, x.isc, w.i8, w.isc, o.res || null, y, m, k, n);
+    } catch (e) {
+      if (!o.out) y.destroy();
+      throw e;
+    }
+    return y;
+  }
+
+  // By experts, w a handle of [E, N, K]: rows of x by position or, with opts {src, k[, xRows]}, the tokens that src names.
+  moeMatmulI8(x, rowOff, w, ySorted, E, rows, K, N, opts) {
+    const o = opts || {}, k = o.src ? o.k : 1;
+    const xRows = o.xRows !== undefined ? o.xRows : o.src ? Math.floor(rows / k) : rows;
+    loadExperts().moeMatmulI8(this.ctx, x.i8, x.isc, o.src || null, rowOff, w.i8, w.isc, ySorted, xRows, k, E, rows, K, N);
+    return ySorted;
   }
 
   // Grouped decode GEMV plan: jobs [{x, w, y, K, N}] (one format), executed by one launch per run().
