@@ -2806,12 +2806,12 @@ static int product_i8(brik_ctx* c, const char* who, brik_i8_launch& a, bool moe)
     if (a.M == 0 || a.N == 0 || (moe && (a.E == 0 || a.x_rows == 0))) return BRIK_OK;
     const int t = brik_plan::i8_plan(a, c->opt_i8_kernel, c->opt_i8_splits);
     const brik_plan::I8Kernel& g = brik_plan::kI8Kernels[t];
+    long blocks = 0;
+    if (!brik_plan::i8_fits(a, t, blocks)) return fail(c, BRIK_EINVAL, "%s: %ld blocks in one call", who, blocks);
     if (a.splits > 1) {
         HIP_TRY_RC(ensure_buf(c, c->iws, c->iws_bytes, 4 * (size_t)a.splits * a.M * a.N));
         a.part = static_cast<int32_t*>(c->iws);
     }
-    const long blocks = (long)a.row_tiles * a.col_tiles * a.splits;
-    if (blocks >= (1l << 23)) return fail(c, BRIK_EINVAL, "%s: %ld blocks in one call", who, blocks);
     c->last_kernel = g.kind == brik_plan::I8_FEW ? "i8_few" : g.kind == brik_plan::I8_TILE ? "i8_tile" : "i8_moe";
     void* args[] = {&a};
     HIP_TRY_RC(launch_fn(c, c->moe_fn[E_I8 + t], (unsigned)blocks, 1, (unsigned)g.threads, 0, args));

@@ -87,6 +87,7 @@ inline int quantize_i8(Why& w, const char* who, brik_quant_launch& a, int flags)
 inline int product_i8(Why& w, const char* who, const brik_i8_launch& a, bool moe)
 {
     if (a.M < 0 || a.K < 0 || a.N < 0) return no(w, BRIK_EINVAL, "%s: negative shape M=%d K=%d N=%d", who, a.M, a.K, a.N);
+    if (a.M > 1 << 30) return no(w, BRIK_EINVAL, "%s: %d rows exceed 2^30 in one call", who, a.M);
     if (a.K % 32 || a.K > BRIK_I8_K) return no(w, BRIK_EINVAL, "%s: K=%d is not a multiple of 32 up to %d", who, a.K, BRIK_I8_K);
     if (moe) {
         if (a.E < 0 || a.E > 65536) return no(w, BRIK_EINVAL, "%s: %d experts (0 to 65536)", who, a.E);

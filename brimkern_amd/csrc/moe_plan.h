@@ -128,4 +128,11 @@ inline int i8_plan(brik_i8_launch& a, int forced, int splits)
     return t;
 }
 
+// What a launch takes: blocks, and threads, that 32 bits count.
+inline bool i8_fits(const brik_i8_launch& a, int kernel, long& blocks)
+{
+    blocks = (long)a.row_tiles * a.col_tiles * a.splits;
+    return blocks < (1l << 23) && blocks * kI8Kernels[kernel].threads < (1l << 32);
+}
+
 }  // namespace brik_plan

@@ -457,11 +457,13 @@ int brik_attention(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batc
  * a = t * k + j; its expert is ids[a]. Assignments whose id is outside [0, experts) (none chosen, or another device's expert)
  * have no row. Sorted rows are the others, by expert, those of an expert in the order of a: row_off[e] is the first row of
  * expert e, row_off[experts] their number; src[r] is the assignment of row r (-1 from there on), slot[a] the row of an
- * assignment (-1: none). All of them int32 DEVICE arrays: row_off [experts + 1], src and slot [tokens * k].
+ * assignment (-1: none). All of them int32 DEVICE arrays: row_off [experts + 1], src and slot [tokens * k]. (The products take
+ * them with tokens * k rows, however many have an expert: rows of y_sorted from row_off[experts] on are left as they are by _i8
+ * and may hold anything after _q4; no row reads another one.)
  *
  * brik_moe_route: the k experts of every token and their weights. With l the token's logits and s = softmax(l) over all
  * experts or, with BRIK_ROUTE_SIGMOID, s = 1 / (1 + exp(-l)):
- *   ids      the k largest s, with bias the k largest s + bias (in 64 bits), the largest first, ties by smaller id; a
+ *   ids      the k largest s, with bias the k largest s + bias (as in 64 bits), the largest first, ties by smaller id; a
  *            logit (or sum) of -infinity or NaN is never chosen: where fewer are left the others are -1
  *   weights  scale * s of the chosen ones (without the bias), with BRIK_ROUTE_RENORM divided by their sum; 0 for id -1
  * A token all of whose logits are -infinity (padding) so goes nowhere. A NaN logit counts as -infinity; +infinity gives a
@@ -528,8 +530,8 @@ int brik_quantize_i8(brik_ctx *ctx, const float *x, int64_t x_stride, const floa
 
 /* y[m, n] = (sum_k x[m, k] * w[n, k]) * w_scales[n] * x_scales[m] (+ res[m, n]): the sum exact, rounded to f32, then two
  * roundings, and one for res. x int8 [M, K], w int8 [N, K], 16-byte aligned; K a multiple of 32 up to BRIK_I8_K (no sum passes 31 bits);
- * N below 2^22; res f32 [M, N] or NULL, may be y. Codes of -128 are taken as they are. N * K below 2^32. Workspace: partial sums of split
- * K, grown on demand. */
+ * M at most 2^30, N below 2^22, N * K below 2^32; res f32 [M, N] or NULL, may be y. Codes of -128 are taken as they are. Workspace:
+ * partial sums of split K, grown on demand. A call of 2^23 blocks of work and more is refused with their number (here and by experts). */
 #define BRIK_I8_K 131040
 int brik_matmul_t_i8(brik_ctx *ctx, const int8_t *x, const float *x_scales, const int8_t *w, const float *w_scales,
                      const float *res, float *y, int M, int K, int N);

@@ -98,7 +98,8 @@ int main()
         product_is(BRIK_OK, moe, [](brik_i8_launch& x) { x.K = BRIK_I8_K; });
         product_is(BRIK_OK, moe, [](brik_i8_launch& x) { x.K = 0, x.x = x.w = nullptr; });
         product_is(BRIK_OK, moe, [](brik_i8_launch& x) { x.N = 0, x.y = nullptr; });
-        for (int v : {-1, least}) product_is(BRIK_EINVAL, moe, [&](brik_i8_launch& x) { x.M = v; });
+        for (int v : {-1, least, (1 << 30) + 1, most - 16, most}) product_is(BRIK_EINVAL, moe, [&](brik_i8_launch& x) { x.M = v, x.x_rows = most; });
+        product_is(BRIK_OK, moe, [](brik_i8_launch& x) { x.M = 1 << 30, x.x_rows = 1 << 30; });
         for (int v : {-32, 16, 33, BRIK_I8_K + 32, most, least}) product_is(BRIK_EINVAL, moe, [&](brik_i8_launch& x) { x.K = v; });
         for (int v : {-1, 1 << 22, most, least}) product_is(BRIK_EINVAL, moe, [&](brik_i8_launch& x) { x.N = v; });
         product_is(BRIK_EINVAL, moe, [](brik_i8_launch& x) { x.N = 40000, x.K = 131040; });
@@ -140,6 +141,9 @@ int main()
         EXPECT(g.kind == brik_plan::I8_FEW || (g.kind == brik_plan::I8_MOE) == (a.E > 0));
         EXPECT(forced == 0 || n == forced - 1 || brik_plan::kI8Kernels[forced - 1].kind == (a.E ? brik_plan::I8_TILE : brik_plan::I8_MOE));
         EXPECT((long)a.col_tiles * g.bn >= a.N && (long)(a.col_tiles - 1) * g.bn < a.N);
+        long blocks = 0;
+        if (brik_plan::i8_fits(a, n, blocks)) EXPECT(blocks * g.threads <= 4294967295l && blocks == (long)a.row_tiles * a.col_tiles * a.splits);
+        else EXPECT(blocks >= 1 << 22);
         const long steps = (a.K + 63) / 64;
         EXPECT(a.steps >= 1 && a.splits >= 1 && (long)a.splits * a.steps >= steps && (long)(a.splits - 1) * a.steps < steps);
         EXPECT(a.E == 0 || a.splits == 1);
@@ -156,6 +160,12 @@ int main()
             EXPECT(tiles <= a.row_tiles);
         }
     }
+    // forced onto many experts and channels: more threads than a launch has
+    brik_i8_launch many{};
+    many.E = 65536, many.M = 65536, many.K = 64, many.N = 1280;
+    long blocks = 0;
+    EXPECT(!brik_plan::i8_fits(many, brik_plan::i8_plan(many, 4, 0), blocks) && blocks == 65536 * 80l);
+    EXPECT(brik_plan::i8_fits(many, brik_plan::i8_plan(many, 1, 0), blocks) && blocks == 65536 * 80l);
     std::printf(failures ? "%d failures\n" : "ok\n", failures);
     return failures != 0;
 }

@@ -132,6 +132,90 @@ def test_every_kernel(dev, kernel, splits):
         ctx.set_option(BRIK_OPT_I8_SPLITS, 0)
 
 
+def test_recorded_products_follow_their_inputs(dev):
+    """A captured step with K split over blocks (sums in the context's workspace), replayed with other inputs and smaller calls between;
+    after a call that needed a larger workspace the recording is refused."""
+    ctx, M, K, N = dev.ctx, 40, 4096, 100
+    ops = operands(np.random.default_rng(0), M, K, N)
+    x, xs, w, ws, res, y, h = *[dev.up(o) for o in ops], dev.full((M, N)), dev.full((M, N)), dev.full((M, K))
+    try:
+        ctx.set_option(BRIK_OPT_I8_KERNEL, 9)
+        ctx.set_option(BRIK_OPT_I8_SPLITS, 4)
+        def step():
+            ctx.quantize_i8(h, x, xs, M, K)
+            ctx.matmul_t_i8(x, xs, w, ws, y, M, K, N, res=res)
+            ctx.matmul_t_i8(x, xs, w, ws, y, M, K, N, res=y)
+        step()
+        ctx.graph_begin()
+        step()
+        graph = ctx.graph_end()
+        for i in range(4):
+            rng = np.random.default_rng(i)
+            hv, r = rng.standard_normal((M, K)).astype(np.float32), rng.standard_normal((M, N)).astype(np.float32)
+            ctx.h2d(h, hv)
+            ctx.h2d(res, r)
+            graph.launch()
+            codes, scales = R.quantize(hv)
+            p, bound = R.product(codes, scales, *ops[2:], res=r)
+            want, more = R.product(codes, scales, *ops[2:], res=p)
+            close(dev.get(y, (M, N)), want, bound + more + R.HALF * bound)
+            small = operands(rng, 3, 512, 60)
+            close(run_product(dev, *small), *R.product(*small))
+        ctx.set_option(BRIK_OPT_I8_SPLITS, 16)
+        large = operands(np.random.default_rng(9), 130, 4096, 1100)
+        close(run_product(dev, *large), *R.product(*large))
+        with pytest.raises(BrikError) as e:
+            graph.launch()
+        assert e.value.code == BRIK_EINVAL
+        graph.destroy()
+    finally:
+        ctx.set_option(BRIK_OPT_I8_KERNEL, 0)
+        ctx.set_option(BRIK_OPT_I8_SPLITS, 0)
+
+
+def test_two_contexts_at_once(dev):
+    from brimkern_amd.capi import Context
+    from test_gpu_moe import Dev
+    M, K, N = 200, 4096, 300
+    with Context(0) as second:
+        d2, runs = Dev(second), []
+        for i, d in enumerate((dev, d2)):
+            ops = operands(np.random.default_rng(i), M, K, N)
+            d.ctx.set_option(BRIK_OPT_I8_SPLITS, 5)
+            runs.append((d, ops, [d.up(o) for o in ops], d.full((M, N))))
+        try:
+            for _ in range(5):
+                for d, _, b, y in runs:
+                    d.ctx.matmul_t_i8(*b, y, M, K, N)
+            for d, ops, _, y in runs:
+                close(d.get(y, (M, N)), *R.product(*ops))
+        finally:
+            dev.ctx.set_option(BRIK_OPT_I8_SPLITS, 0)
+            d2.free()
+
+
+@pytest.mark.parametrize("large", ["x", "y", "y by experts"])
+def test_past_32_bits(dev, large):
+    """The last rows of operands of more than 2^32 bytes."""
+    ctx, rng, last = dev.ctx, np.random.default_rng(3), 20
+    M, K, N = (33001, 131040, 9) if large == "x" else (60001, 32, 20000)
+    x, xs, w, ws = operands(rng, last, K, N)
+    xd, sd, yd = ctx.alloc(M * K), ctx.alloc(4 * M), ctx.alloc(4 * M * N)      # (what lies before the last rows does not matter)
+    dev.bufs += [xd, sd, yd]
+    ctx.h2d(xd, x, (M - last) * K)
+    ctx.h2d(sd, xs, 4 * (M - last))
+    if large == "y by experts":
+        ctx.moe_matmul_t_i8(xd, sd, dev.up(np.array([0, M - 7, M], np.int32)), dev.up(np.concatenate([w, w[::-1]])), dev.up(np.concatenate([ws, ws[::-1]])),
+                            yd, 2, M, K, N)
+    else:
+        ctx.matmul_t_i8(xd, sd, dev.up(w), dev.up(ws), yd, M, K, N)
+    got = ctx.download(yd, np.float32, last * N, 4 * (M - last) * N).reshape(last, N)
+    want, bound = R.product(x, xs, w, ws)
+    if large == "y by experts":
+        want[-7:], bound[-7:] = want[-7:, ::-1].copy(), bound[-7:, ::-1].copy()
+    close(got, want, bound)
+
+
 @pytest.mark.parametrize("M", [1, 100])
 def test_largest_sums(dev, M):
     """K at its limit with all codes -128: the largest sum that 31 bits hold."""
@@ -320,6 +404,27 @@ def test_experts_of_q4(dev):
             continue
         want = sum(float(w[a, j]) * got[slot[a, j]].astype(np.float64) for j in range(k))
         assert (np.abs(o[a] - want) <= 4 * R.HALF * sum(np.abs(w[a, j] * got[slot[a, j]]) for j in range(k))).all()
+
+
+def test_fewer_rows_than_assignments_of_q4(dev):
+    """Few rows of 4-bit experts, some assignments without one: the rows of the others are those of a call without them, bit for bit
+    (the sizes that choose the kernel are the same)."""
+    import oracle as O
+    from helpers import PLANES
+    ctx, rng, T, E, k, K, N = dev.ctx, np.random.default_rng(4), 12, 4, 2, 2048, 160
+    t = dict(zip(PLANES["q4"], O.quantize_q4(rng.standard_normal(E * N * K).astype(np.float32))))
+    planes = [dev.up(t[p]) for p in PLANES["q4"]]
+    x = rng.standard_normal((T * k, K)).astype(np.float32)
+    off = np.array([0, 5, 5, 9, 14], np.int32)
+    full = off.copy()
+    full[-1] = T * k
+    out = []
+    for o, rest in ((off, np.nan), (full, 0.5)):
+        x[off[-1]:] = rest
+        y = dev.full((T * k, N))
+        ctx.moe_matmul_t_q4(dev.up(x), dev.up(o), *planes, y, E, T * k, K, N)
+        out.append(dev.get(y, (T * k, N))[: off[-1]])
+    assert np.isfinite(out[0]).all() and (out[0] == out[1]).all()
 
 
 def test_refusals(dev):

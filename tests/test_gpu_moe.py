@@ -264,6 +264,33 @@ def test_recorded_routing_follows_its_inputs(dev):
     graph.destroy()
 
 
+def test_past_32_bits(dev):
+    """Sorted rows of more than 2^32 bytes, there and back, and the gradient of that: the last rows."""
+    ctx, rng, T, k, H = dev.ctx, np.random.default_rng(5), 33001, 8, 4096
+    n, last = T * k, 3
+    slot = np.arange(n, dtype=np.int32).reshape(T, k)
+    slot[-last:] = slot[-last:, ::-1]
+    x, w = rng.standard_normal((last, H)).astype(np.float32), rng.standard_normal((last, k)).astype(np.float32)
+    xd, wd, rows, sd = ctx.alloc(4 * T * H), ctx.alloc(4 * n), ctx.alloc(4 * n * H), dev.up(slot)
+    out, dw = ctx.alloc(4 * T * H), ctx.alloc(4 * n)                                # (what lies before the last rows does not matter)
+    dev.bufs += [xd, wd, rows, out, dw]
+    ctx.h2d(xd, x, 4 * (T - last) * H)
+    ctx.h2d(wd, w, 4 * (T - last) * k)
+    ctx.moe_dispatch(xd, sd, wd, rows, T, k, H)
+    got = ctx.download(rows, np.float32, last * k * H, 4 * (n - last * k) * H).reshape(last, k, H)
+    want = (w[:, :, None] * x[:, None])[:, ::-1]
+    assert (got == want).all()
+    ctx.moe_combine(rows, sd, None, None, out, T, k, H)
+    back = ctx.download(out, np.float32, last * H, 4 * (T - last) * H).reshape(last, H)
+    assert (np.abs(back - want.astype(np.float64).sum(1)) <= k * R.HALF * np.abs(want).sum(1)).all()
+    ctx.moe_combine_grad(xd, rows, sd, wd, rows, dw, T, k, H)
+    g = ctx.download(dw, np.float32, last * k, 4 * (T - last) * k).reshape(last, k)
+    terms = x[:, None].astype(np.float64) * want[:, ::-1]
+    # the products and sums of a thread's 16 values, 6 steps over the lanes and 2 over the waves
+    assert (np.abs(g - terms.sum(-1)) <= (16 + 6 + 2 + 2) * R.HALF * np.abs(terms).sum(-1)).all()
+    assert (ctx.download(rows, np.float32, last * k * H, 4 * (n - last * k) * H).reshape(last, k, H) == want).all()
+
+
 def test_two_contexts_at_once(dev):
     from brimkern_amd.capi import Context
     rng, T, E, k = np.random.default_rng(2), 3000, 64, 6
