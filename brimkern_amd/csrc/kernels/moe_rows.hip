@@ -3,7 +3,9 @@
 //   dispatch: xs[slot_j] = w_j x     combine: out = res + sum_j w_j y[slot_j]     gradient: dy[slot_j] = w_j dout, dw_j = dout . y[slot_j]
 //
 // All three go by token: a row of the token is read once and its k sorted rows are named by the slots, so nothing is read
-// twice and no sum depends on an order. Bound by memory: a token's row and its k sorted ones, read or written once.
+// twice and no sum depends on an order. Bound by memory: a token's row and its k sorted ones, read or written once. Rows of 2048: 16384
+// tokens, 6 places, three quarters of them elsewhere, there 66 us (5.1 TB/s) and back 100 (4.7); 4096 tokens, 8 places, the gradient 104
+// (5.5 TB/s) and the sum of its rows 79; 256 tokens 6 each, the latency of slot, row, store.
 #include "attn_common.h"
 #include "moe_abi.h"
 

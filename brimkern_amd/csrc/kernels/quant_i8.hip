@@ -5,7 +5,8 @@
 // 2^-21 of itself. What depends on the last bits is then done in 64: the maximum among the values next to the f32 one, and the codes
 // whose f32 quotient lies nearer to a border than its error. A row with values that f32 does not hold to 2^-21 (gates below -64,
 // overflow, NaN) and one under GELU take 64 bits throughout. Bound by memory: 4 bytes read a value (8 with a gate), one written.
-// 8192 x 9728 85 us, 4.7 TB/s; with a gate
+// 8192 x 9728 84 us, 4.75 TB/s, vector instructions in 79 % of the cycles; with a gate 32768 x 768 55 us, 4.15 TB/s and 84 %; 512 x 2560
+// 4 us and one row 3, a launch's latency.
 #include "attn_common.h"
 #include "moe_abi.h"
 
