@@ -5,7 +5,7 @@
 // Integer sums have no order, so K may be split over waves and blocks freely: results are the same bits. Two kernels:
 //   few rows (decoding, experts of few tokens): bound by the bytes of w and by latency. A block has 16 channels; its 4 to 16 waves split
 //     K, and a wave loads all of its part of w at once, into registers, and multiplies it with 16 or 32 rows of x after the other. 1 row of
-//     2560 x 9728 7.7 us (3.2 TB/s, a launch among them), of 9728 x 2560 9.7; 24 rows of 4096 x 2561 8.5.
+//     2560 x 9728 7.7 us (3.2 TB/s, a launch among them), of 9728 x 2560 8.9; 24 rows of 4096 x 2561 7.6.
 //   tiles (prompts): bound by the matrix cores. Both operands go through LDS, 128 of K a step, double-buffered, the loads of the next
 //     step (256 x 256) or of the next two in registers meanwhile. 8192^3 492 us, 2.2 POP/s (the card's library 2.1; the clock falls
 //     under this load); 8192 x 9728 x 2560 218 (library 202); 512 x 2560 x 9728 21 to 22 (library 38), where loads through the
@@ -105,7 +105,7 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
     }
     const int n0 = ct * C, K = a.K;
     const int steps = (K + 63) >> 6, s0 = split * a.steps, s1 = min(steps, s0 + a.steps);
-    const int per = min(FEW_S, (s1 - s0 + NW - 1) / NW), pieces = (s1 - s0 + NW * per - 1) / (NW * per);
+    const int pieces = (s1 - s0 + NW * FEW_S - 1) / (NW * FEW_S), per = (s1 - s0 + NW * pieces - 1) / (NW * pieces);
     const int8_t* wr[CB];
 #pragma unroll
     for (int c = 0; c < CB; ++c) wr[c] = r.w + (size_t)min(n0 + 16 * c + i16, a.N - 1) * K;

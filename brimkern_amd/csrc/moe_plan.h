@@ -71,7 +71,7 @@ inline double i8_few_us(long M, long K, long N, int waves)
 }
 
 // The kernel of a dense product and the splits of its K, by these times. What it weighs (us): 1 x 2560 x 9728 few 7.7, tiles 9.1; 1 x
-// 9728 x 2560 few by 16 waves 9.7, by 8 11.1, tiles 23.7, in 8 splits 11.5; 64 x 2560 x 9728 few 20, 64 x 128 tiles 9.6; 128 x 9728 x
+// 9728 x 2560 few by 16 waves 8.9, by 8 10.8, tiles 23.7, in 8 splits 11.5; 64 x 2560 x 9728 few 20, 64 x 128 tiles 9.6; 128 x 9728 x
 // 2560 64 x 128 tiles 23.5, in 4 splits 13.2; 512 x 2560 x 9728 256 x 128 25, 128 x 128 30, 256 x 256 35; 1536 rows of it 54, 57, 45.
 inline int i8_dense(brik_i8_launch& a, int forced, int splits)
 {
