@@ -281,9 +281,9 @@ __device__ __forceinline__ uint64_t peers_of(int id, bool in, int bits)
     return m;
 }
 
-// The rows of the assignments [a0, a1) of `n`, by a block of MOE_NT threads. With one chunk their counts are all there are;
+// The rows of the assignments [a0, a1), by a block of MOE_NT threads. With one chunk their counts are all there are;
 // else `counts` holds those of every chunk.
-__device__ __forceinline__ void sort_chunk(const int32_t* ids, int a0, int a1, int n, int E, const int32_t* counts, int chunks, int chunk,
+__device__ __forceinline__ void sort_chunk(const int32_t* ids, int a0, int a1, int E, const int32_t* counts, int chunks, int chunk,
                                            int32_t* row_off, int32_t* src, int32_t* slot)
 {
     __shared__ int cnt[MOE_NW * BRIK_MOE_EXPERTS];
@@ -361,7 +361,6 @@ __device__ __forceinline__ void sort_chunk(const int32_t* ids, int a0, int a1, i
         if (in) src[row] = i;
         if (i < w1 && i >= total) src[i] = -1;
     }
-    (void)n;
 }
 
 // Routes the chunk of the block. One chunk is then sorted here; of several, each block counts its own.
@@ -413,7 +412,7 @@ __device__ __forceinline__ void route_body(const brik_route_launch& a)
     } else if (a.r.slot) {
         __threadfence_block();
         __syncthreads();
-        sort_chunk(a.r.ids, 0, a.r.tokens * k, a.r.tokens * k, E, nullptr, 1, 0, a.r.row_off, a.r.src, a.r.slot);
+        sort_chunk(a.r.ids, 0, a.r.tokens * k, E, nullptr, 1, 0, a.r.row_off, a.r.src, a.r.slot);
     }
 }
 
@@ -512,5 +511,5 @@ extern "C" __global__ __launch_bounds__(MOE_NT) void brik_route_count(brik_route
 extern "C" __global__ __launch_bounds__(MOE_NT) void brik_route_sort(brik_route_launch a)
 {
     const int per = a.chunk * a.r.k, n = a.r.tokens * a.r.k, a0 = blockIdx.x * per;
-    sort_chunk(a.r.ids, a0, min(n, a0 + per), n, a.r.experts, a.counts, a.chunks, blockIdx.x, a.r.row_off, a.r.src, a.r.slot);
+    sort_chunk(a.r.ids, a0, min(n, a0 + per), a.r.experts, a.counts, a.chunks, blockIdx.x, a.r.row_off, a.r.src, a.r.slot);
 }

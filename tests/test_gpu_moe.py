@@ -86,6 +86,25 @@ def test_route_with_bias(dev, T, E, k, how):
     check_route(run_route(dev, logits, k, bias=bias, **HOW[how]), logits, k, bias=bias, **HOW[how])
 
 
+@pytest.mark.parametrize("E", [1, 20, 300])
+@pytest.mark.parametrize("how", range(4))
+def test_route_with_bias_at_its_ends(dev, E, how):
+    """Biases of NaN and -infinity are never chosen, +infinity always; large ones swallow the scores (as in 64 bits), so ties by lower id;
+    a token of which nothing is left, and an infinite logit (a softmax of NaN: nothing to choose)."""
+    rng = np.random.default_rng(E)
+    logits = rng.standard_normal((40, E)).astype(np.float32)
+    logits[5] = -np.inf
+    logits[6, ::2] = np.nan
+    ends = [np.nan] if E == 1 else [np.nan, np.inf, -np.inf, np.inf, 1e30, 1e30, -1e30, 3e38, -3e38, 2.0 ** 40, 2.0 ** 40, 0.0, -0.0]
+    bias = np.resize(np.array(ends, np.float32), E)
+    for b in (bias, np.zeros(E, np.float32)):
+        check_route(run_route(dev, logits, min(E, 12), bias=b, **HOW[how]), logits, min(E, 12), bias=b, **HOW[how])
+    if E > 1 and not HOW[how].get("sigmoid"):
+        logits[:, 3] = np.inf
+        ids, w = run_route(dev, logits, 4, bias=np.zeros(E, np.float32), **HOW[how])[:2]
+        assert (ids == -1).all() and (w == 0).all()
+
+
 @pytest.mark.parametrize("sort", [True, False])
 def test_route_ties_masks_and_strides(dev, sort):
     """Equal logits by lower id; masked experts, NaN, rows with fewer experts than k and with none; rows of a wider buffer."""
