@@ -33,6 +33,14 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// A product and what is added to it, a rounding of its own whatever kernel computes it: the build lets products and sums fuse, so the
+// product passes out of the compiler's sight between.
+__device__ __forceinline__ float plus(float y, float res)
+{
+    asm("" : "+v"(y));
+    return y + res;
+}
+
 // What a block multiplies: rows [m0, m1) of y, and the weight of their expert.
 struct I8Rows {
     int m0, m1;
@@ -170,7 +178,7 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
             const int from = x_row(a, row);
             if (from < 0) continue;
             const float y = (float)sum * r.ws[n] * a.xs[from];
-            a.y[at] = a.res ? y + a.res[at] : y;
+            a.y[at] = a.res ? plus(y, a.res[at]) : y;
         }
         __syncthreads();
     }
@@ -240,7 +248,7 @@ __device__ __forceinline__ void i8_write(i32x16_t (&acc)[T::WA][T::WB], brsrc_t 
 #pragma unroll
                 for (int j = 0; j < T::WB; ++j) {
                     float val = (float)acc[part / 2][j][8 * (part & 1) + 4 * q + v] * ws[j] * xs[v];
-                    if constexpr (RES) val += add[part & 1][4 * q + v][j];
+                    if constexpr (RES) val = plus(val, add[part & 1][4 * q + v][j]);
                     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, val), y, offset(16 * part + 8 * q + v, is[v], j), 0, 0);
                 }
         }
@@ -449,6 +457,6 @@ extern "C" __global__ __launch_bounds__(256) void brik_i8_join(brik_i8_launch a)
         for (int s = 0; s < a.splits; ++s) sum += a.part[s * all + i];
         const size_t m = i / a.N, n = i - m * a.N;
         const float y = (float)sum * a.ws[n] * a.xs[m];
-        a.y[i] = a.res ? y + a.res[i] : y;
+        a.y[i] = a.res ? plus(y, a.res[i]) : y;
     }
 }
