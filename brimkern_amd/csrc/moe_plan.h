@@ -115,24 +115,41 @@ inline int i8_experts(brik_i8_launch& a, int forced)
     return rows <= 160 ? kI8Moe + 2 : rows <= 768 || a.K < 1024 ? kI8Moe + 1 : kI8Moe;
 }
 
-// The kernel of a call, and its grid in `a`. forced: 0, or 1 + index of a kernel (a tile of the other kind: 0).
-inline int i8_plan(brik_i8_launch& a, int forced, int splits)
-{
-    if (a.K == 0) forced = a.E ? kI8Moe + 3 : kI8Tiles + 4, splits = 1;      // (a tile without steps: sums of 0)
-    if (!a.E && forced > kI8Moe) forced = 0;
-    const int t = a.E ? i8_experts(a, forced) : i8_dense(a, forced, splits);
-    const I8Kernel& g = kI8Kernels[t];
-    a.col_tiles = (a.N + g.bn - 1) / g.bn;
-    if (g.kind == I8_FEW) a.row_tiles = std::max(1, a.E);
-    else a.row_tiles = (int)(((long)a.M + g.bm - 1) / g.bm + (a.E ? std::min(a.E, a.M) : 0));
-    return t;
-}
-
 // What a launch takes: blocks, and threads, that 32 bits count.
 inline bool i8_fits(const brik_i8_launch& a, int kernel, long& blocks)
 {
     blocks = (long)a.row_tiles * a.col_tiles * a.splits;
     return blocks < (1l << 23) && blocks * kI8Kernels[kernel].threads < (1l << 32);
+}
+
+inline void i8_grid(brik_i8_launch& a, int kernel)
+{
+    const I8Kernel& g = kI8Kernels[kernel];
+    a.col_tiles = (a.N + g.bn - 1) / g.bn;
+    if (g.kind == I8_FEW) a.row_tiles = std::max(1, a.E);
+    else a.row_tiles = (int)(((long)a.M + g.bm - 1) / g.bm + (a.E ? std::min(a.E, a.M) : 0));
+}
+
+// The kernel of a call, and its grid in `a`. forced: 0, or 1 + index of a kernel (a tile of the other kind: 0). A kernel that nobody
+// forced gives way to larger tiles where a launch does not hold its blocks.
+inline int i8_plan(brik_i8_launch& a, int forced, int splits)
+{
+    if (!a.E && forced > kI8Moe) forced = 0;
+    int t;
+    if (a.K == 0) {                      // (a tile without steps: sums of 0)
+        forced = 0;
+        t = a.E ? kI8Moe + 2 : kI8Tiles + 3;
+        a.splits = a.steps = 1;
+    } else t = a.E ? i8_experts(a, forced) : i8_dense(a, forced, splits);
+    i8_grid(a, t);
+    if (forced && t == forced - 1) return t;
+    long blocks;
+    while (!i8_fits(a, t, blocks)) {
+        const int larger = a.E && kI8Kernels[t].kind == I8_FEW ? kI8Moe + 2 : t - 1;
+        if (larger < kI8Tiles || larger == kI8Moe - 1) break;
+        i8_grid(a, t = larger);
+    }
+    return t;
 }
 
 }  // namespace brik_plan

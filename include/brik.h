@@ -531,7 +531,8 @@ int brik_quantize_i8(brik_ctx *ctx, const float *x, int64_t x_stride, const floa
 /* y[m, n] = (sum_k x[m, k] * w[n, k]) * w_scales[n] * x_scales[m] (+ res[m, n]): the sum exact, rounded to f32, then two
  * roundings, and one for res. x int8 [M, K], w int8 [N, K], 16-byte aligned; K a multiple of 32 up to BRIK_I8_K (no sum passes 31 bits);
  * M at most 2^30, N below 2^22, N * K below 2^32; res f32 [M, N] or NULL, may be y. Codes of -128 are taken as they are. Workspace:
- * partial sums of split K, grown on demand. A call of 2^23 blocks of work and more is refused with their number (here and by experts). */
+ * partial sums of split K, grown on demand. A call of 2^23 tiles of 256 x 256 values of y and more (by experts
+ * counted as if each ended in a tile of its own) is refused with their number. */
 #define BRIK_I8_K 131040
 int brik_matmul_t_i8(brik_ctx *ctx, const int8_t *x, const float *x_scales, const int8_t *w, const float *w_scales,
                      const float *res, float *y, int M, int K, int N);
