@@ -111,7 +111,7 @@ class Engine:
         h = QWeight({k: buf.offset(o) for k, (o, _) in offs.items()})
         try:
             self.ctx.quantize(dtype, src, [h[p] for p in self._PLANES[dtype]], n_elems)
-        except BrikError:
+        except BaseException:
             self.ctx.free(buf)
             raise
         if dtype == "q3":
@@ -198,7 +198,7 @@ class Engine:
         planes = (w["codes"], w["sc"]) if fmt == "q8" else (w["nib"], w["sc"], w["mn"])
         try:
             self.ctx.conv2d(fmt, dev(inp), planes, dev(bias), y, Cin, H, W, Cout, kh, kw, stride, pad)
-        except BrikError:
+        except BaseException:
             if out is None:
                 self.ctx.free(y)
             raise
@@ -279,7 +279,7 @@ class Engine:
         bufs = [self.ctx.alloc(layout.byte_length(dtype, n))]
         try:
             bufs.append(self.ctx.alloc(layout.byte_length(dtype, n)))
-        except BrikError:
+        except BaseException:
             self.ctx.free(bufs[0])
             raise
         planes = [[b.offset(offs[p][0]) for p in self._PLANES[dtype]] for b in bufs]
@@ -313,7 +313,7 @@ class Engine:
         y = self.ctx.alloc(max(4 * batch.rows * (args.get("out_stride") or heads * cache.head_dim), 4)) if out is None else out
         try:
             self.ctx.attention(cache, batch, self.ctx.attn_args(q, y, heads, cache.head_dim ** -0.5 if scale is None else scale, **args))
-        except BrikError:
+        except BaseException:
             if out is None:
                 self.ctx.free(y)
             raise
@@ -329,10 +329,10 @@ class Engine:
             at[name], total = total, total + (4 * max(n, 0) + 15) // 16 * 16
         buf = self.ctx.alloc(max(total, 16))
         r = {name: buf.offset(o) for name, o in at.items()}
-        r["args"] = self.ctx.moe_route_args(logits, tokens, experts, k, **r, **how)
         try:
+            r["args"] = self.ctx.moe_route_args(logits, tokens, experts, k, **r, **how)
             self.ctx.moe_route(r["args"])
-        except BrikError:
+        except BaseException:
             self.ctx.free(buf)
             raise
         r["_buf"] = buf
@@ -362,7 +362,7 @@ class Engine:
             h = I8Rows(i8=buf.offset(0), isc=buf.offset(at), _buf=buf)
         try:
             self.ctx.quantize_i8(x, h["i8"], h["isc"], M, K, **how)
-        except BrikError:
+        except BaseException:
             if out is None:
                 self.ctx.free(h["_buf"])
             raise
@@ -373,7 +373,7 @@ class Engine:
         y = self.ctx.alloc(max(m * n, 1) * 4) if out is None else out
         try:
             self.ctx.matmul_t_i8(x["i8"], x["isc"], w["i8"], w["isc"], y, m, k, n, res=res)
-        except BrikError:
+        except BaseException:
             if out is None:
                 self.ctx.free(y)
             raise
