@@ -218,6 +218,14 @@ def _addr(p) -> _P:
     return _P(int(p))
 
 
+def _i32(*sizes):
+    """The sizes of a call, refused where 32 bits do not hold them (ctypes would cut them off)."""
+    for v in sizes:
+        if not -(1 << 31) <= v < 1 << 31:
+            raise BrikError(BRIK_EINVAL, f"{v} is no 32-bit integer")
+    return sizes
+
+
 class Context:
     """One device + one stream (``brik_ctx``)."""
 
@@ -466,7 +474,7 @@ class Context:
         """The routing of a step, made once and used in every one (``brik_moe_route_args``)."""
         flags = (BRIK_ROUTE_SIGMOID if sigmoid else 0) | (BRIK_ROUTE_RENORM if renorm else 0)
         return MoeRouteArgs(_addr(logits), _addr(bias), logit_stride, _addr(ids), _addr(weights), _addr(row_off), _addr(src), _addr(slot),
-                            tokens, experts, k, flags, scale, 0)
+                            *_i32(tokens, experts, k), flags, scale, 0)
 
     def moe_route(self, args: MoeRouteArgs):
         """The k experts of every token, their weights and, if asked for, the sorted assignments (brik_moe_route)."""
@@ -478,39 +486,40 @@ class Context:
 
     def moe_sort(self, ids, tokens, k, experts, row_off, src, slot):
         """Assignments ``ids`` [tokens, k] sorted by expert (brik_moe_sort)."""
-        self._check(self.lib.brik_moe_sort(self.handle, _addr(ids), tokens, k, experts, _addr(row_off), _addr(src), _addr(slot)))
+        self._check(self.lib.brik_moe_sort(self.handle, _addr(ids), *_i32(tokens, k, experts), _addr(row_off), _addr(src), _addr(slot)))
 
     def moe_dispatch(self, x, slot, weights, x_sorted, tokens, k, width):
         """The tokens' rows to their experts' rows, times ``weights`` unless None (brik_moe_dispatch)."""
-        self._check(self.lib.brik_moe_dispatch(self.handle, _addr(x), _addr(slot), _addr(weights), _addr(x_sorted), tokens, k, width))
+        self._check(self.lib.brik_moe_dispatch(self.handle, _addr(x), _addr(slot), _addr(weights), _addr(x_sorted), *_i32(tokens, k, width)))
 
     def moe_combine(self, y_sorted, slot, weights, res, out, tokens, k, width):
         """The experts' rows back to the tokens, weighted and summed, plus ``res`` unless None (brik_moe_combine)."""
-        self._check(self.lib.brik_moe_combine(self.handle, _addr(y_sorted), _addr(slot), _addr(weights), _addr(res), _addr(out), tokens, k,
-                                              width))
+        self._check(self.lib.brik_moe_combine(self.handle, _addr(y_sorted), _addr(slot), _addr(weights), _addr(res), _addr(out),
+                                              *_i32(tokens, k, width)))
 
     def moe_combine_grad(self, dout, y_sorted, slot, weights, dy_sorted, dweights, tokens, k, width):
         """The gradients of the experts' rows and of the weights (brik_moe_combine_grad)."""
         self._check(self.lib.brik_moe_combine_grad(self.handle, _addr(dout), _addr(y_sorted), _addr(slot), _addr(weights), _addr(dy_sorted),
-                                                   _addr(dweights), tokens, k, width))
+                                                   _addr(dweights), *_i32(tokens, k, width)))
 
     # ---- products of 8-bit integers ---------------------------------------------------------------
     def quantize_i8(self, x, codes, scales, M, K, x_stride=0, gate=None, gate_stride=0, gelu=False):
         """Rows of x, or of act(gate) * x, to int8 codes and a scale each (brik_quantize_i8)."""
         self._check(self.lib.brik_quantize_i8(self.handle, _addr(x), x_stride, _addr(gate), gate_stride, BRIK_JOB_ACT_GELU if gelu else 0,
-                                              _addr(codes), _addr(scales), M, K))
+                                              _addr(codes), _addr(scales), *_i32(M, K)))
 
     def matmul_t_i8(self, x, x_scales, w, w_scales, y, M, K, N, res=None):
         """y = x . w^T of int8 codes, scaled by row and channel, plus ``res`` unless None (brik_matmul_t_i8)."""
-        self._check(self.lib.brik_matmul_t_i8(self.handle, _addr(x), _addr(x_scales), _addr(w), _addr(w_scales), _addr(res), _addr(y), M, K, N))
+        self._check(self.lib.brik_matmul_t_i8(self.handle, _addr(x), _addr(x_scales), _addr(w), _addr(w_scales), _addr(res), _addr(y),
+                                              *_i32(M, K, N)))
 
     def moe_matmul_t_i8(self, x, x_scales, row_off, w, w_scales, y_sorted, E, rows, K, N, src=None, k=1, x_rows=None):
         """The same by experts (brik_moe_matmul_t_i8). x: the sorted rows or, with ``src`` and ``k``, the tokens (rows / k of them
         unless ``x_rows`` says otherwise)."""
         if x_rows is None:
             x_rows = rows if src is None else rows // max(k, 1)
-        self._check(self.lib.brik_moe_matmul_t_i8(self.handle, _addr(x), _addr(x_scales), x_rows, _addr(src), k, _addr(row_off), _addr(w),
-                                                  _addr(w_scales), _addr(y_sorted), E, rows, K, N))
+        self._check(self.lib.brik_moe_matmul_t_i8(self.handle, _addr(x), _addr(x_scales), *_i32(x_rows), _addr(src), *_i32(k), _addr(row_off),
+                                                  _addr(w), _addr(w_scales), _addr(y_sorted), *_i32(E, rows, K, N)))
 
     def dequant_q8(self, codes, sc, out, n):
         self._check(self.lib.brik_dequant_q8_f32(self.handle, _addr(codes), _addr(sc), _addr(out), n))
