@@ -168,16 +168,31 @@ inline napi_value undefined(napi_env env)
     return u;
 }
 
-// Parse (ctx, p0 .. p{np-1}, i0 .. i{ni-1}).
-inline bool parse(napi_env env, napi_callback_info info, brik_ctx** ctx, void** p, int np, int32_t* iv, int ni)
+// An integer of the range of its C type: anything else is refused, not cut off.
+inline bool get_whole(napi_env env, napi_value v, const std::string& what, double most, double* out)
+{
+    if (napi_get_value_double(env, v, out) != napi_ok || !(*out >= -most && *out <= most) || *out != (double)(int64_t)*out) {
+        napi_throw_type_error(env, "BRIK_EINVAL", ("expected an integer: " + what).c_str());
+        return false;
+    }
+    return true;
+}
+
+// Parse (ctx, p0 .. p{np-1}, i0 .. i{ni-1}). whole: numbers that are no 32-bit integers are refused, else converted as by ToInt32.
+inline bool parse(napi_env env, napi_callback_info info, brik_ctx** ctx, void** p, int np, int32_t* iv, int ni, bool whole = false)
 {
     Args a;
     if (!get_args(env, info, a, (size_t)(1 + np + ni))) return false;
     if (!get_ctx(env, a.v[0], ctx)) return false;
     for (int i = 0; i < np; ++i)
         if (!get_ptr(env, a.v[1 + i], &p[i])) return false;
-    for (int i = 0; i < ni; ++i)
-        if (!get_i32(env, a.v[1 + np + i], &iv[i])) return false;
+    for (int i = 0; i < ni; ++i) {
+        double d = 0;
+        if (!whole) {
+            if (!get_i32(env, a.v[1 + np + i], &iv[i])) return false;
+        } else if (!get_whole(env, a.v[1 + np + i], "argument " + std::to_string(np + i + 1), 2147483647.0, &d)) return false;
+        else iv[i] = (int32_t)d;
+    }
     return true;
 }
 
@@ -209,18 +224,11 @@ inline bool opt_f32(napi_env env, napi_value o, const char* name, float* out)
     bool has;
     return get_field(env, o, name, &f, &has) && (!has || get_f32(env, f, out));
 }
-// An integer of the range of its C type: anything else is refused, not cut off.
 inline bool opt_int(napi_env env, napi_value o, const char* name, double most, double* out)
 {
     napi_value f;
     bool has;
-    if (!get_field(env, o, name, &f, &has)) return false;
-    if (!has) return true;
-    if (napi_get_value_double(env, f, out) != napi_ok || !(*out >= -most && *out <= most) || *out != (double)(int64_t)*out) {
-        napi_throw_type_error(env, "BRIK_EINVAL", (std::string("expected an integer: ") + name).c_str());
-        return false;
-    }
-    return true;
+    return get_field(env, o, name, &f, &has) && (!has || get_whole(env, f, name, most, out));
 }
 inline bool opt_i32(napi_env env, napi_value o, const char* name, int32_t* out)
 {

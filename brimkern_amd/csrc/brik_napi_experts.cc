@@ -48,7 +48,7 @@ napi_value MoeRouteGrad(napi_env env, napi_callback_info info)   // (ctx, route,
 napi_value MoeSort(napi_env env, napi_callback_info info)   // (ctx, ids, rowOff, src, slot, tokens, k, experts)
 {
     brik_ctx* c; void* p[4]; int32_t i[3];
-    if (!parse(env, info, &c, p, 4, i, 3)) return nullptr;
+    if (!parse(env, info, &c, p, 4, i, 3, true)) return nullptr;
     if (check(env, c, brik_moe_sort(c, (const int32_t*)p[0], i[0], i[1], i[2], (int32_t*)p[1], (int32_t*)p[2], (int32_t*)p[3]))) return nullptr;
     return undefined(env);
 }
@@ -56,7 +56,7 @@ napi_value MoeSort(napi_env env, napi_callback_info info)   // (ctx, ids, rowOff
 napi_value MoeDispatch(napi_env env, napi_callback_info info)   // (ctx, x, slot, weights, xSorted, tokens, k, width)
 {
     brik_ctx* c; void* p[4]; int32_t i[3];
-    if (!parse(env, info, &c, p, 4, i, 3)) return nullptr;
+    if (!parse(env, info, &c, p, 4, i, 3, true)) return nullptr;
     if (check(env, c, brik_moe_dispatch(c, (const float*)p[0], (const int32_t*)p[1], (const float*)p[2], (float*)p[3], i[0], i[1], i[2])))
         return nullptr;
     return undefined(env);
@@ -65,7 +65,7 @@ napi_value MoeDispatch(napi_env env, napi_callback_info info)   // (ctx, x, slot
 napi_value MoeCombine(napi_env env, napi_callback_info info)   // (ctx, ySorted, slot, weights, res, out, tokens, k, width)
 {
     brik_ctx* c; void* p[5]; int32_t i[3];
-    if (!parse(env, info, &c, p, 5, i, 3)) return nullptr;
+    if (!parse(env, info, &c, p, 5, i, 3, true)) return nullptr;
     if (check(env, c, brik_moe_combine(c, (const float*)p[0], (const int32_t*)p[1], (const float*)p[2], (const float*)p[3], (float*)p[4], i[0], i[1],
                                        i[2])))
         return nullptr;
@@ -75,7 +75,7 @@ napi_value MoeCombine(napi_env env, napi_callback_info info)   // (ctx, ySorted,
 napi_value MoeCombineGrad(napi_env env, napi_callback_info info)   // (ctx, dout, ySorted, slot, weights, dySorted, dweights, tokens, k, width)
 {
     brik_ctx* c; void* p[6]; int32_t i[3];
-    if (!parse(env, info, &c, p, 6, i, 3)) return nullptr;
+    if (!parse(env, info, &c, p, 6, i, 3, true)) return nullptr;
     if (check(env, c, brik_moe_combine_grad(c, (const float*)p[0], (const float*)p[1], (const int32_t*)p[2], (const float*)p[3], (float*)p[4],
                                             (float*)p[5], i[0], i[1], i[2])))
         return nullptr;
@@ -103,7 +103,7 @@ napi_value QuantizeI8(napi_env env, napi_callback_info info)   // (ctx, {x, code
 napi_value MatmulI8(napi_env env, napi_callback_info info)   // (ctx, x, xScales, w, wScales, res, y, M, K, N)
 {
     brik_ctx* c; void* p[6]; int32_t i[3];
-    if (!parse(env, info, &c, p, 6, i, 3)) return nullptr;
+    if (!parse(env, info, &c, p, 6, i, 3, true)) return nullptr;
     if (check(env, c, brik_matmul_t_i8(c, (const int8_t*)p[0], (const float*)p[1], (const int8_t*)p[2], (const float*)p[3], (const float*)p[4],
                                        (float*)p[5], i[0], i[1], i[2])))
         return nullptr;
@@ -114,7 +114,7 @@ napi_value MatmulI8(napi_env env, napi_callback_info info)   // (ctx, x, xScales
 napi_value MoeMatmulI8(napi_env env, napi_callback_info info)
 {
     brik_ctx* c; void* p[7]; int32_t i[6];
-    if (!parse(env, info, &c, p, 7, i, 6)) return nullptr;
+    if (!parse(env, info, &c, p, 7, i, 6, true)) return nullptr;
     if (check(env, c, brik_moe_matmul_t_i8(c, (const int8_t*)p[0], (const float*)p[1], i[0], (const int32_t*)p[2], i[1], (const int32_t*)p[3],
                                            (const int8_t*)p[4], (const float*)p[5], (float*)p[6], i[2], i[3], i[4], i[5])))
         return nullptr;
