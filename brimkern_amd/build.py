@@ -9,9 +9,9 @@
    ``libbrik.so`` (the C ABI declared in ``include/brik.h``)
 4. ``csrc/brik_napi.cc`` -> ``js/brik.node`` (Node N-API addon over libbrik.so, rpath $ORIGIN/..), and
    ``csrc/brik_napi_experts.cc`` -> ``js/brik_experts.node`` (experts, 8-bit products)
-5. ``tests/native/host_sanitize.cpp`` and ``attn_sanitize.cpp`` + the runtime sources, host code built with AddressSanitizer
-   and UndefinedBehaviorSanitizer -> ``tests/native/host_sanitize``, ``attn_sanitize`` (test drivers, not part of the
-   library; skipped when g++ cannot link the sanitizer runtimes)
+5. ``tests/native/host_sanitize.cpp``, ``attn_sanitize.cpp`` and ``experts_sanitize.cpp`` + the runtime sources, host code built
+   with AddressSanitizer and UndefinedBehaviorSanitizer -> ``tests/native/host_sanitize``, ``attn_sanitize``,
+   ``experts_sanitize`` (test drivers, not part of the library; skipped when g++ cannot link the sanitizer runtimes)
 
 Run ``python -m brimkern_amd.build`` or call :func:`build`.
 """
@@ -37,7 +37,7 @@ SCRATCH_OBJ = os.path.join(BUILD, "brik_scratch.o")
 LIB = os.path.join(PKG, "libbrik.so")
 ADDON = os.path.join(PKG, "js", "brik.node")
 EXPERTS_ADDON = os.path.join(PKG, "js", "brik_experts.node")
-SANITIZE_BINS = [os.path.join(ROOT, "tests", "native", n) for n in ("host_sanitize", "attn_sanitize")]
+SANITIZE_BINS = [os.path.join(ROOT, "tests", "native", n) for n in ("host_sanitize", "attn_sanitize", "experts_sanitize")]
 
 # Device flags. packed-fp32-ops is switched off: the compiler would otherwise fuse pairs of f32
 # operations into v_pk_* forms.
@@ -120,7 +120,7 @@ def _build_addon(name, out, verbose):
 
 def build_host_sanitize(verbose=False):
     """The runtime's host code with ASan + UBSan (g++, host only; the kernels stay the ordinary code object), linked with the
-    drivers that exercise the entry points (tests/test_host_sanitize.py, tests/test_attn_sanitize.py)."""
+    drivers that exercise the entry points (tests/test_host_sanitize.py, test_attn_sanitize.py, test_experts_sanitize.py)."""
     with concurrent.futures.ThreadPoolExecutor(len(SANITIZE_BINS)) as pool:
         return list(pool.map(lambda out: _build_sanitize(out, verbose), SANITIZE_BINS))
 
