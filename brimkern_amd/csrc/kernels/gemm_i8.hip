@@ -92,11 +92,11 @@ __device__ __forceinline__ int x_row(const brik_i8_launch& a, int m)
 
 constexpr int FEW_S = 8;         // 64-byte steps of K that a wave holds at once
 
-// MB: 16 rows each at a time, CB: 16 channels each, NW waves.
-template <int MB, int CB, int NW>
+// MB: 16 rows each at a time, by NW waves.
+template <int MB, int NW>
 __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
 {
-    constexpr int C = 16 * CB, R = 16 * MB, LD = C + 1;
+    constexpr int C = 16, R = 16 * MB, LD = C + 1;
     __shared__ int red[R * LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), i16 = lane & 15, q = lane >> 4;
     int id = blockIdx.x;
@@ -114,10 +114,8 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
     const int n0 = ct * C, K = a.K;
     const int steps = (K + 63) >> 6, s0 = split * a.steps, s1 = min(steps, s0 + a.steps);
     const int pieces = (s1 - s0 + NW * FEW_S - 1) / (NW * FEW_S), per = (s1 - s0 + NW * pieces - 1) / (NW * pieces);
-    const int8_t* wr[CB];
-#pragma unroll
-    for (int c = 0; c < CB; ++c) wr[c] = r.w + (size_t)min(n0 + 16 * c + i16, a.N - 1) * K;
-    i32x4_t w[CB][FEW_S];
+    const int8_t* const wr = r.w + (size_t)min(n0 + i16, a.N - 1) * K;
+    i32x4_t w[FEW_S];
     for (int m = r.m0; m < r.m1; m += R) {
         const int8_t* xr[MB];
 #pragma unroll
@@ -125,21 +123,15 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
             const int mine = m + 16 * b + i16, row = mine < r.m1 ? x_row(a, mine) : -1;
             xr[b] = row < 0 ? nullptr : a.x + (size_t)row * K;
         }
-        i32x4_t acc[MB][CB];
+        i32x4_t acc[MB];
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
-#pragma unroll
-            for (int c = 0; c < CB; ++c) acc[b][c] = i32x4_t{0, 0, 0, 0};
+        for (int b = 0; b < MB; ++b) acc[b] = i32x4_t{0, 0, 0, 0};
         for (int p = 0; p < pieces; ++p) {
             const int first = s0 + (p * NW + wave) * per, count = min(per, s1 - first);
             if (pieces > 1 || m == r.m0) {
 #pragma unroll
                 for (int s = 0; s < FEW_S; ++s)
-                    if (s < count) {
-                        const int k = min(64 * (first + s) + 16 * q, K - 16);
-#pragma unroll
-                        for (int c = 0; c < CB; ++c) w[c][s] = *(const i32x4_t*)(wr[c] + k);
-                    }
+                    if (s < count) w[s] = *(const i32x4_t*)(wr + min(64 * (first + s) + 16 * q, K - 16));
             }
 #pragma unroll
             for (int s = 0; s < FEW_S; ++s)
@@ -152,9 +144,7 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
                         if (xr[b] && k < K) x[b] = *(const i32x4_t*)(xr[b] + k);
                     }
 #pragma unroll
-                    for (int b = 0; b < MB; ++b)
-#pragma unroll
-                        for (int c = 0; c < CB; ++c) acc[b][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[c][s], x[b], acc[b][c], 0, 0, 0);
+                    for (int b = 0; b < MB; ++b) acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[s], x[b], acc[b], 0, 0, 0);
                 }
         }
         for (int i = tid; i < R * LD; i += 64 * NW) red[i] = 0;
@@ -162,9 +152,7 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
 #pragma unroll
         for (int b = 0; b < MB; ++b)
 #pragma unroll
-            for (int c = 0; c < CB; ++c)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) atomicAdd(&red[(16 * b + i16) * LD + 16 * c + 4 * q + v], acc[b][c][v]);
+            for (int v = 0; v < 4; ++v) atomicAdd(&red[(16 * b + i16) * LD + 4 * q + v], acc[b][v]);
         __syncthreads();
         for (int i = tid; i < R * C; i += 64 * NW) {
             const int t = i / C, c = i - t * C, row = m + t, n = n0 + c;
@@ -187,17 +175,17 @@ __device__ __forceinline__ void i8_few(const brik_i8_launch& a)
 // ---- tiles -----------------------------------------------------------------------------------------
 
 // WR x WC waves, each WA x WB blocks of 32 x 32; BK of K a step, double-buffered.
-template <int WR_, int WC_, int WA_, int WB_, int BK_, int AHEAD_, int FD_>
+template <int WR_, int WC_, int WA_, int WB_, int AHEAD_, int FD_>
 struct I8Tile {
-    static constexpr int WR = WR_, WC = WC_, WA = WA_, WB = WB_, BK = BK_, AHEAD = AHEAD_, FD = FD_;
+    static constexpr int WR = WR_, WC = WC_, WA = WA_, WB = WB_, BK = 128, AHEAD = AHEAD_, FD = FD_;
     static constexpr int NT = 64 * WR * WC, BM = 32 * WR * WA, BN = 32 * WC * WB;
     static constexpr int CH = BK / 16, ROWS = NT / CH;           // 16-byte chunks of a row, rows that the block loads at once
     static constexpr int CX = BM / ROWS, CW = BN / ROWS;         // chunks of a thread and step
     static constexpr int BUF = (BM + BN) * BK, H = BK / 32;
-    static_assert(BM % ROWS == 0 && BN % ROWS == 0 && ROWS % 32 == 0 && (BK == 64 || BK == 128), "whole chunks");
+    static_assert(BM % ROWS == 0 && BN % ROWS == 0 && ROWS % 32 == 0, "whole chunks");
     // Chunk c of row r lies at c ^ turn(r): a column of chunks is read in groups of the rows 4 a .. 4 a + 3 and 4 (a ^ 5) .. 4 (a ^ 5) + 3,
     // which then meet every bank once (no conflicts counted).
-    static __device__ __forceinline__ int turn(int r) { return BK == 128 ? (r & 7) ^ ((r >> 3) & 1) : ((r >> 1) & 1) | ((r >> 3) & 2); }
+    static __device__ __forceinline__ int turn(int r) { return (r & 7) ^ ((r >> 3) & 1); }
 };
 
 // Loads past `bytes` give zeros.
@@ -422,31 +410,31 @@ __device__ __forceinline__ void i8_tile(const brik_i8_launch& a)
 
 }  // namespace
 
-#define BRIK_I8_FEW(MB, CB, NW) \
-    extern "C" __global__ __launch_bounds__(64 * NW) void brik_i8_few_##MB##_##CB##_##NW(brik_i8_launch a) { i8_few<MB, CB, NW>(a); }
-BRIK_I8_FEW(1, 1, 4)
-BRIK_I8_FEW(1, 1, 8)
-BRIK_I8_FEW(2, 1, 8)
-BRIK_I8_FEW(1, 1, 16)
-BRIK_I8_FEW(2, 1, 16)
+#define BRIK_I8_FEW(MB, NW) \
+    extern "C" __global__ __launch_bounds__(64 * NW) void brik_i8_few_##MB##_##NW(brik_i8_launch a) { i8_few<MB, NW>(a); }
+BRIK_I8_FEW(1, 4)
+BRIK_I8_FEW(1, 8)
+BRIK_I8_FEW(2, 8)
+BRIK_I8_FEW(1, 16)
+BRIK_I8_FEW(2, 16)
 
-#define BRIK_I8_TILE(NAME, WR, WC, WA, WB, BK, AHEAD, FD, OCC)                                                  \
-    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##NAME(brik_i8_launch a)         \
-    {                                                                                                           \
-        i8_tile<I8Tile<WR, WC, WA, WB, BK, AHEAD, FD>, false>(a);                                               \
+#define BRIK_I8_TILE(NAME, WR, WC, WA, WB, AHEAD, FD, OCC)                                                    \
+    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_tile_##NAME(brik_i8_launch a)     \
+    {                                                                                                         \
+        i8_tile<I8Tile<WR, WC, WA, WB, AHEAD, FD>, false>(a);                                                 \
     }
-#define BRIK_I8_MOE(NAME, WR, WC, WA, WB, BK, AHEAD, FD, OCC)                                                   \
-    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_moe_##NAME(brik_i8_launch a)          \
-    {                                                                                                           \
-        i8_tile<I8Tile<WR, WC, WA, WB, BK, AHEAD, FD>, true>(a);                                                \
+#define BRIK_I8_MOE(NAME, WR, WC, WA, WB, AHEAD, FD, OCC)                                                     \
+    extern "C" __global__ __launch_bounds__(64 * WR * WC, OCC) void brik_i8_moe_##NAME(brik_i8_launch a)      \
+    {                                                                                                         \
+        i8_tile<I8Tile<WR, WC, WA, WB, AHEAD, FD>, true>(a);                                                  \
     }
-BRIK_I8_TILE(256x256, 2, 2, 4, 4, 128, 1, 1, 1)
-BRIK_I8_TILE(256x128, 2, 2, 4, 2, 128, 2, 2, 1)
-BRIK_I8_TILE(128x128, 2, 2, 2, 2, 128, 2, 2, 2)
-BRIK_I8_TILE(64x128, 2, 2, 1, 2, 128, 2, 2, 2)
-BRIK_I8_MOE(256x256, 2, 2, 4, 4, 128, 1, 1, 1)
-BRIK_I8_MOE(128x128, 2, 2, 2, 2, 128, 2, 2, 2)
-BRIK_I8_MOE(64x128, 2, 2, 1, 2, 128, 2, 2, 3)
+BRIK_I8_TILE(256x256, 2, 2, 4, 4, 1, 1, 1)
+BRIK_I8_TILE(256x128, 2, 2, 4, 2, 2, 2, 1)
+BRIK_I8_TILE(128x128, 2, 2, 2, 2, 2, 2, 2)
+BRIK_I8_TILE(64x128, 2, 2, 1, 2, 2, 2, 2)
+BRIK_I8_MOE(256x256, 2, 2, 4, 4, 1, 1, 1)
+BRIK_I8_MOE(128x128, 2, 2, 2, 2, 2, 2, 2)
+BRIK_I8_MOE(64x128, 2, 2, 1, 2, 2, 2, 3)
 
 // The splits' sums and the scaling: a thread per four neighbours of y.
 extern "C" __global__ __launch_bounds__(256) void brik_i8_join(brik_i8_launch a)

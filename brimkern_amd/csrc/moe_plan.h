@@ -35,9 +35,9 @@ struct I8Kernel {
     const char* name;
 };
 constexpr I8Kernel kI8Kernels[] = {
-    {I8_FEW, 16, 16, 256, "brik_i8_few_1_1_4"},       {I8_FEW, 16, 16, 512, "brik_i8_few_1_1_8"},
-    {I8_FEW, 32, 16, 512, "brik_i8_few_2_1_8"},       {I8_FEW, 16, 16, 1024, "brik_i8_few_1_1_16"},
-    {I8_FEW, 32, 16, 1024, "brik_i8_few_2_1_16"},     {I8_TILE, 256, 256, 256, "brik_i8_tile_256x256"},
+    {I8_FEW, 16, 16, 256, "brik_i8_few_1_4"},       {I8_FEW, 16, 16, 512, "brik_i8_few_1_8"},
+    {I8_FEW, 32, 16, 512, "brik_i8_few_2_8"},       {I8_FEW, 16, 16, 1024, "brik_i8_few_1_16"},
+    {I8_FEW, 32, 16, 1024, "brik_i8_few_2_16"},     {I8_TILE, 256, 256, 256, "brik_i8_tile_256x256"},
     {I8_TILE, 256, 128, 256, "brik_i8_tile_256x128"}, {I8_TILE, 128, 128, 256, "brik_i8_tile_128x128"},
     {I8_TILE, 64, 128, 256, "brik_i8_tile_64x128"},   {I8_MOE, 256, 256, 256, "brik_i8_moe_256x256"},
     {I8_MOE, 128, 128, 256, "brik_i8_moe_128x128"},   {I8_MOE, 64, 128, 256, "brik_i8_moe_64x128"},
