@@ -76,7 +76,8 @@ def build_attn_hsaco(verbose=False):
 
 
 def build_moe_hsaco(verbose=False):
-    return _genco("brik_moe_kernels.hip", MOE_HSACO, [], verbose)
+    # (plain "fast" fuses products and sums past a pragma that forbids it)
+    return _genco("brik_moe_kernels.hip", MOE_HSACO, ["-ffp-contract=fast-honor-pragmas"], verbose)
 
 
 def build_scratch(verbose=False):

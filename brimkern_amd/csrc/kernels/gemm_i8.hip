@@ -33,11 +33,10 @@ __device__ __forceinline__ void lds_barrier()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// A product and what is added to it, a rounding of its own whatever kernel computes it: the build lets products and sums fuse, so the
-// product passes out of the compiler's sight between.
+// A product and what is added to it, a rounding of its own whatever kernel computes it (elsewhere the build lets products and sums fuse).
 __device__ __forceinline__ float plus(float y, float res)
 {
-    asm("" : "+v"(y));
+#pragma clang fp contract(off)
     return y + res;
 }
 
