@@ -2,16 +2,18 @@
 //
 //   y_mn = (sum_k x_mk w_nk) ws_n xs_m (+ res_mn), the sum exact in int32
 //
-// Integer sums have no order, so K may be split over waves and blocks freely: results are the same bits. Two kernels:
+// Integer sums have no order and every rounding after them is one of its own, so K may be split over waves and blocks freely: results are
+// the same bits, whichever kernel computes them. Two kernels:
 //   few rows (decoding, experts of few tokens): bound by the bytes of w and by latency. A block has 16 channels; its 4 to 16 waves split
 //     K, and a wave loads all of its part of w at once, into registers, and multiplies it with 16 or 32 rows of x after the other. 1 row of
 //     2560 x 9728 7.7 us (3.2 TB/s, a launch among them), of 9728 x 2560 8.9; 24 rows of 4096 x 2561 7.6.
 //   tiles (prompts): bound by the matrix cores. Both operands go through LDS, 128 of K a step, double-buffered, the loads of the next
 //     step (256 x 256) or of the next two in registers meanwhile. 8192^3 492 us, 2.2 POP/s (the card's library 2.1; the clock falls
-//     under this load); 8192 x 9728 x 2560 218 (library 202); 512 x 2560 x 9728 21 to 22 (library 38), where loads through the
-//     vector-memory path, some 22 clocks a KiB, take as long as the products, so tiles of 256 x 128, which load least, are fastest. By experts, 64
-//     of them, 8 a token: 256 tokens by 2048 x 1536 50 (201 MB of w, 4.0 TB/s), 4096 by 768 x 2048 141 to 145 (268 MB of y, 2.8 TB/s in all:
-//     a tile has 6 steps between its loads' start and its stores).
+//     under this load); 8192 x 9728 x 2560 218 (library 202); 512 x 2560 x 9728 21 to 22 with w in the last-level cache, 26 from memory (library
+//     38), where loads through the vector-memory path, some 22 clocks a KiB, take as long as the products, so tiles of 256 x 128, which load least,
+//     are fastest. By experts, 64 of them, 8 a token: 256 tokens by 2048 x 1536 51 (201 MB of w, 4.2 TB/s), 4096 by 768 x 2048 145 (268 MB of y,
+//     2.7 TB/s in all: a tile has 6 steps between its loads' start and its stores), 8192 by 2048 x 1536 318 (1.3 POP/s: the experts' last tiles are
+//     part filled, and brik_i8_moe_256x256 has two registers more than there are, so its loop reads 12 bytes a lane from scratch).
 #include "attn_common.h"
 #include "moe_abi.h"
 
@@ -435,7 +437,7 @@ BRIK_I8_MOE(256x256, 2, 2, 4, 4, 1, 1, 1)
 BRIK_I8_MOE(128x128, 2, 2, 2, 2, 2, 2, 2)
 BRIK_I8_MOE(64x128, 2, 2, 1, 2, 2, 2, 3)
 
-// The splits' sums and the scaling: a thread per four neighbours of y.
+// The splits' sums and the scaling: a thread takes one value of y at a time.
 extern "C" __global__ __launch_bounds__(256) void brik_i8_join(brik_i8_launch a)
 {
     const size_t all = (size_t)a.M * a.N;

@@ -13,9 +13,11 @@
 // a second launch adds up the counts of the chunks before its own and writes the rows. Few assignments are routed and sorted
 // by one block.
 //
-// Bound by latency and vector instructions, not by bytes: 64 tokens of 64 experts, 8 each, 4.4 us, sorted 7.2; 16384 of 64 12; of 256 with a
-// bias 15 (73 % of the cycles issue vector instructions; the last waves are those of tokens taken again in 64 bits, 3 to 4 us each), sorted 26.
-// The gradient of 4096 tokens of 64 experts 5 us.
+// Bound by latency and vector instructions, not by bytes: 64 tokens of 64 experts, 8 each, 4.4 us, sorted 7.2; 16384 of them 4.9, sorted 11.8;
+// 64 of 256 experts with a bias 11.7, 16384 of them 15.6 to 17 (73 % of the cycles issue vector instructions; the last waves are those of tokens taken
+// again in 64 bits, one after the other, 3 to 4 us each), sorted 26 to 27. Assignments alone: 1024 sorted in 4.3 us by one block, 4096 in 7.8, 8192
+// in 7.4 by two launches, 131072 in 8.6. The gradient of 4096 tokens of 64 experts 5 us. By whole waves with a bias, 16 experts a lane, 84 bytes a
+// lane lie in scratch (1024 threads a block leave 128 registers).
 #include "attn_common.h"
 #include "moe_abi.h"
 

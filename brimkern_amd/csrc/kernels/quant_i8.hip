@@ -4,9 +4,10 @@
 // up to 4096 or 16384, longer ones are read again. The values go in f32 first, which without a gate is exact; with one, SiLU is within
 // 2^-21 of itself. What depends on the last bits is then done in 64: the maximum among the values next to the f32 one, and the codes
 // whose f32 quotient lies nearer to a border than its error. A row with values that f32 does not hold to 2^-21 (gates below -64 or
-// subnormal, overflow, NaN) and one under GELU take 64 bits throughout. Bound by memory: 4 bytes read a value (8 with a gate), one written.
-// 8192 x 9728 84 us, 4.75 TB/s, vector instructions in 79 % of the cycles; with a gate 32768 x 768 55 us, 4.15 TB/s and 84 %; 512 x 2560
-// 4 us and one row 3, a launch's latency.
+// subnormal, overflow, NaN) and one under GELU take 64 bits throughout. 4 bytes are read a value (8 with a gate), one written: without a gate
+// memory bounds it, 8192 x 9728 84 us, 4.75 TB/s, vector instructions in 79 % of the cycles. With one vector instructions do: under SiLU
+// 32768 x 768 55 us, 4.1 TB/s and 84 %, 8192 x 9728 251 us (2.9 TB/s); under GELU, two exponentials of 64 bits a value, 121 and 474 us.
+// 512 x 2560 4 us and one row 3, a launch's latency.
 #include "attn_common.h"
 #include "moe_abi.h"
 

@@ -8,7 +8,7 @@
 
 namespace brik_plan {
 
-// Chunks of a routing or sorting call: one block of all assignments where they are few, else as many as BRIK_MOE_CHUNKS.
+// Chunks of a routing or sorting call: one block of all assignments where they are few (`alone`), else as many as BRIK_MOE_CHUNKS.
 inline void moe_chunks(brik_route_launch& a, int alone)
 {
     const long n = (long)a.r.tokens * a.r.k;
@@ -101,10 +101,16 @@ inline int i8_dense(brik_i8_launch& a, int forced, int splits)
     return best;
 }
 
-// The kernel of a product by experts, by the mean of their rows. 64 experts, 8 a token, 2048 x 1536 and 768 x 2048 (us): 8 tokens few
-// 31 and 16, 64-row tiles 37 and 22, 128-row 44 and 28; 32 tokens 41 and 25, 40 and 25, 48 and 32; 256 tokens 66 and 38 (128 tokens),
-// 50 and 29, 52 and 35; 1024 tokens 79 and 55 by 64 rows, 78 and 57 by 128;
-// 8192 tokens by 2048 x 1536 374 by 64, 332 by 128, 322 by 256.
+// The kernel of a product by experts, by the mean of their rows (all rows count, those without an expert too: how many there are stays on
+// the device). 64 experts, 8 a token, 2048 x 1536 and 768 x 2048 (us; 256 and 1024 tokens the first alone, 4096 the second; up to 4 tokens
+// with the weights in the last-level cache):
+//   tokens      1           2           4           8           16          32          256         1024       4096   8192
+//   few         9.8   6.7   13.4  8.4   22.4  12.4  31.0  16.3  35.9  20.7  40.5  24.7
+//   64 rows     9.1   6.1   12.5  9.3   20.7  13.7  36.1  21.3  37.7  22.4  39.6  24.4  51.1        77.9           156  366   281
+//   128 rows    12.0  7.6               25.3  18.4  43.5  27.6              47.2  31.9  52.9        78.1           145  326   254
+//   256 rows                                                                                        114            143  319   236
+// So few rows are right from 8 tokens to 16 and cost up to 9 % at 1 to 4, which the mean cannot tell from 8; with 256 experts, where few rows
+// start a block for each, one token takes 15.2 against 9.8 by 64 rows, 8 tokens 36.7 against 38.5. K < 1024 keeps 128 rows, 2 to 8 % behind 256.
 inline int i8_experts(brik_i8_launch& a, int forced)
 {
     a.splits = 1;

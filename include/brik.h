@@ -467,7 +467,9 @@ int brik_attention(brik_ctx *ctx, const brik_kv_cache *cache, const brik_kv_batc
  *            logit (or sum) of -infinity or NaN is never chosen: where fewer are left the others are -1
  *   weights  scale * s of the chosen ones (without the bias), with BRIK_ROUTE_RENORM divided by their sum; 0 for id -1
  * A token all of whose logits are -infinity (padding) so goes nowhere. A NaN logit counts as -infinity; +infinity gives a
- * softmax of NaN. row_off, src and slot: all three, and the assignments are sorted by the same call, or none.
+ * softmax of NaN. A weight is off by at most (2.3 d + 44) 2^-24 of itself and 2^-125 of scale, d how far its logit lies below the token's
+ * largest (with RENORM the largest chosen; a sigmoid alone: below 0). row_off, src and slot: all three, and the assignments are sorted by
+ * the same call, or none.
  * tokens below 2^24, tokens * k at most 2^30, experts at most BRIK_MOE_EXPERTS, k at most BRIK_MOE_K and at most experts. Logits are 4-byte aligned,
  * [tokens, experts] with a row every logit_stride values (0: packed). Workspace: at most 1 MiB, taken once. */
 #define BRIK_MOE_EXPERTS 1024
@@ -490,7 +492,7 @@ int brik_moe_route(brik_ctx *ctx, const brik_moe_route_args *args);
 
 /* dlogits [tokens, experts] (packed) of a call of brik_moe_route whose weights have the gradient dweights [tokens, k]; ids are
  * read as that call left them, weights and the sorted arrays are not looked at. The choice itself and the bias have no
- * gradient. */
+ * gradient. (This and brik_moe_combine_grad are for a layer whose experts' own backward pass is the caller's: no product here has one.) */
 int brik_moe_route_grad(brik_ctx *ctx, const brik_moe_route_args *args, const float *dweights, float *dlogits);
 
 /* row_off, src and slot of ids [tokens, k] that come from elsewhere. */
@@ -524,7 +526,8 @@ int brik_moe_combine_grad(brik_ctx *ctx, const float *dout, const float *y_sorte
  *   scales[m] = the f32 nearest max|h[m]| / 127,   codes = floor(h / scale + 1/2)
  * in exact arithmetic (ties upward, as the .brik encoders), within [-127, 127]. A row whose scale would be below 2^-126 gets scale 0
  * and codes 0; a row with a NaN or an infinity gets scale NaN and codes 0, so that its products are NaN. Rows of x and gate
- * every *_stride values (0: packed; multiples of 4), 16-byte aligned; M below 2^22. */
+ * every *_stride values (0: packed; multiples of 4), 16-byte aligned; M below 2^22 (weights of more channels, of all experts together, by
+ * several calls). */
 int brik_quantize_i8(brik_ctx *ctx, const float *x, int64_t x_stride, const float *gate, int64_t gate_stride, int flags,
                      int8_t *codes, float *scales, int M, int K);
 
