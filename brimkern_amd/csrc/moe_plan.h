@@ -35,9 +35,9 @@ struct I8Kernel {
     const char* name;
 };
 constexpr I8Kernel kI8Kernels[] = {
-    {I8_FEW, 16, 16, 256, "brik_i8_few_1_4"},       {I8_FEW, 16, 16, 512, "brik_i8_few_1_8"},
-    {I8_FEW, 32, 16, 512, "brik_i8_few_2_8"},       {I8_FEW, 16, 16, 1024, "brik_i8_few_1_16"},
-    {I8_FEW, 32, 16, 1024, "brik_i8_few_2_16"},     {I8_TILE, 256, 256, 256, "brik_i8_tile_256x256"},
+    {I8_FEW, 16, 16, 256, "brik_i8_few_1_4"},         {I8_FEW, 16, 16, 512, "brik_i8_few_1_8"},
+    {I8_FEW, 32, 16, 512, "brik_i8_few_2_8"},         {I8_FEW, 16, 16, 1024, "brik_i8_few_1_16"},
+    {I8_FEW, 32, 16, 1024, "brik_i8_few_2_16"},       {I8_TILE, 256, 256, 256, "brik_i8_tile_256x256"},
     {I8_TILE, 256, 128, 256, "brik_i8_tile_256x128"}, {I8_TILE, 128, 128, 256, "brik_i8_tile_128x128"},
     {I8_TILE, 64, 128, 256, "brik_i8_tile_64x128"},   {I8_MOE, 256, 256, 256, "brik_i8_moe_256x256"},
     {I8_MOE, 128, 128, 256, "brik_i8_moe_128x128"},   {I8_MOE, 64, 128, 256, "brik_i8_moe_64x128"},
@@ -109,8 +109,11 @@ inline int i8_dense(brik_i8_launch& a, int forced, int splits)
 //   64 rows     9.1   6.1   12.5  9.3   20.7  13.7  36.1  21.3  37.7  22.4  39.6  24.4  51.1        77.9           156  366   281
 //   128 rows    12.0  7.6               25.3  18.4  43.5  27.6              47.2  31.9  52.9        78.1           145  326   254
 //   256 rows                                                                                        114            143  319   236
-// So few rows are right from 8 tokens to 16 and cost up to 9 % at 1 to 4, which the mean cannot tell from 8; with 256 experts, where few rows
+// and by 2048 x 1536 alone 512 tokens 61.2 by 64 rows, 63.7 by 128; 2048 tokens 128, 116, 128 by 256; 4096 215, 193, 209; 6144 268, 264 (128, 256).
+// So few rows are right from 8 tokens to 16 and cost up to 11 % at 1 to 4, which the mean cannot tell from 8; with 256 experts, where few rows
 // start a block for each, one token takes 15.2 against 9.8 by 64 rows, 8 tokens 36.7 against 38.5. K < 1024 keeps 128 rows, 2 to 8 % behind 256.
+// Waves of a few-row block, 4, 8, 16, 8 tokens: 1024 x 2048 22.9, 31.7, 54.0; 2048 x 1536 31.1, 34.9, 47.7; 4096 x 1024 45.2, 39.1, 45.8; 8192 x 512
+// 43.0, 43.4, 40.3.
 inline int i8_experts(brik_i8_launch& a, int forced)
 {
     a.splits = 1;
